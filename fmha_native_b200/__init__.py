@@ -14,6 +14,11 @@ Host-side mirror of the poyenc/fmha_native operator surface:
 * :func:`fmha_fwd` -- a convenience call over torch CUDA tensors that builds
   the params from tensor strides and calls the C ABI.
 
+The serving operators (rotary positions, the paged K/V cache, attention over
+it and under a shared prefix) live in :mod:`fmha_native_b200.paged` and are
+reached as ``fmha_native_b200.rope``, ``paged_append``, ``paged_fwd``,
+``prefix_fwd`` and so on.
+
 There is no CPU fallback: every compute call goes through the CUDA library
 and raises :class:`FmhaError` if it is missing or fails.
 """
@@ -39,6 +44,7 @@ FMHA_ERR_LAUNCH = 2
 FMHA_ERR_TIMEOUT = 3
 FMHA_ERR_DEVICE = 4
 FMHA_ERR_SCRATCH = 5
+FMHA_ERR_INDEX = 6
 
 ENTRY_POINTS = (
     "fmha_fwd_d64_bf16_msk0",
@@ -55,6 +61,11 @@ ENTRY_POINTS = (
     "fmha_fwd_d64_set_wait_limit_ns",
     "fmha_fwd_d64_release",
     "fmha_fwd_d64_error_string",
+    "fmha_rope_d64_bf16",
+    "fmha_paged_append_d64_bf16",
+    "fmha_paged_workspace_bytes",
+    "fmha_paged_fwd_d64_bf16",
+    "fmha_prefix_fwd_d64_bf16",
 )
 
 
@@ -134,6 +145,13 @@ def load_library(path: str = LIB_PATH) -> ctypes.CDLL:
     lib.fmha_fwd_d64_error_string.restype = ctypes.c_char_p
     lib.fmha_fwd_d64_debug_set_stall.argtypes = [ctypes.c_int]
     lib.fmha_fwd_d64_debug_set_stall.restype = None
+    for name in ("fmha_rope_d64_bf16", "fmha_paged_append_d64_bf16", "fmha_paged_fwd_d64_bf16",
+                 "fmha_prefix_fwd_d64_bf16"):
+        fn = getattr(lib, name)
+        fn.argtypes = [ctypes.c_char_p, ctypes.c_void_p]  # the packed parameter block, the stream
+        fn.restype = ctypes.c_int
+    lib.fmha_paged_workspace_bytes.argtypes = [ctypes.c_int] * 6
+    lib.fmha_paged_workspace_bytes.restype = ctypes.c_size_t
     _lib = lib
     return lib
 
@@ -141,7 +159,8 @@ def load_library(path: str = LIB_PATH) -> ctypes.CDLL:
 def error_string(status: int) -> str:
     names = {0: "ok", 1: "invalid argument", 2: "CUDA launch or runtime error",
              3: "device pipeline wait exceeded its time limit", 4: "no supported sm_100 device",
-             5: "request exceeds the allocation-free scratch"}
+             5: "request exceeds the allocation-free scratch",
+             6: "a page id, length, position or prefix sum on the device was out of range"}
     return names.get(status, "unknown status")
 
 
@@ -424,3 +443,18 @@ def fmha_fwd_from_host(q, k, v, causal: bool = False, layout: str = "bshd", out=
 
 
 _host_state: dict = {}
+
+#: Names of fmha_native_b200.paged that are reached from here (that module needs
+#: torch, which importing this package alone does not).
+_PAGED = ("FmhaRopeParams", "FmhaPagedParams", "rope_table", "rope", "rope_bwd", "paged_append", "paged_fwd",
+          "paged_workspace_bytes", "prefix_fwd")
+
+
+def __getattr__(name: str):
+    if name in _PAGED:
+        from . import paged
+
+        for n in _PAGED:
+            globals()[n] = getattr(paged, n)
+        return globals()[name]
+    raise AttributeError(f"module {__name__!r} has no attribute {name!r}")

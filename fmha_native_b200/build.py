@@ -18,10 +18,10 @@ REPO_DIR = os.path.dirname(PKG_DIR)
 CSRC = os.path.join(PKG_DIR, "csrc")
 LIB_PATH = os.path.join(PKG_DIR, "libfmha_b200.so")
 
-SOURCES = [os.path.join(CSRC, "fmha_fwd_kernel.cu")]
+SOURCES = [os.path.join(CSRC, f) for f in ("fmha_fwd_kernel.cu", "fmha_rope.cu", "fmha_paged.cu")]
 DEPS = SOURCES + [
-    os.path.join(CSRC, "sm100_ptx.cuh"),
-    os.path.join(REPO_DIR, "include", "fmha_fwd.h"),
+    *(os.path.join(CSRC, f) for f in ("sm100_ptx.cuh", "host_context.h", "paged_common.cuh", "paged_rows.cuh")),
+    *(os.path.join(REPO_DIR, "include", f) for f in ("fmha_fwd.h", "fmha_paged.h")),
 ]
 
 ARCH_FLAGS = ["-gencode", "arch=compute_100a,code=sm_100a"]

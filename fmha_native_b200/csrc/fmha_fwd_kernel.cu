@@ -65,6 +65,7 @@
 #include <vector>
 
 #include "../../include/fmha_fwd.h"
+#include "host_context.h"
 #include "sm100_ptx.cuh"
 
 using namespace fmha_sm100;
@@ -119,7 +120,8 @@ constexpr float kPLog2Bias = 0.0040614f;
 #endif
 constexpr int kExpPolyPairs = FMHA_EXP_POLY_PAIRS;
 
-// Error codes written to the device error word.
+// Error codes written to the device error word (host_context.h has the paged
+// operators' ones).
 constexpr int kErrTimeoutLoad = 0x101;
 constexpr int kErrTimeoutMma = 0x102;
 constexpr int kErrTimeoutSoftmax = 0x103;
@@ -1443,6 +1445,21 @@ int launch(const FmhaFwdParams* p, int batch, bool causal, bool varlen, int tota
 
 }  // namespace
 
+// What the paged operators' launchers share with this file.
+int fmha_host::acquire(Context* out) {
+    int dev = 0;
+    if (cudaGetDevice(&dev) != cudaSuccess) return FMHA_ERR_DEVICE;
+    DeviceContext* ctx = nullptr;
+    const int st = ensure_context(dev, &ctx);
+    if (st != FMHA_OK) return st;
+    std::lock_guard<std::mutex> lock(g_mutex);
+    out->device = dev;
+    out->err_word = ctx->err_word;
+    out->encode = g_encode;
+    out->wait_limit_ns = g_wait_limit_ns;
+    return FMHA_OK;
+}
+
 // ============================================ allocation-free variant (host)
 //
 // For callers that may not allocate device memory themselves -- for example
@@ -1676,7 +1693,7 @@ int fmha_fwd_d64_status(CUstream_st* stream) {
         return FMHA_ERR_LAUNCH;
     if (h != 0) {
         cudaMemset(word, 0, sizeof(int));
-        return FMHA_ERR_TIMEOUT;
+        return h == fmha_host::kErrIndex ? FMHA_ERR_INDEX : FMHA_ERR_TIMEOUT;
     }
     return FMHA_OK;
 }
@@ -1727,6 +1744,8 @@ const char* fmha_fwd_d64_error_string(int status) {
         case FMHA_ERR_DEVICE: return "no supported sm_100 device";
         case FMHA_ERR_SCRATCH:
             return "work list longer than the allocation-free entry's scratch (16384 blocks)";
+        case FMHA_ERR_INDEX:
+            return "a page id, length, position or prefix sum on the device was out of range";
         default: return "unknown status";
     }
 }

@@ -1,0 +1,204 @@
+// paged_common.cuh -- what the kernels over the paged K/V cache share: their
+// arguments, the addressing of query rows, bounded waits and the folding of
+// partial softmax results.
+#pragma once
+#include <cuda.h>
+#include <cuda_runtime.h>
+
+#include <cstdint>
+
+#include "host_context.h"
+#include "sm100_ptx.cuh"
+
+namespace fmha_paged {
+
+using namespace fmha_sm100;
+
+constexpr int kHeadDim = 64;
+constexpr float kLn2 = 0.69314718055994531f;
+
+// Rows.  The new tokens of a call are numbered f = 0 .. tokens-1 (dense:
+// batch * seqlen_q + index; packed: the packed index).  For one K/V head the
+// rows of a sequence are (token, query head of the group), group fastest:
+// row r is token r / group, query head kvh * group + r % group, so all rows
+// that read the same keys sit in one tile.
+struct Args {
+    CUtensorMap tm_k;
+    CUtensorMap tm_v;
+    const uint16_t* q;
+    uint16_t* o;
+    float* lse;                 // or null
+    const int32_t* page_table;
+    const int32_t* seqlens_k;   // null: every sequence has fixed_len keys
+    const int32_t* seqstart_q;  // null: dense
+    long long table_stride;
+    long long stride_q, nhead_stride_q, batch_stride_q;
+    long long stride_o, nhead_stride_o, batch_stride_o;
+    int batch, seqlen_q, tokens;
+    int nhead_q, nhead_k, group;
+    int page_shift, num_pages, max_pages;
+    int fixed_len;
+    int causal;
+    int row_div;                // tokens per batch entry of q/o (packed: INT_MAX)
+    int lse_len;                // seqlen_q or total_q
+    float scale;                // softmax scale * log2(e)
+    // Sequences whose rows per K/V head lie in [min_rows, max_rows] take part.
+    int min_rows, max_rows;
+    int m_tiles;                // row tiles per sequence (rows kernel)
+    // Partial results of other launches that the final rows fold in: part_n
+    // of them, [part][token * nhead_q + head], normalised O and its LSE in
+    // log2 units (-inf: nothing, O unwritten).
+    const float* part_o;
+    const float* part_lse;
+    int part_n;
+    // Where a launch that makes such partial results puts its own (its split s
+    // into slot s); null: final rows go to o and lse.
+    float* out_o;
+    float* out_lse;
+    int splits;                 // tile kernel: key ranges per row tile
+    int tile_slots;             // tile kernel: row tiles in the grid
+    float* pieces;              // rows kernel: scratch between its blocks
+    int* err_word;
+    unsigned long long wait_limit_ns;
+};
+
+__device__ __forceinline__ void flag_index_error(int* err_word) {
+    atomicCAS(err_word, 0, fmha_host::kErrIndex);
+}
+
+// A sequence as the kernels see it; index data out of range is flagged and
+// cut to what memory holds.
+struct Sequence {
+    int first;   // number of its first new token
+    int count;   // new tokens
+    int keys;    // keys in the cache
+};
+
+__device__ __forceinline__ Sequence load_sequence(const Args& a, int b) {
+    Sequence s;
+    if (a.seqstart_q != nullptr) {
+        s.first = a.seqstart_q[b];
+        s.count = a.seqstart_q[b + 1] - s.first;
+        if (s.first < 0 || s.count < 0 || s.first > a.tokens - s.count) {
+            flag_index_error(a.err_word);
+            s.first = s.count = 0;
+        }
+    } else {
+        s.first = b * a.seqlen_q;
+        s.count = a.seqlen_q;
+    }
+    if (a.seqlens_k != nullptr) {
+        s.keys = max(a.seqlens_k[b], 0);
+        const long long cap = (long long)a.max_pages << a.page_shift;
+        if (s.keys > cap) {
+            flag_index_error(a.err_word);
+            s.keys = (int)cap;
+        }
+    } else {
+        s.keys = a.fixed_len;
+    }
+    return s;
+}
+
+// Keys visible to new token t of a sequence: [0, limit).
+__device__ __forceinline__ int key_limit(const Args& a, const Sequence& s, int t) {
+    return a.causal ? min(s.keys, s.keys - s.count + t + 1) : s.keys;
+}
+
+__device__ __forceinline__ const uint16_t* q_row(const Args& a, int token, int head) {
+    const int b = token / a.row_div;
+    return a.q + b * a.batch_stride_q + (long long)(token - b * a.row_div) * a.stride_q +
+           head * a.nhead_stride_q;
+}
+__device__ __forceinline__ uint16_t* o_row(const Args& a, int token, int head) {
+    const int b = token / a.row_div;
+    return a.o + b * a.batch_stride_o + (long long)(token - b * a.row_div) * a.stride_o +
+           head * a.nhead_stride_o;
+}
+__device__ __forceinline__ float* lse_at(const Args& a, int token, int head) {
+    const int b = token / a.row_div;
+    return a.lse + ((long long)b * a.nhead_q + head) * a.lse_len + (token - b * a.row_div);
+}
+__device__ __forceinline__ long long flat_row(const Args& a, int token, int head) {
+    return (long long)token * a.nhead_q + head;
+}
+
+// Running state of a softmax over disjoint sets of keys: reference maximum m
+// (log2 units), weight sum l, and O un-normalised, all fp32.
+// fold_scales: factors for the state (m, l) and for a newcomer (m2, l2).
+struct Fold {
+    float keep, take;
+};
+__device__ __forceinline__ Fold fold_scales(float& m, float m2) {
+    const float mn = fmaxf(m, m2);
+    Fold f;
+    f.keep = m == -INFINITY ? 0.0f : ex2_approx(m - mn);
+    f.take = m2 == -INFINITY ? 0.0f : ex2_approx(m2 - mn);
+    m = mn;
+    return f;
+}
+
+// The final row's four columns [c, c+4): folds the other launches' partial
+// results in, then writes O (or the normalised partial) and, once per row
+// (`first`), the LSE.  O is rounded once, to nearest even.
+__device__ __forceinline__ void finish_row4(const Args& a, int token, int head, int c, float m,
+                                            float l, float4 o, bool first) {
+    const long long row = flat_row(a, token, head);
+    const long long rows = (long long)a.tokens * a.nhead_q;
+    for (int s = 0; s < a.part_n; ++s) {
+        const float m2 = a.part_lse[s * rows + row];
+        if (m2 == -INFINITY) continue;
+        const float4 x = *reinterpret_cast<const float4*>(a.part_o + (s * rows + row) * kHeadDim + c);
+        const Fold f = fold_scales(m, m2);
+        l = l * f.keep + f.take;
+        o.x = o.x * f.keep + x.x * f.take;
+        o.y = o.y * f.keep + x.y * f.take;
+        o.z = o.z * f.keep + x.z * f.take;
+        o.w = o.w * f.keep + x.w * f.take;
+    }
+    const float inv = l > 0.0f ? 1.0f / l : 0.0f;
+    o.x *= inv, o.y *= inv, o.z *= inv, o.w *= inv;
+    const float lse2 = l > 0.0f ? m + __log2f(l) : -INFINITY;
+    if (a.out_o != nullptr) {
+        *reinterpret_cast<float4*>(a.out_o + row * kHeadDim + c) = o;
+        if (first) a.out_lse[row] = lse2;
+        return;
+    }
+    *reinterpret_cast<uint2*>(o_row(a, token, head) + c) =
+        make_uint2(pack_bf16_rne(o.x, o.y), pack_bf16_rne(o.z, o.w));
+    if (first && a.lse != nullptr) *lse_at(a, token, head) = lse2 * kLn2;
+}
+
+// Bounded wait on an mbarrier phase; false once the block's abort flag is up
+// or the time limit ran out (which raises the flag and the error word).
+__device__ __forceinline__ bool wait_phase(uint32_t bar, uint32_t parity, volatile int* abort_flag,
+                                           const Args& a) {
+    if (mbar_try_wait(bar, parity)) return true;
+    const uint64_t t0 = globaltimer_ns();
+    for (uint32_t it = 1;; ++it) {
+        if (mbar_try_wait(bar, parity)) return true;
+        if ((it & 63u) == 0) {
+            if (*abort_flag) return false;
+            if (globaltimer_ns() - t0 > a.wait_limit_ns) {
+                *abort_flag = 1;
+                atomicCAS(a.err_word, 0, fmha_host::kErrTimeoutPaged);
+                return false;
+            }
+        }
+    }
+}
+// While tearing down: lets copies in flight land, silently, within the limit.
+__device__ __forceinline__ void drain_phase(uint32_t bar, uint32_t parity, const Args& a) {
+    const uint64_t t0 = globaltimer_ns();
+    while (!mbar_try_wait(bar, parity))
+        if (globaltimer_ns() - t0 > a.wait_limit_ns) return;
+}
+
+// One box of a page: 64 values x box rows, tensor coordinates (0, token in
+// page, head, page).  A page id outside the cache reads zeros.
+__device__ __forceinline__ void load_page_box(uint32_t dst, const CUtensorMap* tm, uint32_t bar,
+                                              int token, int head, int page, uint64_t policy) {
+    tma_load_4d(dst, tm, bar, 0, token, head, page, policy);
+}
+
+}  // namespace fmha_paged

@@ -82,7 +82,9 @@ enum {
     FMHA_ERR_LAUNCH = 2,   /* CUDA launch / driver error                       */
     FMHA_ERR_TIMEOUT = 3,  /* a device-side pipeline wait exceeded its limit   */
     FMHA_ERR_DEVICE = 4,   /* no sm_100 device / unsupported device            */
-    FMHA_ERR_SCRATCH = 5   /* request exceeds the allocation-free scratch      */
+    FMHA_ERR_SCRATCH = 5,  /* request exceeds the allocation-free scratch      */
+    FMHA_ERR_INDEX = 6     /* index data on the device was out of range (status
+                              of the paged operators, fmha_paged.h)            */
 };
 
 /* Dense (fixed-length batch) forward, no mask.
@@ -203,8 +205,9 @@ int fmha_fwd_d64_bf16_tiles_noalloc(const FmhaFwdParams* params, int batch, int 
 int fmha_fwd_d64_noalloc_status(struct CUstream_st* stream);
 
 /* Synchronizes `stream`, then reads and clears the device error word written
- * by bounded pipeline waits on the current device.  Returns FMHA_OK or
- * FMHA_ERR_TIMEOUT (or FMHA_ERR_LAUNCH if the synchronization failed).
+ * by bounded pipeline waits on the current device.  Returns FMHA_OK,
+ * FMHA_ERR_TIMEOUT, or FMHA_ERR_INDEX where an operator of fmha_paged.h met
+ * index data out of range (or FMHA_ERR_LAUNCH if the synchronization failed).
  * No reference counterpart (the reference kernel has no error reporting). */
 int fmha_fwd_d64_status(struct CUstream_st* stream);
 

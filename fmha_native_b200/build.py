@@ -20,7 +20,8 @@ LIB_PATH = os.path.join(PKG_DIR, "libfmha_b200.so")
 
 SOURCES = [os.path.join(CSRC, f) for f in ("fmha_fwd_kernel.cu", "fmha_rope.cu", "fmha_paged.cu")]
 DEPS = SOURCES + [
-    *(os.path.join(CSRC, f) for f in ("sm100_ptx.cuh", "host_context.h", "paged_common.cuh", "paged_rows.cuh")),
+    *(os.path.join(CSRC, f) for f in ("sm100_ptx.cuh", "host_context.h", "paged_common.cuh", "paged_rows.cuh",
+                                    "paged_tile.cuh")),
     *(os.path.join(REPO_DIR, "include", f) for f in ("fmha_fwd.h", "fmha_paged.h")),
 ]
 

@@ -13,6 +13,7 @@
 #include "host_context.h"
 #include "paged_common.cuh"
 #include "paged_rows.cuh"
+#include "paged_tile.cuh"
 
 using namespace fmha_paged;
 
@@ -20,6 +21,7 @@ namespace {
 
 static_assert(sizeof(RowsShared<1>) + 1024 <= 227 * 1024, "shared memory of a block");
 static_assert(sizeof(RowsShared<2>) + 1024 <= 227 * 1024, "shared memory of a block");
+static_assert(2 * (sizeof(TileShared) + 2048) <= 228 * 1024, "two tile blocks per SM");
 
 bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
 
@@ -36,28 +38,72 @@ int log2_exact(int v) {
     return -1;
 }
 
-// Rows per K/V head that one sequence may have, and the scratch of a call.
-struct Sizes {
+// Sequences with at most this many rows per K/V head (tokens x group) go to
+// the rows kernel, the others to the tile kernel.  A tile of 128 rows costs the
+// tile kernel the same however many of them are real, and a sequence is cut
+// among blocks only as the host's sizes allow; the rows kernel shares out every
+// key, but each warp holds all rows in registers: 32 is what fits.
+constexpr int kMostRows = 32;
+
+// The launches of a call and its scratch, from sizes that the host has.
+struct Plan {
     long long tokens;
     int group;
-    long long max_rows;
-    size_t pieces;    // bytes of the rows kernel's scratch
-    size_t partials;  // bytes of partial results between launches
+    int max_rows;             // rows per K/V head that one sequence may have
+    bool rows, tile;          // which kernels serve the sequences' own keys
+    long long slots;          // row tiles of the tile kernel (at most)
+    int splits;               // its key ranges
+    long long prefix_slots;   // the same for the prefix
+    int prefix_splits;
+    size_t pieces, part;      // bytes: rows kernel's scratch; one partial result
+    int parts;                // partial results: the prefix's first
     size_t total;
 };
 
-bool sizes_of(int batch, int seqlen_q, int total_q, bool packed, int nhead_q, int nhead_k, int prefix_len,
-              Sizes& z) {
+// Key ranges per row tile where the number of key tiles is known: the time is
+// about waves x (tiles of a range + 2 for a block's start and end).
+int pick_splits(long long jobs, long long tiles) {
+    const long long most = std::min({(long long)16, tiles, std::max(1ll, 4ll * kTileBlocks / jobs)});
+    int best = 1;
+    long long cost = LLONG_MAX;
+    for (int s = 1; s <= most; ++s) {
+        const long long c = (jobs * s + kTileBlocks - 1) / kTileBlocks * ((tiles + s - 1) / s + 2);
+        if (c < cost) cost = c, best = s;
+    }
+    return best;
+}
+
+bool make_plan(int batch, int seqlen_q, int total_q, bool packed, int nhead_q, int nhead_k, int prefix_len,
+               Plan& z) {
+    memset(&z, 0, sizeof(z));
     if (batch <= 0 || seqlen_q < 0 || total_q < 0 || nhead_q <= 0 || nhead_k <= 0 ||
         nhead_q % nhead_k != 0 || prefix_len < 0)
         return false;
     z.tokens = packed ? total_q : (long long)batch * seqlen_q;
     z.group = nhead_q / nhead_k;
-    z.max_rows = (long long)(packed ? std::min(seqlen_q, total_q) : seqlen_q) * z.group;
-    if (z.tokens * nhead_q > INT_MAX || z.max_rows > INT_MAX) return false;
-    z.pieces = rows_scratch_bytes(32);
-    z.partials = prefix_len > 0 ? (size_t)z.tokens * nhead_q * (kHeadDim + 1) * sizeof(float) : 0;
-    z.total = z.pieces + z.partials;
+    const long long max_rows = (long long)(packed ? std::min(seqlen_q, total_q) : seqlen_q) * z.group;
+    if (z.tokens * nhead_q > INT_MAX) return false;
+    z.max_rows = (int)max_rows;
+    z.tile = max_rows > kMostRows;
+    z.rows = packed || !z.tile;
+    z.pieces = rows_scratch_bytes(kMostRows);
+    z.part = (size_t)z.tokens * nhead_q * (kHeadDim + 1) * sizeof(float);
+    if (z.tile) {
+        const long long all = z.tokens * z.group;
+        z.slots = packed ? all / kTileM + std::min<long long>(batch, all / (kMostRows + 1))
+                         : (max_rows + kTileM - 1) / kTileM * batch;
+        // Key counts are on the device: one wave of blocks, if that many.
+        z.splits = (int)std::max(1ll, std::min(16ll, kTileBlocks / (z.slots * nhead_k)));
+        if (z.slots * nhead_k * z.splits > INT_MAX) return false;
+    }
+    if (prefix_len > 0) {
+        z.prefix_slots = (z.tokens * z.group + kTileM - 1) / kTileM;
+        const long long jobs = std::max(1ll, z.prefix_slots * nhead_k);
+        z.prefix_splits = pick_splits(jobs, (prefix_len + kTileN - 1) / kTileN);
+        z.parts = z.prefix_splits;
+    }
+    if (z.tile && (z.splits > 1 || prefix_len > 0)) z.parts += z.splits;
+    z.total = z.pieces + z.part * z.parts;
     return true;
 }
 
@@ -85,12 +131,12 @@ int cache_maps(const fmha_host::Context& ctx, Args& a, const FmhaPagedParams* p,
     return cache_map(ctx, &a.tm_v, p->v_cache, p, p->stride_v, p->nhead_stride_v, p->page_stride_v, box);
 }
 
-int check(const FmhaPagedParams* p, bool prefix, Sizes& z) {
+int check(const FmhaPagedParams* p, bool prefix, Plan& z) {
     if (p == nullptr) return FMHA_ERR_ARG;
     const bool packed = p->seqstart_q != nullptr;
     if (!p->q || !p->k_cache || !p->v_cache || !p->o || !p->page_table || !p->seqlens_k) return FMHA_ERR_ARG;
     if (prefix ? (p->prefix_len <= 0 || !p->prefix_pages) : false) return FMHA_ERR_ARG;
-    if (!sizes_of(p->batch, p->seqlen_q, p->total_q, packed, p->nhead_q, p->nhead_k,
+    if (!make_plan(p->batch, p->seqlen_q, p->total_q, packed, p->nhead_q, p->nhead_k,
                   prefix ? p->prefix_len : 0, z))
         return FMHA_ERR_ARG;
     if (!aligned16(p->q) || !aligned16(p->k_cache) || !aligned16(p->v_cache) || !aligned16(p->o))
@@ -114,7 +160,7 @@ int check(const FmhaPagedParams* p, bool prefix, Sizes& z) {
     return FMHA_OK;
 }
 
-Args base_args(const FmhaPagedParams* p, const Sizes& z, const fmha_host::Context& ctx) {
+Args base_args(const FmhaPagedParams* p, const Plan& z, const fmha_host::Context& ctx) {
     Args a;
     memset(&a, 0, sizeof(a));
     const bool packed = p->seqstart_q != nullptr;
@@ -154,66 +200,108 @@ bool allow_smem(std::atomic<unsigned long long>& ready, int device, const void* 
     return true;
 }
 
-// The rows kernel and, as its programmatic dependent, the merge of the jobs
-// that cross blocks.
-template <int MT>
-int launch_rows_mt(Args& a, int max_rows, int device, cudaStream_t stream) {
-    constexpr int kRows = 16 * MT;
-    constexpr size_t smem = sizeof(RowsShared<MT>) + 1024;
-    static std::atomic<unsigned long long> ready{0};
-    if (!allow_smem(ready, device, reinterpret_cast<const void*>(fmha_paged_rows_kernel<MT>), smem))
-        return FMHA_ERR_LAUNCH;
-    a.m_tiles = std::max(1, (max_rows + kRows - 1) / kRows);
-    if ((long long)a.batch * a.m_tiles > INT_MAX) return FMHA_ERR_ARG;
-    fmha_paged_rows_kernel<MT><<<kMaxRowBlocks, kRowThreadsTotal, smem, stream>>>(a);
+// A launch that may start while the one before it on the stream still runs.
+template <typename Kernel>
+int launch_dependent(Kernel kernel, dim3 grid, int threads, size_t smem, cudaStream_t stream, const Args& a) {
     cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3(kMaxRowBlocks, kRows / 8);
-    cfg.blockDim = dim3(256);
+    cfg.gridDim = grid;
+    cfg.blockDim = dim3(threads);
+    cfg.dynamicSmemBytes = smem;
     cfg.stream = stream;
     cudaLaunchAttribute attr[1];
     attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
     attr[0].val.programmaticStreamSerializationAllowed = 1;
     cfg.attrs = attr;
     cfg.numAttrs = 1;
-    if (cudaLaunchKernelEx(&cfg, fmha_paged_rows_merge<MT>, a) != cudaSuccess) return FMHA_ERR_LAUNCH;
-    return cudaGetLastError() == cudaSuccess ? FMHA_OK : FMHA_ERR_LAUNCH;
+    return cudaLaunchKernelEx(&cfg, kernel, a) == cudaSuccess ? FMHA_OK : FMHA_ERR_LAUNCH;
 }
-int launch_rows(Args& a, int max_rows, int device, cudaStream_t stream) {
-    return max_rows <= 16 ? launch_rows_mt<1>(a, max_rows, device, stream)
-                          : launch_rows_mt<2>(a, max_rows, device, stream);
+
+// The rows kernel (after = it follows another kernel of the call) and the merge
+// of the jobs that cross its blocks.
+template <int MT>
+int launch_rows_mt(const Args& a, bool after, int device, cudaStream_t stream) {
+    constexpr size_t smem = sizeof(RowsShared<MT>) + 1024;
+    static std::atomic<unsigned long long> ready{0};
+    if (!allow_smem(ready, device, reinterpret_cast<const void*>(fmha_paged_rows_kernel<MT>), smem))
+        return FMHA_ERR_LAUNCH;
+    if (after) {
+        const int st = launch_dependent(fmha_paged_rows_kernel<MT>, dim3(kMaxRowBlocks), kRowThreadsTotal, smem,
+                                        stream, a);
+        if (st != FMHA_OK) return st;
+    } else {
+        fmha_paged_rows_kernel<MT><<<kMaxRowBlocks, kRowThreadsTotal, smem, stream>>>(a);
+        if (cudaGetLastError() != cudaSuccess) return FMHA_ERR_LAUNCH;
+    }
+    return launch_dependent(fmha_paged_rows_merge<MT>, dim3(kMaxRowBlocks, 16 * MT / 8), 256, 0, stream, a);
+}
+
+int launch_tile(const Args& a, long long slots, int device, cudaStream_t stream) {
+    constexpr size_t smem = sizeof(TileShared) + 1024;
+    static std::atomic<unsigned long long> ready{0};
+    if (!allow_smem(ready, device, reinterpret_cast<const void*>(fmha_paged_tile_kernel), smem))
+        return FMHA_ERR_LAUNCH;
+    fmha_paged_tile_kernel<<<(unsigned)(slots * a.nhead_k * a.splits), kTileThreads, smem, stream>>>(a);
+    return cudaGetLastError() == cudaSuccess ? FMHA_OK : FMHA_ERR_LAUNCH;
 }
 
 int run(const FmhaPagedParams* p, bool prefix, cudaStream_t stream) {
-    Sizes z;
+    Plan z;
     int st = check(p, prefix, z);
     if (st != FMHA_OK) return st;
     fmha_host::Context ctx;
     if ((st = fmha_host::acquire(&ctx)) != FMHA_OK) return st;
     if (z.tokens == 0) return FMHA_OK;
     Args a = base_args(p, z, ctx);
-    if ((st = cache_maps(ctx, a, p, kUnit)) != FMHA_OK) return st;
-    if (prefix) {
-        // Every token's rows against the prefix, as one sequence without mask.
-        Args b = a;
-        b.seqstart_q = nullptr;
-        b.seqlens_k = nullptr;
-        b.fixed_len = p->prefix_len;
-        b.page_table = p->prefix_pages;
-        b.table_stride = 0;
-        b.max_pages = (p->prefix_len + p->page_size - 1) / p->page_size;
-        b.batch = 1;
-        b.seqlen_q = a.tokens;
-        b.causal = 0;
-        b.out_o = reinterpret_cast<float*>(static_cast<uint8_t*>(p->workspace) + z.pieces);
-        b.out_lse = b.out_o + (size_t)a.tokens * a.nhead_q * kHeadDim;
-        const long long rows = (long long)a.tokens * a.group;
-        if (rows > INT_MAX) return FMHA_ERR_ARG;
-        if ((st = launch_rows(b, (int)rows, ctx.device, stream)) != FMHA_OK) return st;
-        a.part_o = b.out_o;
-        a.part_lse = b.out_lse;
-        a.part_n = 1;
+    float* parts = reinterpret_cast<float*>(static_cast<uint8_t*>(p->workspace) + z.pieces);
+    const size_t part_rows = (size_t)z.tokens * p->nhead_q;
+    float* part_lse = parts + part_rows * kHeadDim * z.parts;
+    if (z.tile || prefix) {
+        Args t = a;
+        if ((st = cache_maps(ctx, t, p, kTileN)) != FMHA_OK) return st;
+        if (prefix) {
+            // Every token's rows against the prefix, as one sequence without mask.
+            Args b = t;
+            b.seqstart_q = nullptr;
+            b.seqlens_k = nullptr;
+            b.fixed_len = p->prefix_len;
+            b.page_table = p->prefix_pages;
+            b.batch = 1;
+            b.seqlen_q = a.tokens;
+            b.causal = 0;
+            b.splits = z.prefix_splits;
+            b.out_o = parts;
+            b.out_lse = part_lse;
+            if ((st = launch_tile(b, z.prefix_slots, ctx.device, stream)) != FMHA_OK) return st;
+        }
+        if (z.tile) {
+            t.min_rows = kMostRows + 1;
+            t.splits = z.splits;
+            if (z.parts > 0) {
+                t.out_o = parts + part_rows * kHeadDim * z.prefix_splits;
+                t.out_lse = part_lse + part_rows * z.prefix_splits;
+            }
+            if ((st = launch_tile(t, z.slots, ctx.device, stream)) != FMHA_OK) return st;
+        }
     }
-    return launch_rows(a, (int)z.max_rows, ctx.device, stream);
+    a.part_o = parts;
+    a.part_lse = part_lse;
+    if (z.rows) {
+        a.part_n = z.prefix_splits;
+        a.m_tiles = 1;
+        if (z.tile) a.max_rows = kMostRows;
+        if ((st = cache_maps(ctx, a, p, kUnit)) != FMHA_OK) return st;
+        const bool after = z.tile || prefix;
+        st = z.max_rows <= 16 ? launch_rows_mt<1>(a, after, ctx.device, stream)
+                              : launch_rows_mt<2>(a, after, ctx.device, stream);
+        if (st != FMHA_OK) return st;
+    }
+    if (z.tile && z.parts > 0) {
+        a.min_rows = kMostRows + 1, a.max_rows = INT_MAX;
+        a.part_n = z.parts;
+        const size_t blocks = (part_rows * 16 + 255) / 256;
+        if ((st = launch_dependent(fmha_paged_combine, dim3((unsigned)blocks), 256, 0, stream, a)) != FMHA_OK) return st;
+    }
+    return FMHA_OK;
 }
 
 }  // namespace
@@ -222,8 +310,8 @@ extern "C" {
 
 size_t fmha_paged_workspace_bytes(int batch, int seqlen_q, int total_q, int nhead_q, int nhead_k,
                                   int prefix_len) {
-    Sizes z;
-    if (!sizes_of(batch, seqlen_q, total_q, total_q > 0, nhead_q, nhead_k, prefix_len, z)) return 0;
+    Plan z;
+    if (!make_plan(batch, seqlen_q, total_q, total_q > 0, nhead_q, nhead_k, prefix_len, z)) return 0;
     return z.total;
 }
 

@@ -51,12 +51,11 @@ struct Args {
     const float* part_o;
     const float* part_lse;
     int part_n;
-    // Where a launch that makes such partial results puts its own (its split s
-    // into slot s); null: final rows go to o and lse.
+    // Where a tile launch that makes such partial results puts its own (split s
+    // into slot s); null: it writes final rows.
     float* out_o;
     float* out_lse;
     int splits;                 // tile kernel: key ranges per row tile
-    int tile_slots;             // tile kernel: row tiles in the grid
     float* pieces;              // rows kernel: scratch between its blocks
     int* err_word;
     unsigned long long wait_limit_ns;
@@ -139,8 +138,7 @@ __device__ __forceinline__ Fold fold_scales(float& m, float m2) {
 }
 
 // The final row's four columns [c, c+4): folds the other launches' partial
-// results in, then writes O (or the normalised partial) and, once per row
-// (`first`), the LSE.  O is rounded once, to nearest even.
+// results in, then writes O and, once per row (`first`), the LSE.  O is rounded once, to nearest even.
 __device__ __forceinline__ void finish_row4(const Args& a, int token, int head, int c, float m,
                                             float l, float4 o, bool first) {
     const long long row = flat_row(a, token, head);
@@ -159,11 +157,6 @@ __device__ __forceinline__ void finish_row4(const Args& a, int token, int head, 
     const float inv = l > 0.0f ? 1.0f / l : 0.0f;
     o.x *= inv, o.y *= inv, o.z *= inv, o.w *= inv;
     const float lse2 = l > 0.0f ? m + __log2f(l) : -INFINITY;
-    if (a.out_o != nullptr) {
-        *reinterpret_cast<float4*>(a.out_o + row * kHeadDim + c) = o;
-        if (first) a.out_lse[row] = lse2;
-        return;
-    }
     *reinterpret_cast<uint2*>(o_row(a, token, head) + c) =
         make_uint2(pack_bf16_rne(o.x, o.y), pack_bf16_rne(o.z, o.w));
     if (first && a.lse != nullptr) *lse_at(a, token, head) = lse2 * kLn2;

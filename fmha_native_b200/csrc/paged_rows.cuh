@@ -152,6 +152,7 @@ fmha_paged_rows_kernel(const __grid_constant__ Args a) {
     volatile int* abort_flag = &sm.abort_flag;
     RowsHeader* headers = piece_headers(a, kRows);
 
+    griddep_launch_dependents();
     if (lane == 0) {
         for (int s = 0; s < kStages; ++s) mbar_init(smem_u32(&sm.bar[warp][s]), 1);
         sm.piece_flags[warp][0] = sm.piece_flags[warp][1] = -1;
@@ -182,6 +183,7 @@ fmha_paged_rows_kernel(const __grid_constant__ Args a) {
     const long long want = (total + kRowWarps - 1) / kRowWarps;
     const int blocks = (int)min((long long)gridDim.x, want);
     if ((int)blockIdx.x >= blocks) {
+        griddep_wait();  // the grid ends after the launch before it
         if (threadIdx.x == 0) headers[blockIdx.x].parts = 0;
         return;
     }
@@ -427,6 +429,7 @@ fmha_paged_rows_kernel(const __grid_constant__ Args a) {
             if (last || c.u + 1 == c.x.units) {
                 const bool begins = seg_begin == 0, ends = c.u + 1 == c.x.units;
                 const bool whole = begins && ends;
+                griddep_wait();  // a launch before this one may hold partial results of the row
                 float* po = last ? reinterpret_cast<float*>(sm.ring[warp]) : sm.first_o[warp];
                 float* pml = last ? po + kRows * kHeadDim : sm.first_ml[warp];
 #pragma unroll
@@ -470,19 +473,11 @@ fmha_paged_rows_kernel(const __grid_constant__ Args a) {
                         }
                         const float inv = lt > 0.0f ? 1.0f / lt : 0.0f;
                         const float lse2 = lt > 0.0f ? mm + __log2f(lt) : -INFINITY;
-                        if (a.out_o != nullptr) {
+                        uint32_t* dst = reinterpret_cast<uint32_t*>(o_row(a, token, head));
 #pragma unroll
-                            for (int n = 0; n < 8; ++n)
-                                *reinterpret_cast<float2*>(a.out_o + row * kHeadDim + n * 8 + 2 * t4) =
-                                    make_float2(o[i][n][2 * hr] * inv, o[i][n][2 * hr + 1] * inv);
-                            if (t4 == 0) a.out_lse[row] = lse2;
-                        } else {
-                            uint32_t* dst = reinterpret_cast<uint32_t*>(o_row(a, token, head));
-#pragma unroll
-                            for (int n = 0; n < 8; ++n)
-                                dst[n * 4 + t4] = pack_bf16_rne(o[i][n][2 * hr] * inv, o[i][n][2 * hr + 1] * inv);
-                            if (t4 == 0 && a.lse != nullptr) *lse_at(a, token, head) = lse2 * kLn2;
-                        }
+                        for (int n = 0; n < 8; ++n)
+                            dst[n * 4 + t4] = pack_bf16_rne(o[i][n][2 * hr] * inv, o[i][n][2 * hr + 1] * inv);
+                        if (t4 == 0 && a.lse != nullptr) *lse_at(a, token, head) = lse2 * kLn2;
                     }
                 if (!whole && lane == 0) {
                     sm.piece_job[warp][last] = (long long)c.e * a.nhead_k + c.h;
@@ -498,7 +493,7 @@ fmha_paged_rows_kernel(const __grid_constant__ Args a) {
     }
 
     // ------------------------------------- pieces: inside the block, then out
-    griddep_launch_dependents();
+    griddep_wait();
     __syncthreads();
     RowsHeader header{0, 0, 0};
     if (!*abort_flag) {

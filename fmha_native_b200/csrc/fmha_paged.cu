@@ -50,6 +50,7 @@ struct Plan {
     long long tokens;
     int group;
     int max_rows;             // rows per K/V head that one sequence may have
+    int row_cap;              // the same for the rows kernel's sequences
     bool rows, tile;          // which kernels serve the sequences' own keys
     long long slots;          // row tiles of the tile kernel (at most)
     int splits;               // its key ranges
@@ -82,11 +83,12 @@ bool make_plan(int batch, int seqlen_q, int total_q, bool packed, int nhead_q, i
     z.tokens = packed ? total_q : (long long)batch * seqlen_q;
     z.group = nhead_q / nhead_k;
     const long long max_rows = (long long)(packed ? std::min(seqlen_q, total_q) : seqlen_q) * z.group;
-    if (z.tokens * nhead_q > INT_MAX) return false;
+    if (z.tokens * nhead_q > INT_MAX || nhead_q > 65535) return false;
     z.max_rows = (int)max_rows;
     z.tile = max_rows > kMostRows;
     z.rows = packed || !z.tile;
-    z.pieces = rows_scratch_bytes(kMostRows);
+    z.row_cap = z.rows ? (int)std::min<long long>(max_rows, kMostRows) : 0;
+    z.pieces = (rows_scratch_bytes((long long)z.row_cap * nhead_k) + 15) / 16 * 16;
     z.part = (size_t)z.tokens * nhead_q * (kHeadDim + 1) * sizeof(float);
     if (z.tile) {
         const long long all = z.tokens * z.group;
@@ -119,7 +121,7 @@ int cache_map(const fmha_host::Context& ctx, CUtensorMap* tm, const uint16_t* ba
     cuuint32_t one[4] = {1, 1, 1, 1};
     const CUresult r = ctx.encode(tm, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 4, const_cast<uint16_t*>(base), dims,
                                   strides, box, one, CU_TENSOR_MAP_INTERLEAVE_NONE,
-                                  CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                                  CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_NONE,
                                   CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
     return r == CUDA_SUCCESS ? FMHA_OK : FMHA_ERR_ARG;
 }
@@ -153,6 +155,8 @@ int check(const FmhaPagedParams* p, bool prefix, Plan& z) {
         !stride_ok(p->page_stride_k, p->num_pages) || !stride_ok(p->stride_v, p->page_size) ||
         !stride_ok(p->nhead_stride_v, p->nhead_k) || !stride_ok(p->page_stride_v, p->num_pages))
         return FMHA_ERR_ARG;
+    // Units of 32 keys over the whole batch are counted in 31 bits.
+    if ((long long)p->batch * (((long long)p->max_pages << shift) / kUnit + 2) > INT_MAX) return FMHA_ERR_ARG;
     if (!(p->scale > 0.0f) || p->scale > 1e30f) return FMHA_ERR_ARG;
     if (z.tokens > 0 && (p->workspace == nullptr || !aligned16(p->workspace) ||
                          p->workspace_bytes < (long long)z.total))
@@ -232,7 +236,8 @@ int launch_rows_mt(const Args& a, bool after, int device, cudaStream_t stream) {
         fmha_paged_rows_kernel<MT><<<kMaxRowBlocks, kRowThreadsTotal, smem, stream>>>(a);
         if (cudaGetLastError() != cudaSuccess) return FMHA_ERR_LAUNCH;
     }
-    return launch_dependent(fmha_paged_rows_merge<MT>, dim3(kMaxRowBlocks, 16 * MT / 8), 256, 0, stream, a);
+    return launch_dependent(fmha_paged_rows_merge<MT>, dim3(kMaxRowBlocks, (a.nhead_k * a.row_cap + 3) / 4), 256, 0,
+                            stream, a);
 }
 
 int launch_tile(const Args& a, long long slots, int device, cudaStream_t stream) {
@@ -287,7 +292,7 @@ int run(const FmhaPagedParams* p, bool prefix, cudaStream_t stream) {
     a.part_lse = part_lse;
     if (z.rows) {
         a.part_n = z.prefix_splits;
-        a.m_tiles = 1;
+        a.row_cap = z.row_cap;
         if (z.tile) a.max_rows = kMostRows;
         if ((st = cache_maps(ctx, a, p, kUnit)) != FMHA_OK) return st;
         const bool after = z.tile || prefix;

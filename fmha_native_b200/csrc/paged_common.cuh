@@ -44,7 +44,7 @@ struct Args {
     float scale;                // softmax scale * log2(e)
     // Sequences whose rows per K/V head lie in [min_rows, max_rows] take part.
     int min_rows, max_rows;
-    int m_tiles;                // row tiles per sequence (rows kernel)
+    int row_cap;                // rows per K/V head that a sequence of the rows kernel may have
     // Partial results of other launches that the final rows fold in: part_n
     // of them, [part][token * nhead_q + head], normalised O and its LSE in
     // log2 units (-inf: nothing, O unwritten).
@@ -137,22 +137,38 @@ __device__ __forceinline__ Fold fold_scales(float& m, float m2) {
     return f;
 }
 
+__device__ __forceinline__ void fold4(float& m, float& l, float4& o, float m2, float l2, float4 o2) {
+    const Fold f = fold_scales(m, m2);
+    l = l * f.keep + l2 * f.take;
+    o.x = o.x * f.keep + o2.x * f.take;
+    o.y = o.y * f.keep + o2.y * f.take;
+    o.z = o.z * f.keep + o2.z * f.take;
+    o.w = o.w * f.keep + o2.w * f.take;
+}
+
 // The final row's four columns [c, c+4): folds the other launches' partial
-// results in, then writes O and, once per row (`first`), the LSE.  O is rounded once, to nearest even.
+// results in, then writes O and, once per row (`first`), the LSE.  O is
+// rounded once, to nearest even.
 __device__ __forceinline__ void finish_row4(const Args& a, int token, int head, int c, float m,
                                             float l, float4 o, bool first) {
     const long long row = flat_row(a, token, head);
     const long long rows = (long long)a.tokens * a.nhead_q;
-    for (int s = 0; s < a.part_n; ++s) {
-        const float m2 = a.part_lse[s * rows + row];
-        if (m2 == -INFINITY) continue;
-        const float4 x = *reinterpret_cast<const float4*>(a.part_o + (s * rows + row) * kHeadDim + c);
-        const Fold f = fold_scales(m, m2);
-        l = l * f.keep + f.take;
-        o.x = o.x * f.keep + x.x * f.take;
-        o.y = o.y * f.keep + x.y * f.take;
-        o.z = o.z * f.keep + x.z * f.take;
-        o.w = o.w * f.keep + x.w * f.take;
+    constexpr int kBatch = 4;  // partial results in flight
+    for (int s0 = 0; s0 < a.part_n; s0 += kBatch) {
+        float m2[kBatch];
+        float4 x[kBatch];
+#pragma unroll
+        for (int u = 0; u < kBatch; ++u) {
+            m2[u] = -INFINITY;
+            x[u] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+            if (s0 + u < a.part_n) {
+                m2[u] = a.part_lse[(s0 + u) * rows + row];
+                x[u] = *reinterpret_cast<const float4*>(a.part_o + ((s0 + u) * rows + row) * kHeadDim + c);
+            }
+        }
+#pragma unroll
+        for (int u = 0; u < kBatch; ++u)
+            if (m2[u] != -INFINITY) fold4(m, l, o, m2[u], 1.0f, x[u]);  // else O was not written
     }
     const float inv = l > 0.0f ? 1.0f / l : 0.0f;
     o.x *= inv, o.y *= inv, o.z *= inv, o.w *= inv;

@@ -8,17 +8,20 @@
 // What bounds it: the cache is read once (256 bytes per key and K/V head) and
 // the arithmetic per byte is small, so it should run at memory speed.  Hence:
 //
-//   work split   The keys of all (sequence, head) jobs are laid end to end in
-//                units of 32 keys; the blocks, and inside a block its 8 warps,
-//                take equal contiguous shares of that line.  Lengths may differ
-//                as they like: every warp streams the same number of bytes.
-//                A job that crosses shares leaves pieces (m, l, O), folded
-//                inside the block through shared memory, and between blocks by
-//                fmha_paged_rows_merge.  The shares follow from the lengths
-//                alone, so results do not depend on timing.
+//   work split   The keys of all sequences are laid end to end in units of 32,
+//                and the blocks take equal contiguous ranges of that line, with
+//                all K/V heads: heads lie side by side in a token, so a block's
+//                warps read neighbouring lines of memory at the same time.
+//                Inside a block the line (sequence, head, unit) of its range is
+//                cut into equal shares for the 8 warps.  Lengths may differ as
+//                they like: every warp streams the same number of bytes.
+//                Pieces (m, l, O) of a head whose units went to several warps
+//                are folded through shared memory, those of a sequence that
+//                crosses blocks by fmha_paged_rows_merge.  The shares follow
+//                from the lengths alone, so results do not depend on timing.
 //   streaming    Each warp has its own ring of kStages units in shared memory,
 //                filled by TMA (one box per page) several units ahead, across
-//                job boundaries too; no block-wide step until the share ends.
+//                heads and sequences; no block-wide step until the share ends.
 //   arithmetic   mma.sync m16n8k16 with the rows as M: the tile of a decode
 //                step is far too thin for a 128-row tensor-memory tile, and
 //                the reads leave the tensor pipe idle anyway.  P enters the
@@ -41,67 +44,73 @@ constexpr int kMaxRowBlocks = 148;    // one block per SM
 
 constexpr int row_stages(int mt) { return mt == 1 ? 3 : 2; }
 
+// A (sequence, head) result of a block: where it goes.
+struct Target {
+    int first, rows;  // the sequence's first token; its rows per K/V head
+    int h;            // K/V head
+    int slot;         // piece slot of the block's scratch, or -1: the final rows
+};
+
 template <int MT>
 struct alignas(1024) RowsShared {
     static constexpr int kRows = 16 * MT;
     static constexpr int kStages = row_stages(MT);
     uint8_t ring[kRowWarps][kStages][2][kUnitBytes];
-    // A piece whose job ended inside the warp's share; a piece at the share's
-    // end reuses the warp's (then idle) ring.
+    // A warp's piece of a head that an earlier warp began.  A piece that a later
+    // warp goes on with comes last and takes the warp's (then idle) ring.
     float first_o[kRowWarps][kRows * kHeadDim];
     float first_ml[kRowWarps][kRows * 2];
+    // (m, l) of a result on its way out, where a ring slot only takes its O.
+    static constexpr bool kSlotTakesAll = kRows * (kHeadDim + 2) * 4 <= 2 * kUnitBytes;
+    float out_ml[kSlotTakesAll ? 1 : kRowWarps][kRows * 2];
     uint64_t bar[kRowWarps][kStages];
-    long long scan[kRowWarps];
-    long long piece_job[kRowWarps][2];
-    int piece_flags[kRowWarps][2];    // -1: none; bit 0: job begins, bit 1: job ends here
-    int piece_left[kRowWarps][2];     // units of the job after this piece
-    int start_entry[kRowWarps];
-    int start_off[kRowWarps];
+    Target piece_to[kRowWarps][2];
+    int piece_job[kRowWarps][2];      // segment of the block * heads + head, -1: none
+    int scan[kRowWarps];
+    int start_b, start_u;
     int abort_flag;
 };
 
-// Scratch between blocks: two piece slots per block, then one header each.
+// Scratch between blocks: per block two slots (0: a sequence that an earlier
+// block began, 1: one that a later block goes on with) of nhead_k x row_cap
+// rows of O, then as many (m, l), then a header per block.
 struct RowsHeader {
-    long long job;
-    int parts;   // blocks that share the job beginning in this block; 0: none
-    int pad;
+    int b;
+    int parts;   // blocks that share sequence b, which begins in this one; 0: none
 };
-__host__ __device__ constexpr size_t rows_piece_floats(int rows) { return (size_t)rows * (kHeadDim + 2); }
-__host__ __device__ constexpr size_t rows_scratch_bytes(int rows) {
-    return kMaxRowBlocks * (2 * rows_piece_floats(rows) * sizeof(float) + sizeof(RowsHeader));
+__host__ __device__ constexpr size_t rows_scratch_bytes(long long rows) {
+    return kMaxRowBlocks * (2 * (size_t)rows * (kHeadDim + 2) * sizeof(float) + sizeof(RowsHeader));
 }
-__device__ __forceinline__ float* piece_o(const Args& a, int rows, int slot) {
-    return a.pieces + (size_t)slot * rows * kHeadDim;
+__device__ __forceinline__ long long piece_row(const Args& a, int slot, int h, int r) {
+    return ((long long)slot * a.nhead_k + h) * a.row_cap + r;
 }
-__device__ __forceinline__ float* piece_ml(const Args& a, int rows, int slot) {
-    return a.pieces + (size_t)2 * kMaxRowBlocks * rows * kHeadDim + (size_t)slot * rows * 2;
+__device__ __forceinline__ float* piece_o(const Args& a, long long row) { return a.pieces + row * kHeadDim; }
+__device__ __forceinline__ float* piece_ml(const Args& a, long long row) {
+    return a.pieces + 2ll * kMaxRowBlocks * a.nhead_k * a.row_cap * kHeadDim + row * 2;
 }
-__device__ __forceinline__ RowsHeader* piece_headers(const Args& a, int rows) {
-    return reinterpret_cast<RowsHeader*>(a.pieces + 2 * kMaxRowBlocks * rows_piece_floats(rows));
+__device__ __forceinline__ RowsHeader* piece_headers(const Args& a) {
+    return reinterpret_cast<RowsHeader*>(a.pieces + 2ll * kMaxRowBlocks * a.nhead_k * a.row_cap * (kHeadDim + 2));
 }
 
-// One row tile of one sequence; its job exists once per K/V head.
-struct Entry {
-    Sequence s;
-    int b;
-    int row0, rows;  // first row of the tile; rows of the sequence
-    int kv_end;      // keys that any row of the tile sees
-    int units;       // 0: nothing to do; a tile that sees no key counts one (empty) unit
+// A sequence as this kernel takes it.
+struct RowSeq {
+    int first, count, keys;
+    int kv_end;      // keys that any of its rows sees
+    int units;       // 0: not ours; a sequence that sees no key counts one (empty) unit
 };
 template <int kRows>
-__device__ __forceinline__ Entry load_entry(const Args& a, int e) {
-    Entry x;
-    x.b = e / a.m_tiles;
-    x.row0 = (e - x.b * a.m_tiles) * kRows;
-    x.s = load_sequence(a, x.b);
-    x.rows = x.s.count * a.group;
-    x.units = 0;
-    x.kv_end = 0;
-    if (x.rows < a.min_rows || x.rows > a.max_rows) x.rows = 0;
-    if (x.rows > a.m_tiles * kRows) flag_index_error(a.err_word);  // more tokens than the call said
-    if (x.row0 >= x.rows) return x;
-    const int t_last = (min(x.rows, x.row0 + kRows) - 1) / a.group;
-    x.kv_end = max(0, key_limit(a, x.s, t_last));
+__device__ __forceinline__ RowSeq load_row_seq(const Args& a, int b) {
+    const Sequence s = load_sequence(a, b);
+    RowSeq x{s.first, s.count, s.keys, 0, 0};
+    int rows = s.count * a.group;
+    if (rows < a.min_rows || rows > a.max_rows) return x;
+    if (rows > kRows || rows > a.row_cap) {  // more tokens than the call said: the first ones only
+        flag_index_error(a.err_word);
+        x.count = min(kRows, a.row_cap) / a.group;
+        if (x.count == 0) return x;
+        x.keys = max(0, min(s.keys, s.keys - s.count + x.count));
+    }
+    x.kv_end = max(0, key_limit(a, Sequence{x.first, x.count, x.keys}, x.count - 1));
     x.units = max(1, (x.kv_end + kUnit - 1) / kUnit);
     return x;
 }
@@ -125,16 +134,29 @@ __device__ __forceinline__ void fence_async_smem() {
     asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
 }
 
-// Equal contiguous shares of `total` units: share c of n starts at
+// Row rt of a result, columns [4 c4, 4 c4 + 4): into the final rows or the
+// block's scratch.
+__device__ __forceinline__ void emit_row4(const Args& a, const Target& to, int rt, int c4, float m, float l,
+                                          float4 o) {
+    if (to.slot < 0) {
+        const int t = rt / a.group;
+        finish_row4(a, to.first + t, to.h * a.group + rt - t * a.group, c4 * 4, m, l, o, c4 == 0);
+    } else {
+        const long long row = piece_row(a, to.slot, to.h, rt);
+        *reinterpret_cast<float4*>(piece_o(a, row) + c4 * 4) = o;
+        if (c4 == 0) *reinterpret_cast<float2*>(piece_ml(a, row)) = make_float2(m, l);
+    }
+}
+
+// Equal contiguous ranges of `total` units: range c of n begins at
 // c * base + min(c, rem).
-struct Shares {
-    long long base, rem;
-    int n;
-    __device__ Shares(long long total, int n_) : base(total / n_), rem(total % n_), n(n_) {}
-    __device__ long long begin(int c) const { return c * base + min((long long)c, rem); }
-    __device__ int owner(long long x) const {
-        const long long wide = rem * (base + 1);
-        return x < wide ? (int)(x / (base + 1)) : (int)(rem + (x - wide) / base);
+struct Ranges {
+    unsigned base, rem;
+    __device__ Ranges(unsigned total, unsigned n) : base(total / n), rem(total % n) {}
+    __device__ unsigned begin(unsigned c) const { return c * base + min(c, rem); }
+    __device__ unsigned owner(unsigned x) const {
+        const unsigned wide = rem * (base + 1);
+        return x < wide ? x / (base + 1) : rem + (x - wide) / base;
     }
 };
 
@@ -150,118 +172,146 @@ fmha_paged_rows_kernel(const __grid_constant__ Args a) {
     const int warp = threadIdx.x >> 5;
     const int lane = threadIdx.x & 31;
     volatile int* abort_flag = &sm.abort_flag;
-    RowsHeader* headers = piece_headers(a, kRows);
 
     griddep_launch_dependents();
     if (lane == 0) {
+        tma_prefetch_desc(&a.tm_k);
+        tma_prefetch_desc(&a.tm_v);
         for (int s = 0; s < kStages; ++s) mbar_init(smem_u32(&sm.bar[warp][s]), 1);
-        sm.piece_flags[warp][0] = sm.piece_flags[warp][1] = -1;
+        sm.piece_job[warp][0] = sm.piece_job[warp][1] = -1;
         if (warp == 0) sm.abort_flag = 0;
         fence_barrier_init();
     }
 
-    // ------------------------------------------------- shares of the line
-    const int entries = a.batch * a.m_tiles;
-    const int per = (entries + kRowThreadsTotal - 1) / kRowThreadsTotal;
-    const int e0 = min(entries, (int)threadIdx.x * per), e1 = min(entries, e0 + per);
-    long long mine = 0;
-    for (int e = e0; e < e1; ++e) mine += (long long)load_entry<kRows>(a, e).units * a.nhead_k;
-    long long incl = mine;
+    // ------------------------------------------------- the block's range
+    const int per = (a.batch + kRowThreadsTotal - 1) / kRowThreadsTotal;
+    const int b0 = min(a.batch, (int)threadIdx.x * per), b1 = min(a.batch, b0 + per);
+    int mine = 0;
+    for (int b = b0; b < b1; ++b) mine += load_row_seq<kRows>(a, b).units;
+    int incl = mine;
 #pragma unroll
     for (int d = 1; d < 32; d <<= 1) {
-        const long long v = __shfl_up_sync(0xffffffffu, incl, d);
+        const int v = __shfl_up_sync(0xffffffffu, incl, d);
         if (lane >= d) incl += v;
     }
     if (lane == 31) sm.scan[warp] = incl;
     __syncthreads();
-    long long before = incl - mine, total = 0;
+    unsigned before = incl - mine, total = 0;
 #pragma unroll
     for (int w = 0; w < kRowWarps; ++w) {
         if (w < warp) before += sm.scan[w];
         total += sm.scan[w];
     }
-    const long long want = (total + kRowWarps - 1) / kRowWarps;
-    const int blocks = (int)min((long long)gridDim.x, want);
-    if ((int)blockIdx.x >= blocks) {
+    // As many blocks as give every warp a unit of some head.
+    const unsigned want = (unsigned)min(((unsigned long long)total * a.nhead_k + kRowWarps - 1) / kRowWarps,
+                                        (unsigned long long)total);
+    const unsigned blocks = min(gridDim.x, want);
+    if (blockIdx.x >= blocks) {
         griddep_wait();  // the grid ends after the launch before it
-        if (threadIdx.x == 0) headers[blockIdx.x].parts = 0;
+        if (threadIdx.x == 0) piece_headers(a)[blockIdx.x].parts = 0;
         return;
     }
-    const Shares shares(total, blocks);
-    const long long beg = shares.begin(blockIdx.x), end = shares.begin(blockIdx.x + 1);
-    const long long len = end - beg;
-#pragma unroll
-    for (int w = 0; w < kRowWarps; ++w) {
-        const long long x = beg + len * w / kRowWarps;
-        if (x >= before && x < before + mine) {
-            long long p = before;
-            for (int e = e0; e < e1; ++e) {
-                const long long c = (long long)load_entry<kRows>(a, e).units * a.nhead_k;
-                if (x < p + c) {
-                    sm.start_entry[w] = e;
-                    sm.start_off[w] = (int)(x - p);
-                    break;
-                }
-                p += c;
+    const Ranges ranges(total, blocks);
+    const unsigned beg = ranges.begin(blockIdx.x), end = ranges.begin(blockIdx.x + 1);
+    if (beg >= before && beg < before + mine) {
+        unsigned p = before;
+        for (int b = b0; b < b1; ++b) {
+            const unsigned n = load_row_seq<kRows>(a, b).units;
+            if (beg < p + n) {
+                sm.start_b = b;
+                sm.start_u = (int)(beg - p);
+                break;
             }
+            p += n;
         }
     }
     __syncthreads();
-    const int count = (int)(len * (warp + 1) / kRowWarps - len * warp / kRowWarps);
 
     // ------------------------------------------------------- the share
-    // Two cursors over the line: `p` issues loads, `c` computes.
+    // A place on the block's line: segment (a sequence's units [unit0, unit0 +
+    // n) in this block), head, unit.  Two cursors: `p` issues loads, `c` computes.
     struct Cursor {
-        Entry x;
-        int e, h, u;
+        RowSeq x;
+        int b, seg, left;  // left: units of the block from this segment on
+        int unit0, n, h, u;
+    };
+    auto next_seq = [&](Cursor& k) {
+        k.left -= k.n;
+        k.unit0 = k.n = 0;
+        if (k.left <= 0) return false;
+        do {
+            if (++k.b >= a.batch) return false;
+            k.x = load_row_seq<kRows>(a, k.b);
+        } while (k.x.units == 0);
+        ++k.seg;
+        k.n = min(k.x.units, k.left);
+        return true;
     };
     auto advance = [&](Cursor& k) {
-        if (++k.u < k.x.units) return;
+        if (++k.u < k.n) return;
         k.u = 0;
         if (++k.h < a.nhead_k) return;
         k.h = 0;
-        do {
-            if (++k.e >= entries) return;
-            k.x = load_entry<kRows>(a, k.e);
-        } while (k.x.units == 0);
+        next_seq(k);
     };
-    if (count > 0) {
+    const unsigned long long tiles = (unsigned long long)(end - beg) * a.nhead_k;
+    const unsigned long long from = tiles * warp / kRowWarps;
+    const long long count = (long long)(tiles * (warp + 1) / kRowWarps - from);
+    RowsHeader header{0, 0};
+    bool waited = false;
+    if (count > 0 || warp == 0) {
         Cursor c;
-        c.e = sm.start_entry[warp];
-        c.x = load_entry<kRows>(a, c.e);
-        c.h = sm.start_off[warp] / c.x.units;
-        c.u = sm.start_off[warp] - c.h * c.x.units;
+        c.b = sm.start_b;
+        c.x = load_row_seq<kRows>(a, c.b);
+        c.seg = 0;
+        c.left = (int)(end - beg);
+        c.unit0 = sm.start_u;
+        c.n = min(c.x.units - c.unit0, c.left);
+        if (warp == 0) {
+            // The block's last segment, if its sequence begins here and goes on.
+            Cursor k = c;
+            while (k.left > k.n && next_seq(k)) {}
+            const int after = k.x.units - k.unit0 - k.n;
+            if (k.unit0 == 0 && after > 0) {
+                header.b = k.b;
+                header.parts = (int)(ranges.owner(end + after - 1) - blockIdx.x) + 1;
+            }
+        }
+        unsigned long long x = from;
+        while (x >= (unsigned long long)c.n * a.nhead_k) {
+            x -= (unsigned long long)c.n * a.nhead_k;
+            if (!next_seq(c)) break;
+        }
+        c.h = c.n > 0 ? (int)((unsigned)x / (unsigned)c.n) : 0;
+        c.u = (int)x - c.h * c.n;
         Cursor p = c;
-        int to_issue = count, issued = 0, done = 0;
+        long long to_issue = count;
+        int issued = 0, done = 0;
 
         // Page ids: lane i holds entry win + i of sequence win_b's table row.
         const int box_rows = min(1 << a.page_shift, kUnit);
         const int boxes = kUnit / box_rows;
         int win_b = -1, win = 0, ids = 0, ids_next = 0;
-        auto load_ids = [&](int b, int first, int pages) {
+        auto load_ids = [&](int first, int pages) {
             const int i = first + lane;
-            return i < pages ? __ldg(a.page_table + b * a.table_stride + i) : 0;
+            return i < pages ? __ldg(a.page_table + win_b * a.table_stride + i) : 0;
         };
         const uint64_t policy = l2_policy_evict_first();
-        if (lane == 0) {
-            tma_prefetch_desc(&a.tm_k);
-            tma_prefetch_desc(&a.tm_v);
-        }
         auto produce = [&]() {
             while (to_issue > 0 && issued - done < kStages) {
                 if (p.x.kv_end > 0) {
-                    const int key0 = p.u * kUnit;
-                    const int pages = (p.x.s.keys + (1 << a.page_shift) - 1) >> a.page_shift;
+                    const int key0 = (p.unit0 + p.u) * kUnit;
+                    const int pages = (p.x.keys + (1 << a.page_shift) - 1) >> a.page_shift;
                     const int page0 = key0 >> a.page_shift;
-                    if (win_b != p.x.b || page0 < win || page0 >= win + 64) {
-                        win_b = p.x.b;
+                    if (win_b != p.b || page0 < win || page0 >= win + 64) {
+                        win_b = p.b;
                         win = page0 & ~3;
-                        ids = load_ids(win_b, win, pages);
-                        ids_next = load_ids(win_b, win + 32, pages);
+                        ids = load_ids(win, pages);
+                        ids_next = load_ids(win + 32, pages);
                     } else if (page0 >= win + 32) {
                         win += 32;
                         ids = ids_next;
-                        ids_next = load_ids(win_b, win + 32, pages);
+                        ids_next = load_ids(win + 32, pages);
                     }
                     const int nbox = min(boxes, (p.x.kv_end - key0 + box_rows - 1) / box_rows);
                     const int slot = issued % kStages;
@@ -290,25 +340,26 @@ fmha_paged_rows_kernel(const __grid_constant__ Args a) {
         uint32_t qf[MT][4][4];
         float o[MT][8][4], m[MT][2], l[MT][2];
         int lim[MT][2];
-        int seg_begin = 0;
+        int u0 = 0;
         bool ok = true;
-        for (int it = 0; it < count; ++it) {
+        for (long long it = 0; it < count; ++it) {
+            const int rows = c.x.count * a.group;
             if (it == 0 || c.u == 0) {
-                seg_begin = c.u;
+                u0 = c.u;
 #pragma unroll
                 for (int i = 0; i < MT; ++i) {
 #pragma unroll
                     for (int hr = 0; hr < 2; ++hr) {
-                        const int r = c.x.row0 + i * 16 + hr * 8 + g;
+                        const int r = i * 16 + hr * 8 + g;
                         m[i][hr] = -INFINITY;
                         l[i][hr] = 0.0f;
                         lim[i][hr] = 0;
                         const uint32_t* src = nullptr;
-                        if (r < c.x.rows) {
+                        if (r < rows) {
                             const int t = r / a.group;
-                            lim[i][hr] = key_limit(a, c.x.s, t);
+                            lim[i][hr] = key_limit(a, Sequence{c.x.first, c.x.count, c.x.keys}, t);
                             src = reinterpret_cast<const uint32_t*>(
-                                q_row(a, c.x.s.first + t, c.h * a.group + r - t * a.group));
+                                q_row(a, c.x.first + t, c.h * a.group + r - t * a.group));
                         }
 #pragma unroll
                         for (int kk = 0; kk < 4; ++kk) {
@@ -332,7 +383,7 @@ fmha_paged_rows_kernel(const __grid_constant__ Args a) {
                 }
                 const uint32_t ks = smem_u32(sm.ring[warp][slot][0]);
                 const uint32_t vs = smem_u32(sm.ring[warp][slot][1]);
-                const int key0 = c.u * kUnit;
+                const int key0 = (c.unit0 + c.u) * kUnit;
                 const int valid = c.x.kv_end - key0;
                 if (valid < kUnit) {
                     uint4* v = reinterpret_cast<uint4*>(sm.ring[warp][slot][1]);
@@ -423,68 +474,58 @@ fmha_paged_rows_kernel(const __grid_constant__ Args a) {
                 ++done;
                 __syncwarp();
             }
-            produce();
-
             const bool last = it + 1 == count;
-            if (last || c.u + 1 == c.x.units) {
-                const bool begins = seg_begin == 0, ends = c.u + 1 == c.x.units;
-                const bool whole = begins && ends;
-                griddep_wait();  // a launch before this one may hold partial results of the row
-                float* po = last ? reinterpret_cast<float*>(sm.ring[warp]) : sm.first_o[warp];
-                float* pml = last ? po + kRows * kHeadDim : sm.first_ml[warp];
+            if (last || c.u + 1 == c.n) {
+                // All of the head's units in this block: out with it, laid out by
+                // rows in the ring slot just read.  A part of them: a piece, kept
+                // for the block's fold.
+                const bool all = u0 == 0 && c.u + 1 == c.n;
+                const bool empty = c.x.kv_end == 0;  // no slot was read, and O is zero
+                float* po = all ? reinterpret_cast<float*>(sm.ring[warp][(done + kStages - 1) % kStages])
+                          : last ? reinterpret_cast<float*>(sm.ring[warp]) : sm.first_o[warp];
+                float* pml = all && !Shared::kSlotTakesAll ? sm.out_ml[warp]
+                             : all || last              ? po + kRows * kHeadDim
+                                                        : sm.first_ml[warp];
+                const Target to{c.x.first, rows, c.h,
+                                c.unit0 == 0 && c.n == c.x.units ? -1 : 2 * (int)blockIdx.x + (c.unit0 == 0)};
+                if (!empty) {
 #pragma unroll
-                for (int i = 0; i < MT; ++i)
+                    for (int i = 0; i < MT; ++i)
 #pragma unroll
-                    for (int hr = 0; hr < 2; ++hr) {
-                        float lt = l[i][hr];
-                        lt += __shfl_xor_sync(0xffffffffu, lt, 1);
-                        lt += __shfl_xor_sync(0xffffffffu, lt, 2);
-                        const int rt = i * 16 + hr * 8 + g;
-                        const int r = c.x.row0 + rt;
-                        if (r >= c.x.rows) continue;
-                        if (!whole) {
+                        for (int hr = 0; hr < 2; ++hr) {
+                            float lt = l[i][hr];
+                            lt += __shfl_xor_sync(0xffffffffu, lt, 1);
+                            lt += __shfl_xor_sync(0xffffffffu, lt, 2);
+                            const int rt = i * 16 + hr * 8 + g;
 #pragma unroll
                             for (int n = 0; n < 8; ++n)
                                 *reinterpret_cast<float2*>(po + rt * kHeadDim + n * 8 + 2 * t4) =
                                     make_float2(o[i][n][2 * hr], o[i][n][2 * hr + 1]);
-                            if (t4 == 0) {
-                                pml[rt * 2] = m[i][hr];
-                                pml[rt * 2 + 1] = lt;
-                            }
-                            continue;
+                            if (t4 == 0) *reinterpret_cast<float2*>(pml + rt * 2) = make_float2(m[i][hr], lt);
                         }
-                        const int t = r / a.group;
-                        const int token = c.x.s.first + t, head = c.h * a.group + r - t * a.group;
-                        const long long row = flat_row(a, token, head);
-                        const long long rows = (long long)a.tokens * a.nhead_q;
-                        float mm = m[i][hr];
-                        for (int s = 0; s < a.part_n; ++s) {
-                            const float m2 = a.part_lse[s * rows + row];
-                            if (m2 == -INFINITY) continue;
-                            const Fold f = fold_scales(mm, m2);
-                            lt = lt * f.keep + f.take;
-                            const float* x = a.part_o + (s * rows + row) * kHeadDim + 2 * t4;
-#pragma unroll
-                            for (int n = 0; n < 8; ++n) {
-                                const float2 y = *reinterpret_cast<const float2*>(x + n * 8);
-                                o[i][n][2 * hr] = o[i][n][2 * hr] * f.keep + y.x * f.take;
-                                o[i][n][2 * hr + 1] = o[i][n][2 * hr + 1] * f.keep + y.y * f.take;
-                            }
+                    __syncwarp();
+                }
+                if (all) {
+                    if (!waited) griddep_wait();  // a launch before this one may hold partial results
+                    waited = true;
+                    for (int rt = lane >> 4; rt < rows; rt += 2) {
+                        float mr = -INFINITY, lr = 0.0f;
+                        float4 y = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+                        if (!empty) {
+                            mr = pml[rt * 2];
+                            lr = pml[rt * 2 + 1];
+                            y = *reinterpret_cast<const float4*>(po + rt * kHeadDim + (lane & 15) * 4);
                         }
-                        const float inv = lt > 0.0f ? 1.0f / lt : 0.0f;
-                        const float lse2 = lt > 0.0f ? mm + __log2f(lt) : -INFINITY;
-                        uint32_t* dst = reinterpret_cast<uint32_t*>(o_row(a, token, head));
-#pragma unroll
-                        for (int n = 0; n < 8; ++n)
-                            dst[n * 4 + t4] = pack_bf16_rne(o[i][n][2 * hr] * inv, o[i][n][2 * hr + 1] * inv);
-                        if (t4 == 0 && a.lse != nullptr) *lse_at(a, token, head) = lse2 * kLn2;
+                        emit_row4(a, to, rt, lane & 15, mr, lr, y);
                     }
-                if (!whole && lane == 0) {
-                    sm.piece_job[warp][last] = (long long)c.e * a.nhead_k + c.h;
-                    sm.piece_left[warp][last] = c.x.units - 1 - c.u;
-                    sm.piece_flags[warp][last] = (begins ? 1 : 0) | (ends ? 2 : 0);
+                    fence_async_smem();  // ordered before the slot's next TMA write
+                    __syncwarp();
+                } else if (lane == 0) {
+                    sm.piece_to[warp][last] = to;
+                    sm.piece_job[warp][last] = c.seg * a.nhead_k + c.h;
                 }
             }
+            produce();
             advance(c);
         }
         if (!ok)
@@ -492,127 +533,91 @@ fmha_paged_rows_kernel(const __grid_constant__ Args a) {
                 drain_phase(smem_u32(&sm.bar[warp][i % kStages]), (i / kStages) & 1, a);
     }
 
-    // ------------------------------------- pieces: inside the block, then out
-    griddep_wait();
+    // --------------------------------------------- the block's fold of pieces
+    if (!waited) griddep_wait();
+    if (threadIdx.x == 0) piece_headers(a)[blockIdx.x] = header;
     __syncthreads();
-    RowsHeader header{0, 0, 0};
-    if (!*abort_flag) {
-        const int c4 = threadIdx.x & 15;
-        for (int i = 0; i < 2 * kRowWarps;) {
-            const int flags = sm.piece_flags[i >> 1][i & 1];
-            if (flags < 0) {
-                ++i;
-                continue;
+    if (*abort_flag) return;
+    const int c4 = threadIdx.x & 15;
+    for (int i = 0; i < 2 * kRowWarps;) {
+        const int job = sm.piece_job[i >> 1][i & 1];
+        int next = i + 1;
+        if (job >= 0) {
+            while (next < 2 * kRowWarps) {
+                const int j = sm.piece_job[next >> 1][next & 1];
+                if (j >= 0 && j != job) break;
+                ++next;
             }
-            const long long job = sm.piece_job[i >> 1][i & 1];
-            int last = i, next = i + 1;
-            for (; next < 2 * kRowWarps; ++next) {
-                if (sm.piece_flags[next >> 1][next & 1] < 0) continue;
-                if (sm.piece_job[next >> 1][next & 1] != job) break;
-                last = next;
-            }
-            const bool begins = flags & 1, ends = sm.piece_flags[last >> 1][last & 1] & 2;
-            const int slot = 2 * (int)blockIdx.x + (begins ? 1 : 0);
-            const Entry x = load_entry<kRows>(a, (int)(job / a.nhead_k));
-            const int h = (int)(job % a.nhead_k);
-#pragma unroll
-            for (int pass = 0; pass < MT; ++pass) {
-                const int rt = pass * 16 + (int)(threadIdx.x >> 4);
-                const int r = x.row0 + rt;
-                if (r >= x.rows) continue;
+            const Target to = sm.piece_to[i >> 1][i & 1];
+            for (int rt = threadIdx.x >> 4; rt < to.rows; rt += kRowThreadsTotal / 16) {
                 float m = -INFINITY, l = 0.0f;
                 float4 o = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-                for (int k = i; k <= last; ++k) {
-                    if (sm.piece_flags[k >> 1][k & 1] < 0) continue;
+                for (int k = i; k < next; ++k) {
+                    if (sm.piece_job[k >> 1][k & 1] < 0) continue;
                     const float* po = (k & 1) ? reinterpret_cast<const float*>(sm.ring[k >> 1])
                                               : sm.first_o[k >> 1];
                     const float* pml = (k & 1) ? po + kRows * kHeadDim : sm.first_ml[k >> 1];
-                    const Fold f = fold_scales(m, pml[rt * 2]);
-                    l = l * f.keep + pml[rt * 2 + 1] * f.take;
-                    const float4 y = *reinterpret_cast<const float4*>(po + rt * kHeadDim + c4 * 4);
-                    o.x = o.x * f.keep + y.x * f.take;
-                    o.y = o.y * f.keep + y.y * f.take;
-                    o.z = o.z * f.keep + y.z * f.take;
-                    o.w = o.w * f.keep + y.w * f.take;
+                    fold4(m, l, o, pml[rt * 2], pml[rt * 2 + 1],
+                          *reinterpret_cast<const float4*>(po + rt * kHeadDim + c4 * 4));
                 }
-                if (begins && ends) {
-                    const int t = r / a.group;
-                    finish_row4(a, x.s.first + t, h * a.group + r - t * a.group, c4 * 4, m, l, o, c4 == 0);
-                } else {
-                    *reinterpret_cast<float4*>(piece_o(a, kRows, slot) + rt * kHeadDim + c4 * 4) = o;
-                    if (c4 == 0)
-                        *reinterpret_cast<float2*>(piece_ml(a, kRows, slot) + rt * 2) = make_float2(m, l);
-                }
+                emit_row4(a, to, rt, c4, m, l, o);
             }
-            if (begins && !ends) {
-                const long long job_end = end + sm.piece_left[last >> 1][last & 1];
-                header.job = job;
-                header.parts = shares.owner(job_end - 1) - (int)blockIdx.x + 1;
-            }
-            i = next;
         }
+        i = next;
     }
-    if (threadIdx.x == 0) headers[blockIdx.x] = header;
 }
 
-// Folds the pieces of the job that begins in block blockIdx.x and goes on in
-// the blocks after it.  One warp per row: 16 lanes cover the columns, the two
-// halves take alternate pieces.
+// Folds the pieces of the sequence that begins in block blockIdx.x and goes on
+// in the blocks after it.  64 threads per row: 16 cover the columns, the four
+// sixteens take every fourth piece, kBatch of them in flight.
 template <int MT>
 __global__ void __launch_bounds__(256)
 fmha_paged_rows_merge(const __grid_constant__ Args a) {
-    constexpr int kRows = 16 * MT;
+    constexpr int kBatch = 8;
+    __shared__ float4 other_o[4][16];
+    __shared__ float2 other_ml[4][16];
     griddep_wait();
-    const RowsHeader hd = piece_headers(a, kRows)[blockIdx.x];
+    const RowsHeader hd = piece_headers(a)[blockIdx.x];
     if (hd.parts == 0) return;
-    const Entry x = load_entry<kRows>(a, (int)(hd.job / a.nhead_k));
-    const int h = (int)(hd.job % a.nhead_k);
-    const int rt = blockIdx.y * 8 + (int)(threadIdx.x >> 5);
-    const int r = x.row0 + rt;
-    if (r >= x.rows) return;
+    const RowSeq x = load_row_seq<16 * MT>(a, hd.b);
+    const int rows = x.count * a.group;
+    const int y = blockIdx.y * 4 + (int)(threadIdx.x >> 6);
+    const bool has_row = y < rows * a.nhead_k;
+    const int h = has_row ? y / rows : 0, rt = has_row ? y - h * rows : 0;
     const int lane = threadIdx.x & 31, c4 = lane & 15;
     float m = -INFINITY, l = 0.0f;
     float4 o = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-    constexpr int kBatch = 4;  // pieces in flight per half
-    for (int k0 = lane >> 4; k0 < hd.parts; k0 += 2 * kBatch) {
-        float2 ml[kBatch];
-        float4 y[kBatch];
+    if (has_row)
+        for (int k0 = (threadIdx.x >> 4) & 3; k0 < hd.parts; k0 += 4 * kBatch) {
+            float2 ml[kBatch];
+            float4 z[kBatch];
 #pragma unroll
-        for (int u = 0; u < kBatch; ++u) {
-            const int k = k0 + 2 * u;
-            ml[u] = make_float2(-INFINITY, 0.0f);
-            y[u] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-            if (k < hd.parts) {
-                const int slot = 2 * ((int)blockIdx.x + k) + (k == 0 ? 1 : 0);
-                ml[u] = *reinterpret_cast<const float2*>(piece_ml(a, kRows, slot) + rt * 2);
-                y[u] = *reinterpret_cast<const float4*>(piece_o(a, kRows, slot) + rt * kHeadDim + c4 * 4);
+            for (int u = 0; u < kBatch; ++u) {
+                const int k = k0 + 4 * u;
+                ml[u] = make_float2(-INFINITY, 0.0f);
+                z[u] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+                if (k < hd.parts) {
+                    const long long row = piece_row(a, 2 * ((int)blockIdx.x + k) + (k == 0), h, rt);
+                    ml[u] = *reinterpret_cast<const float2*>(piece_ml(a, row));
+                    z[u] = *reinterpret_cast<const float4*>(piece_o(a, row) + c4 * 4);
+                }
             }
-        }
 #pragma unroll
-        for (int u = 0; u < kBatch; ++u) {
-            const Fold f = fold_scales(m, ml[u].x);
-            l = l * f.keep + ml[u].y * f.take;
-            o.x = o.x * f.keep + y[u].x * f.take;
-            o.y = o.y * f.keep + y[u].y * f.take;
-            o.z = o.z * f.keep + y[u].z * f.take;
-            o.w = o.w * f.keep + y[u].w * f.take;
+            for (int u = 0; u < kBatch; ++u) fold4(m, l, o, ml[u].x, ml[u].y, z[u]);
         }
+    // Within the warp, then the row's second warp.
+    fold4(m, l, o, __shfl_xor_sync(0xffffffffu, m, 16), __shfl_xor_sync(0xffffffffu, l, 16),
+          make_float4(__shfl_xor_sync(0xffffffffu, o.x, 16), __shfl_xor_sync(0xffffffffu, o.y, 16),
+                      __shfl_xor_sync(0xffffffffu, o.z, 16), __shfl_xor_sync(0xffffffffu, o.w, 16)));
+    const int slot = threadIdx.x >> 6;
+    if ((threadIdx.x & 32) && lane < 16) {
+        other_o[slot][c4] = o;
+        other_ml[slot][c4] = make_float2(m, l);
     }
-    // The other half's state (every lane of the warp is here: r is per warp).
-    const float m2 = __shfl_xor_sync(0xffffffffu, m, 16);
-    const float l2 = __shfl_xor_sync(0xffffffffu, l, 16);
-    const float4 y = make_float4(
-        __shfl_xor_sync(0xffffffffu, o.x, 16), __shfl_xor_sync(0xffffffffu, o.y, 16),
-        __shfl_xor_sync(0xffffffffu, o.z, 16), __shfl_xor_sync(0xffffffffu, o.w, 16));
-    const Fold f = fold_scales(m, m2);
-    l = l * f.keep + l2 * f.take;
-    o.x = o.x * f.keep + y.x * f.take;
-    o.y = o.y * f.keep + y.y * f.take;
-    o.z = o.z * f.keep + y.z * f.take;
-    o.w = o.w * f.keep + y.w * f.take;
-    if (lane < 16) {
-        const int t = r / a.group;
-        finish_row4(a, x.s.first + t, h * a.group + r - t * a.group, c4 * 4, m, l, o, c4 == 0);
+    __syncthreads();
+    if (has_row && !(threadIdx.x & 32) && lane < 16) {
+        fold4(m, l, o, other_ml[slot][c4].x, other_ml[slot][c4].y, other_o[slot][c4]);
+        emit_row4(a, Target{x.first, rows, h, -1}, rt, c4, m, l, o);
     }
 }
 

@@ -19,8 +19,7 @@ using namespace fmha_paged;
 
 namespace {
 
-static_assert(sizeof(RowsShared<1>) + 1024 <= 227 * 1024, "shared memory of a block");
-static_assert(sizeof(RowsShared<2>) + 1024 <= 227 * 1024, "shared memory of a block");
+static_assert(sizeof(RowsShared) + 1024 <= 227 * 1024, "shared memory of a block");
 static_assert(2 * (sizeof(TileShared) + 2048) <= 228 * 1024, "two tile blocks per SM");
 
 bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
@@ -38,26 +37,20 @@ int log2_exact(int v) {
     return -1;
 }
 
-// Sequences with at most this many rows per K/V head (tokens x group) go to
-// the rows kernel, the others to the tile kernel.  A tile of 128 rows costs the
-// tile kernel the same however many of them are real, and a sequence is cut
-// among blocks only as the host's sizes allow; the rows kernel shares out every
-// key, but each warp holds all rows in registers: 32 is what fits.
-constexpr int kMostRows = 32;
-
-// The launches of a call and its scratch, from sizes that the host has.
+// Sequences with at most kMostRows rows per K/V head (tokens x group) go to the
+// rows kernel, the others to the tile kernel.  The launches of a call and its
+// scratch, from sizes that the host has.
 struct Plan {
     long long tokens;
     int group;
     int max_rows;             // rows per K/V head that one sequence may have
-    int row_cap;              // the same for the rows kernel's sequences
     bool rows, tile;          // which kernels serve the sequences' own keys
-    long long slots;          // row tiles of the tile kernel (at most)
-    int splits;               // its key ranges
-    long long prefix_slots;   // the same for the prefix
+    int row_cap;              // max_rows for the rows kernel's sequences
+    long long tiles;          // row tiles of the tile kernel (at most)
+    bool planned;             // it plans its key ranges by the lengths
+    long long prefix_tiles;   // row tiles against the prefix, and their key ranges
     int prefix_splits;
-    size_t pieces, part;      // bytes: rows kernel's scratch; one partial result
-    int parts;                // partial results: the prefix's first
+    size_t pieces, slots, part;  // bytes: the two kernels' scratch; one partial result of all rows
     size_t total;
 };
 
@@ -74,6 +67,8 @@ int pick_splits(long long jobs, long long tiles) {
     return best;
 }
 
+size_t round16(size_t n) { return (n + 15) / 16 * 16; }
+
 bool make_plan(int batch, int seqlen_q, int total_q, bool packed, int nhead_q, int nhead_k, int prefix_len,
                Plan& z) {
     memset(&z, 0, sizeof(z));
@@ -87,25 +82,25 @@ bool make_plan(int batch, int seqlen_q, int total_q, bool packed, int nhead_q, i
     z.max_rows = (int)max_rows;
     z.tile = max_rows > kMostRows;
     z.rows = packed || !z.tile;
-    z.row_cap = z.rows ? (int)std::min<long long>(max_rows, kMostRows) : 0;
-    z.pieces = (rows_scratch_bytes((long long)z.row_cap * nhead_k) + 15) / 16 * 16;
-    z.part = (size_t)z.tokens * nhead_q * (kHeadDim + 1) * sizeof(float);
+    if (z.rows) {
+        z.row_cap = (int)std::min<long long>(max_rows, kMostRows);
+        z.pieces = round16(rows_scratch_bytes((long long)z.row_cap * nhead_k));
+    }
     if (z.tile) {
         const long long all = z.tokens * z.group;
-        z.slots = packed ? all / kTileM + std::min<long long>(batch, all / (kMostRows + 1))
+        z.tiles = packed ? all / kTileM + std::min<long long>(batch, all / (kMostRows + 1))
                          : (max_rows + kTileM - 1) / kTileM * batch;
-        // Key counts are on the device: one wave of blocks, if that many.
-        z.splits = (int)std::max(1ll, std::min(16ll, kTileBlocks / (z.slots * nhead_k)));
-        if (z.slots * nhead_k * z.splits > INT_MAX) return false;
+        if ((z.tiles + 2 * kTileBlocks) * nhead_k > INT_MAX) return false;
+        z.planned = z.tiles <= kMaxPlanned && batch <= kMaxPlanned;
+        if (z.planned)
+            z.slots = round16(kMaxTileSlots * (tile_slot_floats() * sizeof(float) + sizeof(TileHeader)));
     }
     if (prefix_len > 0) {
-        z.prefix_slots = (z.tokens * z.group + kTileM - 1) / kTileM;
-        const long long jobs = std::max(1ll, z.prefix_slots * nhead_k);
-        z.prefix_splits = pick_splits(jobs, (prefix_len + kTileN - 1) / kTileN);
-        z.parts = z.prefix_splits;
+        z.prefix_tiles = (z.tokens * z.group + kTileM - 1) / kTileM;
+        z.prefix_splits = pick_splits(std::max(1ll, z.prefix_tiles * nhead_k), (prefix_len + kTileN - 1) / kTileN);
+        z.part = (size_t)z.tokens * nhead_q * (kHeadDim + 1) * sizeof(float);
     }
-    if (z.tile && (z.splits > 1 || prefix_len > 0)) z.parts += z.splits;
-    z.total = z.pieces + z.part * z.parts;
+    z.total = z.pieces + z.slots + z.part * z.prefix_splits;
     return true;
 }
 
@@ -188,7 +183,6 @@ Args base_args(const FmhaPagedParams* p, const Plan& z, const fmha_host::Context
     a.lse_len = packed ? p->total_q : p->seqlen_q;
     a.scale = p->scale;
     a.min_rows = 1, a.max_rows = INT_MAX;
-    a.pieces = static_cast<float*>(p->workspace);
     a.err_word = ctx.err_word;
     a.wait_limit_ns = ctx.wait_limit_ns;
     return a;
@@ -221,31 +215,30 @@ int launch_dependent(Kernel kernel, dim3 grid, int threads, size_t smem, cudaStr
 }
 
 // The rows kernel (after = it follows another kernel of the call) and the merge
-// of the jobs that cross its blocks.
-template <int MT>
-int launch_rows_mt(const Args& a, bool after, int device, cudaStream_t stream) {
-    constexpr size_t smem = sizeof(RowsShared<MT>) + 1024;
+// of the sequences that cross its blocks.
+int launch_rows(const Args& a, bool after, int device, cudaStream_t stream) {
+    constexpr size_t smem = sizeof(RowsShared) + 1024;
     static std::atomic<unsigned long long> ready{0};
-    if (!allow_smem(ready, device, reinterpret_cast<const void*>(fmha_paged_rows_kernel<MT>), smem))
+    if (!allow_smem(ready, device, reinterpret_cast<const void*>(fmha_paged_rows_kernel), smem))
         return FMHA_ERR_LAUNCH;
     if (after) {
-        const int st = launch_dependent(fmha_paged_rows_kernel<MT>, dim3(kMaxRowBlocks), kRowThreadsTotal, smem,
-                                        stream, a);
+        const int st = launch_dependent(fmha_paged_rows_kernel, dim3(kMaxRowBlocks), kRowThreadsTotal, smem, stream, a);
         if (st != FMHA_OK) return st;
     } else {
-        fmha_paged_rows_kernel<MT><<<kMaxRowBlocks, kRowThreadsTotal, smem, stream>>>(a);
+        fmha_paged_rows_kernel<<<kMaxRowBlocks, kRowThreadsTotal, smem, stream>>>(a);
         if (cudaGetLastError() != cudaSuccess) return FMHA_ERR_LAUNCH;
     }
-    return launch_dependent(fmha_paged_rows_merge<MT>, dim3(kMaxRowBlocks, (a.nhead_k * a.row_cap + 3) / 4), 256, 0,
-                            stream, a);
+    return launch_dependent(fmha_paged_rows_merge, dim3(kMaxRowBlocks, (a.nhead_k * a.row_cap + 3) / 4), 256, 0, stream,
+                            a);
 }
 
-int launch_tile(const Args& a, long long slots, int device, cudaStream_t stream) {
+// `ranges`: row tiles and, cut by the plan or the host, their key ranges.
+int launch_tile(const Args& a, long long ranges, int device, cudaStream_t stream) {
     constexpr size_t smem = sizeof(TileShared) + 1024;
     static std::atomic<unsigned long long> ready{0};
     if (!allow_smem(ready, device, reinterpret_cast<const void*>(fmha_paged_tile_kernel), smem))
         return FMHA_ERR_LAUNCH;
-    fmha_paged_tile_kernel<<<(unsigned)(slots * a.nhead_k * a.splits), kTileThreads, smem, stream>>>(a);
+    fmha_paged_tile_kernel<<<(unsigned)(ranges * a.nhead_k), kTileThreads, smem, stream>>>(a);
     return cudaGetLastError() == cudaSuccess ? FMHA_OK : FMHA_ERR_LAUNCH;
 }
 
@@ -257,9 +250,12 @@ int run(const FmhaPagedParams* p, bool prefix, cudaStream_t stream) {
     if ((st = fmha_host::acquire(&ctx)) != FMHA_OK) return st;
     if (z.tokens == 0) return FMHA_OK;
     Args a = base_args(p, z, ctx);
-    float* parts = reinterpret_cast<float*>(static_cast<uint8_t*>(p->workspace) + z.pieces);
-    const size_t part_rows = (size_t)z.tokens * p->nhead_q;
-    float* part_lse = parts + part_rows * kHeadDim * z.parts;
+    uint8_t* scratch = static_cast<uint8_t*>(p->workspace);
+    a.pieces = reinterpret_cast<float*>(scratch);
+    a.slots = reinterpret_cast<float*>(scratch + z.pieces);
+    float* part_o = reinterpret_cast<float*>(scratch + z.pieces + z.slots);
+    float* part_lse = part_o + (size_t)z.tokens * p->nhead_q * kHeadDim * z.prefix_splits;
+    a.splits = 1;
     if (z.tile || prefix) {
         Args t = a;
         if ((st = cache_maps(ctx, t, p, kTileN)) != FMHA_OK) return st;
@@ -274,39 +270,33 @@ int run(const FmhaPagedParams* p, bool prefix, cudaStream_t stream) {
             b.seqlen_q = a.tokens;
             b.causal = 0;
             b.splits = z.prefix_splits;
-            b.out_o = parts;
+            b.out_o = part_o;
             b.out_lse = part_lse;
-            if ((st = launch_tile(b, z.prefix_slots, ctx.device, stream)) != FMHA_OK) return st;
+            if ((st = launch_tile(b, z.prefix_tiles * z.prefix_splits, ctx.device, stream)) != FMHA_OK) return st;
+            a.part_o = t.part_o = part_o;
+            a.part_lse = t.part_lse = part_lse;
+            a.part_n = t.part_n = z.prefix_splits;
         }
         if (z.tile) {
             t.min_rows = kMostRows + 1;
-            t.splits = z.splits;
-            if (z.parts > 0) {
-                t.out_o = parts + part_rows * kHeadDim * z.prefix_splits;
-                t.out_lse = part_lse + part_rows * z.prefix_splits;
-            }
-            if ((st = launch_tile(t, z.slots, ctx.device, stream)) != FMHA_OK) return st;
+            t.plan = z.planned;
+            t.max_slots = kMaxTileSlots;
+            // A plan makes at most one range per tile and 2 kTileBlocks more in all.
+            const long long ranges = z.tiles + (z.planned ? (2 * kTileBlocks + p->nhead_k - 1) / p->nhead_k : 0);
+            if ((st = launch_tile(t, ranges, ctx.device, stream)) != FMHA_OK) return st;
         }
     }
-    a.part_o = parts;
-    a.part_lse = part_lse;
     if (z.rows) {
-        a.part_n = z.prefix_splits;
         a.row_cap = z.row_cap;
         if (z.tile) a.max_rows = kMostRows;
         if ((st = cache_maps(ctx, a, p, kUnit)) != FMHA_OK) return st;
-        const bool after = z.tile || prefix;
-        st = z.max_rows <= 16 ? launch_rows_mt<1>(a, after, ctx.device, stream)
-                              : launch_rows_mt<2>(a, after, ctx.device, stream);
-        if (st != FMHA_OK) return st;
+        if ((st = launch_rows(a, z.tile || prefix, ctx.device, stream)) != FMHA_OK) return st;
     }
-    if (z.tile && z.parts > 0) {
-        a.min_rows = kMostRows + 1, a.max_rows = INT_MAX;
-        a.part_n = z.parts;
-        const size_t blocks = (part_rows * 16 + 255) / 256;
-        if ((st = launch_dependent(fmha_paged_combine, dim3((unsigned)blocks), 256, 0, stream, a)) != FMHA_OK) return st;
+    if (z.tile && z.planned) {
+        a.max_slots = kMaxTileSlots;
+        st = launch_dependent(fmha_paged_combine, dim3(kCombineBlocks), kCombineThreads, 0, stream, a);
     }
-    return FMHA_OK;
+    return st;
 }
 
 }  // namespace

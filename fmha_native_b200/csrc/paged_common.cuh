@@ -55,7 +55,10 @@ struct Args {
     // into slot s); null: it writes final rows.
     float* out_o;
     float* out_lse;
-    int splits;                 // tile kernel: key ranges per row tile
+    int splits;                 // tile kernel, plan == 0: key ranges per row tile
+    int plan;                   // tile kernel: ranges by the lengths (find_item)
+    float* slots;               // and the scratch of the jobs that blocks share
+    int max_slots;
     float* pieces;              // rows kernel: scratch between its blocks
     int* err_word;
     unsigned long long wait_limit_ns;

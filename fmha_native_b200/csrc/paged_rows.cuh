@@ -2,7 +2,7 @@
 // cache: single tokens, a few drafted tokens, grouped query heads.
 //
 // What it computes per (sequence, K/V head): O = softmax(scale Q K^T) V for up
-// to kRows rows that share the keys, as one pass over the keys with a running
+// to kMostRows rows that share the keys, as one pass over the keys with a running
 // maximum m, weight sum l and un-normalised O per row (fp32).
 //
 // What bounds it: the cache is read once (256 bytes per key and K/V head) and
@@ -19,7 +19,7 @@
 //                are folded through shared memory, those of a sequence that
 //                crosses blocks by fmha_paged_rows_merge.  The shares follow
 //                from the lengths alone, so results do not depend on timing.
-//   streaming    Each warp has its own ring of kStages units in shared memory,
+//   streaming    Each warp has its own ring of kRowStages units in shared memory,
 //                filled by TMA (one box per page) several units ahead, across
 //                heads and sequences; no block-wide step until the share ends.
 //   arithmetic   mma.sync m16n8k16 with the rows as M: the tile of a decode
@@ -42,7 +42,8 @@ constexpr int kRowThreadsTotal = 32 * kRowWarps;
 constexpr int kUnitBytes = kUnit * kHeadDim * 2;  // 4 KB of K, as much of V
 constexpr int kMaxRowBlocks = 148;    // one block per SM
 
-constexpr int row_stages(int mt) { return mt == 1 ? 3 : 2; }
+constexpr int kMostRows = 16;         // rows of a K/V head that a warp holds
+constexpr int kRowStages = 3;
 
 // A (sequence, head) result of a block: where it goes.
 struct Target {
@@ -51,22 +52,17 @@ struct Target {
     int slot;         // piece slot of the block's scratch, or -1: the final rows
 };
 
-template <int MT>
 struct alignas(1024) RowsShared {
-    static constexpr int kRows = 16 * MT;
-    static constexpr int kStages = row_stages(MT);
-    uint8_t ring[kRowWarps][kStages][2][kUnitBytes];
+    uint8_t ring[kRowWarps][kRowStages][2][kUnitBytes];
     // A warp's piece of a head that an earlier warp began.  A piece that a later
     // warp goes on with comes last and takes the warp's (then idle) ring.
-    float first_o[kRowWarps][kRows * kHeadDim];
-    float first_ml[kRowWarps][kRows * 2];
-    // (m, l) of a result on its way out, where a ring slot only takes its O.
-    static constexpr bool kSlotTakesAll = kRows * (kHeadDim + 2) * 4 <= 2 * kUnitBytes;
-    float out_ml[kSlotTakesAll ? 1 : kRowWarps][kRows * 2];
-    uint64_t bar[kRowWarps][kStages];
+    float first_o[kRowWarps][kMostRows * kHeadDim];
+    float first_ml[kRowWarps][kMostRows * 2];
+    uint64_t bar[kRowWarps][kRowStages];
     Target piece_to[kRowWarps][2];
     int piece_job[kRowWarps][2];      // segment of the block * heads + head, -1: none
     int scan[kRowWarps];
+    int run[2 * kRowWarps + 1];
     int start_b, start_u;
     int abort_flag;
 };
@@ -75,8 +71,9 @@ struct alignas(1024) RowsShared {
 // block began, 1: one that a later block goes on with) of nhead_k x row_cap
 // rows of O, then as many (m, l), then a header per block.
 struct RowsHeader {
-    int b;
-    int parts;   // blocks that share sequence b, which begins in this one; 0: none
+    int first, rows;  // a sequence that begins in this block and goes on: its first token, rows
+    int parts;        // blocks that share it; 0: none
+    int pad;
 };
 __host__ __device__ constexpr size_t rows_scratch_bytes(long long rows) {
     return kMaxRowBlocks * (2 * (size_t)rows * (kHeadDim + 2) * sizeof(float) + sizeof(RowsHeader));
@@ -98,15 +95,14 @@ struct RowSeq {
     int kv_end;      // keys that any of its rows sees
     int units;       // 0: not ours; a sequence that sees no key counts one (empty) unit
 };
-template <int kRows>
 __device__ __forceinline__ RowSeq load_row_seq(const Args& a, int b) {
     const Sequence s = load_sequence(a, b);
     RowSeq x{s.first, s.count, s.keys, 0, 0};
     int rows = s.count * a.group;
     if (rows < a.min_rows || rows > a.max_rows) return x;
-    if (rows > kRows || rows > a.row_cap) {  // more tokens than the call said: the first ones only
+    if (rows > kMostRows || rows > a.row_cap) {  // more tokens than the call said: the first ones only
         flag_index_error(a.err_word);
-        x.count = min(kRows, a.row_cap) / a.group;
+        x.count = min(kMostRows, a.row_cap) / a.group;
         if (x.count == 0) return x;
         x.keys = max(0, min(s.keys, s.keys - s.count + x.count));
     }
@@ -129,6 +125,9 @@ __device__ __forceinline__ void mma_16816(float (&d)[4], const uint32_t (&a)[4],
         "{%0,%1,%2,%3};"
         : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
         : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ void prefetch_l1(const void* p) {
+    asm volatile("prefetch.global.L1 [%0];" ::"l"(p));
 }
 __device__ __forceinline__ void fence_async_smem() {
     asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
@@ -160,14 +159,10 @@ struct Ranges {
     }
 };
 
-template <int MT>
 __global__ void __launch_bounds__(kRowThreadsTotal, 1)
 fmha_paged_rows_kernel(const __grid_constant__ Args a) {
-    using Shared = RowsShared<MT>;
-    constexpr int kRows = Shared::kRows;
-    constexpr int kStages = Shared::kStages;
     extern __shared__ uint8_t smem_raw[];
-    Shared& sm = *reinterpret_cast<Shared*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) &
+    RowsShared& sm = *reinterpret_cast<RowsShared*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) &
                                             ~uintptr_t(1023));
     const int warp = threadIdx.x >> 5;
     const int lane = threadIdx.x & 31;
@@ -177,7 +172,7 @@ fmha_paged_rows_kernel(const __grid_constant__ Args a) {
     if (lane == 0) {
         tma_prefetch_desc(&a.tm_k);
         tma_prefetch_desc(&a.tm_v);
-        for (int s = 0; s < kStages; ++s) mbar_init(smem_u32(&sm.bar[warp][s]), 1);
+        for (int s = 0; s < kRowStages; ++s) mbar_init(smem_u32(&sm.bar[warp][s]), 1);
         sm.piece_job[warp][0] = sm.piece_job[warp][1] = -1;
         if (warp == 0) sm.abort_flag = 0;
         fence_barrier_init();
@@ -187,7 +182,7 @@ fmha_paged_rows_kernel(const __grid_constant__ Args a) {
     const int per = (a.batch + kRowThreadsTotal - 1) / kRowThreadsTotal;
     const int b0 = min(a.batch, (int)threadIdx.x * per), b1 = min(a.batch, b0 + per);
     int mine = 0;
-    for (int b = b0; b < b1; ++b) mine += load_row_seq<kRows>(a, b).units;
+    for (int b = b0; b < b1; ++b) mine += load_row_seq(a, b).units;
     int incl = mine;
 #pragma unroll
     for (int d = 1; d < 32; d <<= 1) {
@@ -216,7 +211,7 @@ fmha_paged_rows_kernel(const __grid_constant__ Args a) {
     if (beg >= before && beg < before + mine) {
         unsigned p = before;
         for (int b = b0; b < b1; ++b) {
-            const unsigned n = load_row_seq<kRows>(a, b).units;
+            const unsigned n = load_row_seq(a, b).units;
             if (beg < p + n) {
                 sm.start_b = b;
                 sm.start_u = (int)(beg - p);
@@ -241,7 +236,7 @@ fmha_paged_rows_kernel(const __grid_constant__ Args a) {
         if (k.left <= 0) return false;
         do {
             if (++k.b >= a.batch) return false;
-            k.x = load_row_seq<kRows>(a, k.b);
+            k.x = load_row_seq(a, k.b);
         } while (k.x.units == 0);
         ++k.seg;
         k.n = min(k.x.units, k.left);
@@ -257,12 +252,12 @@ fmha_paged_rows_kernel(const __grid_constant__ Args a) {
     const unsigned long long tiles = (unsigned long long)(end - beg) * a.nhead_k;
     const unsigned long long from = tiles * warp / kRowWarps;
     const long long count = (long long)(tiles * (warp + 1) / kRowWarps - from);
-    RowsHeader header{0, 0};
+    RowsHeader header{0, 0, 0, 0};
     bool waited = false;
     if (count > 0 || warp == 0) {
         Cursor c;
         c.b = sm.start_b;
-        c.x = load_row_seq<kRows>(a, c.b);
+        c.x = load_row_seq(a, c.b);
         c.seg = 0;
         c.left = (int)(end - beg);
         c.unit0 = sm.start_u;
@@ -273,7 +268,8 @@ fmha_paged_rows_kernel(const __grid_constant__ Args a) {
             while (k.left > k.n && next_seq(k)) {}
             const int after = k.x.units - k.unit0 - k.n;
             if (k.unit0 == 0 && after > 0) {
-                header.b = k.b;
+                header.first = k.x.first;
+                header.rows = k.x.count * a.group;
                 header.parts = (int)(ranges.owner(end + after - 1) - blockIdx.x) + 1;
             }
         }
@@ -298,7 +294,7 @@ fmha_paged_rows_kernel(const __grid_constant__ Args a) {
         };
         const uint64_t policy = l2_policy_evict_first();
         auto produce = [&]() {
-            while (to_issue > 0 && issued - done < kStages) {
+            while (to_issue > 0 && issued - done < kRowStages) {
                 if (p.x.kv_end > 0) {
                     const int key0 = (p.unit0 + p.u) * kUnit;
                     const int pages = (p.x.keys + (1 << a.page_shift) - 1) >> a.page_shift;
@@ -314,7 +310,7 @@ fmha_paged_rows_kernel(const __grid_constant__ Args a) {
                         ids_next = load_ids(win + 32, pages);
                     }
                     const int nbox = min(boxes, (p.x.kv_end - key0 + box_rows - 1) / box_rows);
-                    const int slot = issued % kStages;
+                    const int slot = issued % kRowStages;
                     const uint32_t bar = smem_u32(&sm.bar[warp][slot]);
                     if (lane == 0) mbar_arrive_expect_tx(bar, 2 * nbox * box_rows * kHeadDim * 2);
                     __syncwarp();
@@ -332,14 +328,24 @@ fmha_paged_rows_kernel(const __grid_constant__ Args a) {
                 }
                 advance(p);
                 --to_issue;
+                if (p.u == 0 && to_issue > 0) {
+                    // A new head: its query rows, and at a new sequence the next
+                    // one's page ids, will be wanted without delay.
+                    if (lane < p.x.count * a.group) {
+                        const int t = lane / a.group;
+                        prefetch_l1(q_row(a, p.x.first + t, p.h * a.group + lane - t * a.group));
+                    }
+                    if (p.h == 0 && lane == 31 && p.b + 1 < a.batch)
+                        prefetch_l1(a.page_table + (p.b + 1) * a.table_stride);
+                }
             }
         };
         produce();
 
         const int g = lane >> 2, t4 = lane & 3;
-        uint32_t qf[MT][4][4];
-        float o[MT][8][4], m[MT][2], l[MT][2];
-        int lim[MT][2];
+        uint32_t qf[4][4];
+        float o[8][4], m[2], l[2];
+        int lim[2];
         int u0 = 0;
         bool ok = true;
         for (long long it = 0; it < count; ++it) {
@@ -347,36 +353,33 @@ fmha_paged_rows_kernel(const __grid_constant__ Args a) {
             if (it == 0 || c.u == 0) {
                 u0 = c.u;
 #pragma unroll
-                for (int i = 0; i < MT; ++i) {
-#pragma unroll
-                    for (int hr = 0; hr < 2; ++hr) {
-                        const int r = i * 16 + hr * 8 + g;
-                        m[i][hr] = -INFINITY;
-                        l[i][hr] = 0.0f;
-                        lim[i][hr] = 0;
-                        const uint32_t* src = nullptr;
-                        if (r < rows) {
-                            const int t = r / a.group;
-                            lim[i][hr] = key_limit(a, Sequence{c.x.first, c.x.count, c.x.keys}, t);
-                            src = reinterpret_cast<const uint32_t*>(
-                                q_row(a, c.x.first + t, c.h * a.group + r - t * a.group));
-                        }
-#pragma unroll
-                        for (int kk = 0; kk < 4; ++kk) {
-                            qf[i][kk][hr] = src ? __ldg(src + kk * 8 + t4) : 0u;
-                            qf[i][kk][hr + 2] = src ? __ldg(src + kk * 8 + 4 + t4) : 0u;
-                        }
+                for (int hr = 0; hr < 2; ++hr) {
+                    const int r = hr * 8 + g;
+                    m[hr] = -INFINITY;
+                    l[hr] = 0.0f;
+                    lim[hr] = 0;
+                    const uint32_t* src = nullptr;
+                    if (r < rows) {
+                        const int t = r / a.group;
+                        lim[hr] = key_limit(a, Sequence{c.x.first, c.x.count, c.x.keys}, t);
+                        src = reinterpret_cast<const uint32_t*>(
+                            q_row(a, c.x.first + t, c.h * a.group + r - t * a.group));
                     }
 #pragma unroll
-                    for (int n = 0; n < 8; ++n)
-#pragma unroll
-                        for (int q = 0; q < 4; ++q) o[i][n][q] = 0.0f;
+                    for (int kk = 0; kk < 4; ++kk) {
+                        qf[kk][hr] = src ? __ldg(src + kk * 8 + t4) : 0u;
+                        qf[kk][hr + 2] = src ? __ldg(src + kk * 8 + 4 + t4) : 0u;
+                    }
                 }
+#pragma unroll
+                for (int n = 0; n < 8; ++n)
+#pragma unroll
+                    for (int q = 0; q < 4; ++q) o[n][q] = 0.0f;
             }
             if (c.x.kv_end > 0) {
-                const int slot = done % kStages;
+                const int slot = done % kRowStages;
                 const bool got =
-                    wait_phase(smem_u32(&sm.bar[warp][slot]), (done / kStages) & 1, abort_flag, a);
+                    wait_phase(smem_u32(&sm.bar[warp][slot]), (done / kRowStages) & 1, abort_flag, a);
                 if (!__all_sync(0xffffffffu, got)) {
                     ok = false;
                     break;
@@ -392,13 +395,11 @@ fmha_paged_rows_kernel(const __grid_constant__ Args a) {
                     __syncwarp();
                 }
                 // S = Q K^T
-                float s[MT][4][4];
+                float s[4][4];
 #pragma unroll
-                for (int i = 0; i < MT; ++i)
+                for (int n = 0; n < 4; ++n)
 #pragma unroll
-                    for (int n = 0; n < 4; ++n)
-#pragma unroll
-                        for (int q = 0; q < 4; ++q) s[i][n][q] = 0.0f;
+                    for (int q = 0; q < 4; ++q) s[n][q] = 0.0f;
 #pragma unroll
                 for (int kk = 0; kk < 4; ++kk)
 #pragma unroll
@@ -407,53 +408,54 @@ fmha_paged_rows_kernel(const __grid_constant__ Args a) {
                         const int chunk = (2 * kk + ((lane >> 3) & 1)) ^ (row & 7);
                         uint32_t kb[4];
                         ldsm4(ks + row * 128 + chunk * 16, kb);
-#pragma unroll
-                        for (int i = 0; i < MT; ++i) {
-                            mma_16816(s[i][2 * j], qf[i][kk], kb[0], kb[1]);
-                            mma_16816(s[i][2 * j + 1], qf[i][kk], kb[2], kb[3]);
-                        }
+                        mma_16816(s[2 * j], qf[kk], kb[0], kb[1]);
+                        mma_16816(s[2 * j + 1], qf[kk], kb[2], kb[3]);
                     }
                 // Running maximum, weights, and their two bf16 parts.
-                uint32_t ph[MT][2][4], pl[MT][2][4];
+                uint32_t ph[2][4], pl[2][4];
 #pragma unroll
-                for (int i = 0; i < MT; ++i)
+                for (int hr = 0; hr < 2; ++hr) {
+                    if (hr == 1 && rows <= 8) {  // no such rows
 #pragma unroll
-                    for (int hr = 0; hr < 2; ++hr) {
-                        if (key0 + kUnit > lim[i][hr]) {
-#pragma unroll
-                            for (int n = 0; n < 4; ++n)
-#pragma unroll
-                                for (int q = 0; q < 2; ++q)
-                                    if (key0 + n * 8 + 2 * t4 + q >= lim[i][hr]) s[i][n][2 * hr + q] = -INFINITY;
-                        }
-                        float mx = -INFINITY;
-#pragma unroll
-                        for (int n = 0; n < 4; ++n) mx = fmax3(mx, s[i][n][2 * hr], s[i][n][2 * hr + 1]);
-                        mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
-                        mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
-                        const float mn = fmaxf(m[i][hr], mx * a.scale);
-                        const float mu = mn == -INFINITY ? 0.0f : mn;
-                        const float keep = ex2_approx(m[i][hr] - mu);
-                        m[i][hr] = mn;
-                        float sum = 0.0f;
-#pragma unroll
-                        for (int n = 0; n < 4; ++n) {
-                            const float p0 = ex2_approx(fmaf(s[i][n][2 * hr], a.scale, -mu));
-                            const float p1 = ex2_approx(fmaf(s[i][n][2 * hr + 1], a.scale, -mu));
-                            sum += p0 + p1;
-                            const uint32_t hi = pack_bf16_rne(p0, p1);
-                            ph[i][n >> 1][hr + 2 * (n & 1)] = hi;
-                            pl[i][n >> 1][hr + 2 * (n & 1)] =
-                                pack_bf16_rne(p0 - __uint_as_float(hi << 16),
-                                              p1 - __uint_as_float(hi & 0xffff0000u));
-                        }
-                        l[i][hr] = l[i][hr] * keep + sum;
-#pragma unroll
-                        for (int n = 0; n < 8; ++n) {
-                            o[i][n][2 * hr] *= keep;
-                            o[i][n][2 * hr + 1] *= keep;
-                        }
+                        for (int n = 0; n < 4; ++n)
+                            ph[n >> 1][1 + 2 * (n & 1)] = pl[n >> 1][1 + 2 * (n & 1)] = 0;
+                        break;
                     }
+                    if (key0 + kUnit > lim[hr]) {
+#pragma unroll
+                        for (int n = 0; n < 4; ++n)
+#pragma unroll
+                            for (int q = 0; q < 2; ++q)
+                                if (key0 + n * 8 + 2 * t4 + q >= lim[hr]) s[n][2 * hr + q] = -INFINITY;
+                    }
+                    float mx = -INFINITY;
+#pragma unroll
+                    for (int n = 0; n < 4; ++n) mx = fmax3(mx, s[n][2 * hr], s[n][2 * hr + 1]);
+                    mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
+                    mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
+                    const float mn = fmaxf(m[hr], mx * a.scale);
+                    const float mu = mn == -INFINITY ? 0.0f : mn;
+                    const float keep = ex2_approx(m[hr] - mu);
+                    m[hr] = mn;
+                    float sum = 0.0f;
+#pragma unroll
+                    for (int n = 0; n < 4; ++n) {
+                        const float p0 = ex2_approx(fmaf(s[n][2 * hr], a.scale, -mu));
+                        const float p1 = ex2_approx(fmaf(s[n][2 * hr + 1], a.scale, -mu));
+                        sum += p0 + p1;
+                        const uint32_t hi = pack_bf16_rne(p0, p1);
+                        ph[n >> 1][hr + 2 * (n & 1)] = hi;
+                        pl[n >> 1][hr + 2 * (n & 1)] =
+                            pack_bf16_rne(p0 - __uint_as_float(hi << 16),
+                                          p1 - __uint_as_float(hi & 0xffff0000u));
+                    }
+                    l[hr] = l[hr] * keep + sum;
+#pragma unroll
+                    for (int n = 0; n < 8; ++n) {
+                        o[n][2 * hr] *= keep;
+                        o[n][2 * hr + 1] *= keep;
+                    }
+                }
                 // O += P V
 #pragma unroll
                 for (int st = 0; st < 2; ++st)
@@ -463,13 +465,10 @@ fmha_paged_rows_kernel(const __grid_constant__ Args a) {
                         const int chunk = (2 * dp + (lane >> 4)) ^ (row & 7);
                         uint32_t vb[4];
                         ldsm4_t(vs + row * 128 + chunk * 16, vb);
-#pragma unroll
-                        for (int i = 0; i < MT; ++i) {
-                            mma_16816(o[i][2 * dp], ph[i][st], vb[0], vb[1]);
-                            mma_16816(o[i][2 * dp], pl[i][st], vb[0], vb[1]);
-                            mma_16816(o[i][2 * dp + 1], ph[i][st], vb[2], vb[3]);
-                            mma_16816(o[i][2 * dp + 1], pl[i][st], vb[2], vb[3]);
-                        }
+                        mma_16816(o[2 * dp], ph[st], vb[0], vb[1]);
+                        mma_16816(o[2 * dp], pl[st], vb[0], vb[1]);
+                        mma_16816(o[2 * dp + 1], ph[st], vb[2], vb[3]);
+                        mma_16816(o[2 * dp + 1], pl[st], vb[2], vb[3]);
                     }
                 ++done;
                 __syncwarp();
@@ -481,28 +480,24 @@ fmha_paged_rows_kernel(const __grid_constant__ Args a) {
                 // for the block's fold.
                 const bool all = u0 == 0 && c.u + 1 == c.n;
                 const bool empty = c.x.kv_end == 0;  // no slot was read, and O is zero
-                float* po = all ? reinterpret_cast<float*>(sm.ring[warp][(done + kStages - 1) % kStages])
+                float* po = all ? reinterpret_cast<float*>(sm.ring[warp][(done + kRowStages - 1) % kRowStages])
                           : last ? reinterpret_cast<float*>(sm.ring[warp]) : sm.first_o[warp];
-                float* pml = all && !Shared::kSlotTakesAll ? sm.out_ml[warp]
-                             : all || last              ? po + kRows * kHeadDim
-                                                        : sm.first_ml[warp];
+                float* pml = all || last ? po + kMostRows * kHeadDim : sm.first_ml[warp];
                 const Target to{c.x.first, rows, c.h,
                                 c.unit0 == 0 && c.n == c.x.units ? -1 : 2 * (int)blockIdx.x + (c.unit0 == 0)};
                 if (!empty) {
 #pragma unroll
-                    for (int i = 0; i < MT; ++i)
+                    for (int hr = 0; hr < 2; ++hr) {
+                        float lt = l[hr];
+                        lt += __shfl_xor_sync(0xffffffffu, lt, 1);
+                        lt += __shfl_xor_sync(0xffffffffu, lt, 2);
+                        const int rt = hr * 8 + g;
 #pragma unroll
-                        for (int hr = 0; hr < 2; ++hr) {
-                            float lt = l[i][hr];
-                            lt += __shfl_xor_sync(0xffffffffu, lt, 1);
-                            lt += __shfl_xor_sync(0xffffffffu, lt, 2);
-                            const int rt = i * 16 + hr * 8 + g;
-#pragma unroll
-                            for (int n = 0; n < 8; ++n)
-                                *reinterpret_cast<float2*>(po + rt * kHeadDim + n * 8 + 2 * t4) =
-                                    make_float2(o[i][n][2 * hr], o[i][n][2 * hr + 1]);
-                            if (t4 == 0) *reinterpret_cast<float2*>(pml + rt * 2) = make_float2(m[i][hr], lt);
-                        }
+                        for (int n = 0; n < 8; ++n)
+                            *reinterpret_cast<float2*>(po + rt * kHeadDim + n * 8 + 2 * t4) =
+                                make_float2(o[n][2 * hr], o[n][2 * hr + 1]);
+                        if (t4 == 0) *reinterpret_cast<float2*>(pml + rt * 2) = make_float2(m[hr], lt);
+                    }
                     __syncwarp();
                 }
                 if (all) {
@@ -530,7 +525,7 @@ fmha_paged_rows_kernel(const __grid_constant__ Args a) {
         }
         if (!ok)
             for (int i = done; i < issued; ++i)
-                drain_phase(smem_u32(&sm.bar[warp][i % kStages]), (i / kStages) & 1, a);
+                drain_phase(smem_u32(&sm.bar[warp][i % kRowStages]), (i / kRowStages) & 1, a);
     }
 
     // --------------------------------------------- the block's fold of pieces
@@ -538,39 +533,40 @@ fmha_paged_rows_kernel(const __grid_constant__ Args a) {
     if (threadIdx.x == 0) piece_headers(a)[blockIdx.x] = header;
     __syncthreads();
     if (*abort_flag) return;
+    // Runs of pieces of one head, in line order: run k is the pieces from the
+    // k-th marked one to the next (every warp finds the same).
+    const int my_job = lane < 2 * kRowWarps ? sm.piece_job[lane >> 1][lane & 1] : -1;
+    const unsigned have = __ballot_sync(0xffffffffu, my_job >= 0);
+    const unsigned below = have & ((1u << lane) - 1);
+    const int job_before = __shfl_sync(0xffffffffu, my_job, below ? 31 - __clz(below) : 0);
+    const bool begins = my_job >= 0 && (below == 0 || job_before != my_job);
+    const unsigned runs = __ballot_sync(0xffffffffu, begins);
+    if (begins) sm.run[__popc(runs & ((1u << lane) - 1))] = lane;  // the same from every warp
+    if (lane == 0) sm.run[__popc(runs)] = 2 * kRowWarps;
+    __syncwarp();
+    // 16 threads per (run, row).
     const int c4 = threadIdx.x & 15;
-    for (int i = 0; i < 2 * kRowWarps;) {
-        const int job = sm.piece_job[i >> 1][i & 1];
-        int next = i + 1;
-        if (job >= 0) {
-            while (next < 2 * kRowWarps) {
-                const int j = sm.piece_job[next >> 1][next & 1];
-                if (j >= 0 && j != job) break;
-                ++next;
-            }
-            const Target to = sm.piece_to[i >> 1][i & 1];
-            for (int rt = threadIdx.x >> 4; rt < to.rows; rt += kRowThreadsTotal / 16) {
-                float m = -INFINITY, l = 0.0f;
-                float4 o = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-                for (int k = i; k < next; ++k) {
-                    if (sm.piece_job[k >> 1][k & 1] < 0) continue;
-                    const float* po = (k & 1) ? reinterpret_cast<const float*>(sm.ring[k >> 1])
-                                              : sm.first_o[k >> 1];
-                    const float* pml = (k & 1) ? po + kRows * kHeadDim : sm.first_ml[k >> 1];
-                    fold4(m, l, o, pml[rt * 2], pml[rt * 2 + 1],
-                          *reinterpret_cast<const float4*>(po + rt * kHeadDim + c4 * 4));
-                }
-                emit_row4(a, to, rt, c4, m, l, o);
-            }
+    for (int x = threadIdx.x >> 4; x < __popc(runs) * a.row_cap; x += kRowThreadsTotal / 16) {
+        const int k = x / a.row_cap, rt = x - k * a.row_cap;
+        const int i = sm.run[k], next = sm.run[k + 1];
+        const Target to = sm.piece_to[i >> 1][i & 1];
+        if (rt >= to.rows) continue;
+        float m = -INFINITY, l = 0.0f;
+        float4 o = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+        for (int j = i; j < next; ++j) {
+            if (!((have >> j) & 1)) continue;
+            const float* po = (j & 1) ? reinterpret_cast<const float*>(sm.ring[j >> 1]) : sm.first_o[j >> 1];
+            const float* pml = (j & 1) ? po + kMostRows * kHeadDim : sm.first_ml[j >> 1];
+            fold4(m, l, o, pml[rt * 2], pml[rt * 2 + 1],
+                  *reinterpret_cast<const float4*>(po + rt * kHeadDim + c4 * 4));
         }
-        i = next;
+        emit_row4(a, to, rt, c4, m, l, o);
     }
 }
 
 // Folds the pieces of the sequence that begins in block blockIdx.x and goes on
 // in the blocks after it.  64 threads per row: 16 cover the columns, the four
 // sixteens take every fourth piece, kBatch of them in flight.
-template <int MT>
 __global__ void __launch_bounds__(256)
 fmha_paged_rows_merge(const __grid_constant__ Args a) {
     constexpr int kBatch = 8;
@@ -579,8 +575,7 @@ fmha_paged_rows_merge(const __grid_constant__ Args a) {
     griddep_wait();
     const RowsHeader hd = piece_headers(a)[blockIdx.x];
     if (hd.parts == 0) return;
-    const RowSeq x = load_row_seq<16 * MT>(a, hd.b);
-    const int rows = x.count * a.group;
+    const int rows = hd.rows;
     const int y = blockIdx.y * 4 + (int)(threadIdx.x >> 6);
     const bool has_row = y < rows * a.nhead_k;
     const int h = has_row ? y / rows : 0, rt = has_row ? y - h * rows : 0;
@@ -617,7 +612,7 @@ fmha_paged_rows_merge(const __grid_constant__ Args a) {
     __syncthreads();
     if (has_row && !(threadIdx.x & 32) && lane < 16) {
         fold4(m, l, o, other_ml[slot][c4].x, other_ml[slot][c4].y, other_o[slot][c4]);
-        emit_row4(a, Target{x.first, rows, h, -1}, rt, c4, m, l, o);
+        emit_row4(a, Target{hd.first, rows, h, -1}, rt, c4, m, l, o);
     }
 }
 

@@ -29,10 +29,15 @@
 // would need twice the tensor pipe's time; a quarter of the exponentials
 // therefore runs as a polynomial on the FMA pipe.
 //
-// Few row tiles: each tile's keys are cut into `splits` equal ranges, a block
-// each, whose normalised results are folded by fmha_paged_combine (or by the
-// rows kernel that ends a prefix call).
+// Work split.  A shared prefix has one length, so the host cuts every row
+// tile's keys into `splits` equal ranges, a block each, and whatever ends the
+// call folds their results.  Sequences' own keys differ as they like: the
+// blocks themselves agree, from the lengths, on a range length that makes about
+// one or two ranges per resident block, cut each (row tile, head) job into that
+// many equal ranges, and take one range each (find_item); jobs of one range go
+// to the output, the others through scratch slots that fmha_paged_combine folds.
 #pragma once
+#include <climits>
 #include <type_traits>
 
 #include "paged_common.cuh"
@@ -51,6 +56,7 @@ constexpr uint32_t kColS = 0, kColO = 128, kColP = 192;
 constexpr int kTileRegsSoftmax = 192, kTileRegsControl = 64;
 static_assert(128 * (kTileRegsSoftmax + kTileRegsControl) <= kTileThreads * 128, "register split");
 constexpr float kLazyLog2 = 8.0f;
+constexpr int kLongRange = 16;  // key tiles of a range from which blocks take two
 constexpr int kPolyOf16 = 4;  // pairs of every 16 whose exponential runs on the FMA pipe
 
 struct alignas(1024) TileShared {
@@ -66,9 +72,28 @@ struct alignas(1024) TileShared {
     uint64_t bar_drain;
     uint32_t tmem_base;
     int abort_flag;
-    int warp_tiles[8];
-    int found_b, found_m, found_total;
+    long long scan_keys[8];
+    int scan_a[8], scan_b[8];
+    int item[5];
 };
+
+// Scratch of the jobs that several blocks share.
+constexpr int kMaxTileSlots = 4 * kTileBlocks;
+constexpr int kMaxPlanned = 8000;  // row tiles and sequences up to which find_item plans
+struct TileHeader {
+    int b, m, h;  // the job
+    int parts;    // its ranges, in the slots from this one on, nhead_k apart; 0: no job begins here
+};
+__host__ __device__ constexpr size_t tile_slot_floats() { return (size_t)kTileM * (kHeadDim + 1); }
+__device__ __forceinline__ float* tile_slot_o(const Args& a, int slot) {
+    return a.slots + (size_t)slot * kTileM * kHeadDim;
+}
+__device__ __forceinline__ float* tile_slot_lse(const Args& a, int slot) {
+    return a.slots + (size_t)a.max_slots * kTileM * kHeadDim + (size_t)slot * kTileM;
+}
+__device__ __forceinline__ TileHeader* tile_headers(const Args& a) {
+    return reinterpret_cast<TileHeader*>(a.slots + (size_t)a.max_slots * tile_slot_floats());
+}
 
 // 2^x for a pair on the FMA and integer pipes: x = n + f, n = round(x), and a
 // degree-4 minimax polynomial for 2^f on [-1/2, 1/2] (relative error 3e-6,
@@ -89,54 +114,165 @@ __device__ __forceinline__ float2 exp2_poly4(float2 x) {
                        __uint_as_float(__float_as_uint(p.y) + (__float_as_uint(t.y) << 23)));
 }
 
-// Row tile `slot` of the grid -> (sequence, tile), tiles of later tokens (the
-// ones with more keys) first.  All threads; false: past the last tile.
-__device__ __forceinline__ bool find_tile(const Args& a, TileShared& sm, int slot, int& b, int& m) {
-    if (a.seqstart_q == nullptr) {
-        const int tiles = (a.seqlen_q * a.group + kTileM - 1) / kTileM;
-        m = tiles - 1 - slot / a.batch;
-        b = slot % a.batch;
-        return m >= 0;
-    }
-    auto tiles_of = [&](int i) {
-        const int rows = load_sequence(a, i).count * a.group;
-        return rows < a.min_rows || rows > a.max_rows ? 0 : (rows + kTileM - 1) / kTileM;
-    };
-    const int per = (a.batch + kTileThreads - 1) / kTileThreads;
-    const int b0 = min(a.batch, (int)threadIdx.x * per), b1 = min(a.batch, b0 + per);
+// A block's work: range k of `parts` of the keys of row tile m of sequence b.
+static_assert((2 * kMaxPlanned + 1) * 4 <= kTileStages * kTileBytes, "find_item's integers fit the ring");
+struct Item {
+    int b, m, k, parts;
+    int slot;  // scratch slot of the job's first range (where parts > 1), for head 0
+};
+
+// Exclusive scan of `mine` over the block; `total` = the sum.
+template <typename T>
+__device__ __forceinline__ T block_scan(T mine, T (&warp_sums)[8], T& total) {
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    int mine = 0;
-    for (int i = b0; i < b1; ++i) mine += tiles_of(i);
-    int incl = mine;
+    T incl = mine;
 #pragma unroll
     for (int d = 1; d < 32; d <<= 1) {
-        const int v = __shfl_up_sync(0xffffffffu, incl, d);
+        const T v = __shfl_up_sync(0xffffffffu, incl, d);
         if (lane >= d) incl += v;
     }
-    if (lane == 31) sm.warp_tiles[warp] = incl;
+    if (lane == 31) warp_sums[warp] = incl;
     __syncthreads();
-    int before = incl - mine, total = 0;
+    T before = incl - mine;
+    total = 0;
 #pragma unroll
     for (int w = 0; w < 8; ++w) {
-        if (w < warp) before += sm.warp_tiles[w];
-        total += sm.warp_tiles[w];
+        if (w < warp) before += warp_sums[w];
+        total += warp_sums[w];
     }
-    if (slot >= total) return false;
-    const int x = total - 1 - slot;
-    if (x >= before && x < before + mine) {
-        for (int i = b0, p = before; i < b1; ++i) {
-            const int n = tiles_of(i);
-            if (x < p + n) {
-                sm.found_b = i;
-                sm.found_m = x - p;
-                break;
-            }
-            p += n;
+    return before;
+}
+
+__device__ __forceinline__ int tile_count(const Args& a, const Sequence& s) {
+    const int rows = s.count * a.group;
+    return rows < a.min_rows || rows > a.max_rows ? 0 : (rows + kTileM - 1) / kTileM;
+}
+__device__ __forceinline__ int tile_kv_end(const Args& a, const Sequence& s, int m) {
+    const int row_end = min(s.count * a.group, (m + 1) * kTileM);
+    return max(0, key_limit(a, s, (row_end - 1) / a.group));
+}
+
+// Item `y` of the grid, tiles of later tokens (the ones with more keys) first.
+// All threads; `ints` is shared memory for 2 * kMaxPlanned + 1 integers.
+// False: past the last one.
+__device__ __forceinline__ bool find_item(const Args& a, TileShared& sm, int* ints, int y, Item& it) {
+    const bool packed = a.seqstart_q != nullptr;
+    if (!a.plan) {
+        // Every tile whole (or cut as the host said), without a look at the lengths.
+        it.k = y % a.splits;
+        it.parts = a.splits;
+        it.slot = 0;
+        const int x = y / a.splits;
+        if (!packed) {
+            const int tiles = (a.seqlen_q * a.group + kTileM - 1) / kTileM;
+            it.m = tiles - 1 - x / a.batch;
+            it.b = x % a.batch;
+            return it.m >= 0;
         }
     }
+    // First row tile of every sequence.
+    const int tid = threadIdx.x;
+    int* first = ints;
+    int tiles;
+    if (packed) {
+        const int per = (a.batch + kTileThreads - 1) / kTileThreads;
+        const int b0 = min(a.batch, tid * per), b1 = min(a.batch, b0 + per);
+        int mine = 0;
+        for (int b = b0; b < b1; ++b) mine += tile_count(a, load_sequence(a, b));
+        int p = block_scan(mine, sm.scan_a, tiles);
+        if (!a.plan) {
+            const int x = tiles - 1 - y / a.splits;
+            if (x < 0) return false;
+            if (x >= p && x < p + mine)
+                for (int b = b0; b < b1; ++b) {
+                    const int n = tile_count(a, load_sequence(a, b));
+                    if (x < p + n) {
+                        sm.item[0] = b;
+                        sm.item[1] = x - p;
+                        break;
+                    }
+                    p += n;
+                }
+            __syncthreads();
+            it.b = sm.item[0];
+            it.m = sm.item[1];
+            return true;
+        }
+        for (int b = b0; b < b1; ++b) {
+            first[b] = p;
+            p += tile_count(a, load_sequence(a, b));
+        }
+        if (tid == 0) first[a.batch] = tiles;
+        __syncthreads();
+    } else {
+        tiles = a.batch * ((a.seqlen_q * a.group + kTileM - 1) / kTileM);
+    }
+    tiles = min(tiles, kMaxPlanned);  // more only if the prefix sums overlap
+    const int per_seq = packed ? 1 : tiles / a.batch;
+    auto sequence_of = [&](int t, int& m) {
+        if (!packed) {
+            m = t % per_seq;
+            return t / per_seq;
+        }
+        int lo = 0, hi = a.batch;  // the last one with first <= t
+        while (hi - lo > 1) {
+            const int mid = (lo + hi) >> 1;
+            if (first[mid] <= t) lo = mid;
+            else hi = mid;
+        }
+        m = t - first[lo];
+        return lo;
+    };
+    // Key tiles of every row tile, and the range length.
+    int* keys = ints + kMaxPlanned + 1;
+    const int per = (tiles + kTileThreads - 1) / kTileThreads;
+    const int t0 = min(tiles, tid * per), t1 = min(tiles, t0 + per);
+    long long mine = 0, total;
+    for (int t = t0; t < t1; ++t) {
+        int m;
+        const int b = sequence_of(t, m);
+        const int n = max(1, (tile_kv_end(a, load_sequence(a, b), m) + kTileN - 1) / kTileN);
+        keys[t] = n;
+        mine += n;
+    }
+    block_scan(mine, sm.scan_keys, total);
+    total *= a.nhead_k;
+    // One range per resident block while ranges are short, two beyond.
+    long long len = (total + kTileBlocks - 1) / kTileBlocks;
+    if (len > kLongRange) len = max((long long)kLongRange, (total + 2 * kTileBlocks - 1) / (2 * kTileBlocks));
+    const int most = (int)min(len, (long long)INT_MAX);
+    auto parts_of = [&](int n) { return (n + most - 1) / most; };
+    int items_mine = 0, split_mine = 0;
+    for (int t = t0; t < t1; ++t) {
+        const int p = parts_of(keys[t]);
+        items_mine += p;
+        if (p > 1) split_mine += p;
+    }
+    int items, split;
+    int items_before = block_scan(items_mine, sm.scan_a, items);
+    int split_before = block_scan(split_mine, sm.scan_b, split);
+    // No job begins in the slots that stay unused.
+    if (blockIdx.x % a.nhead_k == 0)
+        for (int i = split * a.nhead_k + (int)(blockIdx.x / a.nhead_k) * kTileThreads + tid; i < a.max_slots;
+             i += (int)(gridDim.x / a.nhead_k) * kTileThreads)
+            tile_headers(a)[i].parts = 0;
+    const int x = items - 1 - y;
+    if (x < 0) return false;
+    if (x >= items_before && x < items_before + items_mine)
+        for (int t = t0; t < t1; ++t) {
+            const int p = parts_of(keys[t]);
+            if (x < items_before + p) {
+                sm.item[0] = sequence_of(t, sm.item[1]);
+                sm.item[2] = x - items_before;
+                sm.item[3] = p;
+                sm.item[4] = split_before;
+                break;
+            }
+            items_before += p;
+            if (p > 1) split_before += p;
+        }
     __syncthreads();
-    b = sm.found_b;
-    m = sm.found_m;
+    it = Item{sm.item[0], sm.item[1], sm.item[2], sm.item[3], sm.item[4] * a.nhead_k};
     return true;
 }
 
@@ -152,22 +288,26 @@ fmha_paged_tile_kernel(const __grid_constant__ Args a) {
     // blocks run; it waits for their results where it needs them.
     griddep_launch_dependents();
 
-    // Blocks in order: row tile, K/V head, key range.
-    const int split = blockIdx.x % a.splits;
-    const int head_slot = blockIdx.x / a.splits;
-    const int kvh = head_slot % a.nhead_k;
-    int b, mt;
-    if (!find_tile(a, sm, head_slot / a.nhead_k, b, mt)) return;
-    const Sequence seq = load_sequence(a, b);
+    // Neighbouring blocks take the heads of one key range: they read
+    // neighbouring lines of memory at the same time.
+    const int kvh = blockIdx.x % a.nhead_k;
+    Item it;
+    if (!find_item(a, sm, reinterpret_cast<int*>(sm.kv[0]), blockIdx.x / a.nhead_k, it)) return;
+    const Sequence seq = load_sequence(a, it.b);
     const int rows = seq.count * a.group;
-    const int row0 = mt * kTileM;
+    const int row0 = it.m * kTileM;
     if (rows < a.min_rows || rows > a.max_rows || row0 >= rows) return;
     const int row_end = min(rows, row0 + kTileM);
-    const int kv_end = max(0, key_limit(a, seq, (row_end - 1) / a.group));
+    const int kv_end = tile_kv_end(a, seq, it.m);
     const int all = (kv_end + kTileN - 1) / kTileN;
-    const int chunk = (all + a.splits - 1) / a.splits;
-    const int j0 = split * chunk;
-    const int n = max(0, min(all, j0 + chunk) - j0);
+    const int j0 = (int)((long long)all * it.k / it.parts);
+    const int n = (int)((long long)all * (it.k + 1) / it.parts) - j0;
+    const bool shared_job = a.plan && it.parts > 1;  // through a scratch slot
+    const int slot_job = it.slot + it.k * a.nhead_k + kvh;
+    if (shared_job && it.k == 0 && threadIdx.x == 0)
+        tile_headers(a)[slot_job] = TileHeader{it.b, it.m, kvh, it.parts};
+    else if (shared_job && threadIdx.x == 0)
+        tile_headers(a)[slot_job].parts = 0;
     const int tail = kv_end - (j0 + n - 1) * kTileN;  // visible keys of the range's last tile
     const bool has_tail = n > 0 && tail < kTileN;
     const int active = (row_end - row0 + 31) / 32;    // softmax warps with rows
@@ -190,6 +330,8 @@ fmha_paged_tile_kernel(const __grid_constant__ Args a) {
         tmem_alloc(smem_u32(&sm.tmem_base), kTileTmemCols);
         tmem_relinquish();
     }
+    // find_item used the K/V ring: ordered before the first TMA write there.
+    asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
     tc_fence_before();
     __syncthreads();
     tc_fence_after();
@@ -209,7 +351,7 @@ fmha_paged_tile_kernel(const __grid_constant__ Args a) {
             }
             const uint64_t policy = l2_policy_evict_last();
             const int box_rows = min(1 << a.page_shift, kTileN);
-            const int32_t* table = a.page_table + b * a.table_stride;
+            const int32_t* table = a.page_table + it.b * a.table_stride;
             // Lane i loads box i of a tile: box_rows keys of one page.
             auto page_of = [&](int j) {
                 const int key = (j0 + j) * kTileN + lane * box_rows;
@@ -464,20 +606,38 @@ fmha_paged_tile_kernel(const __grid_constant__ Args a) {
                     reg_fence(o[0]);
                     reg_fence(o[1]);
                 }
-                const float inv = l_run > 0.0f ? 1.0f / l_run : 0.0f;
-                const float lse2 = l_run > 0.0f ? fmaf(m_run, scale, __log2f(l_run)) : -INFINITY;
+                float inv = l_run > 0.0f ? 1.0f / l_run : 0.0f;
+                float lse2 = l_run > 0.0f ? fmaf(m_run, scale, __log2f(l_run)) : -INFINITY;
                 auto val = [&](int col) {
                     return n > 0 ? __uint_as_float(o[col >> 5][col & 31]) * inv : 0.0f;
                 };
-                if (has_row && a.out_o != nullptr) {
-                    const long long at = (long long)split * a.tokens * a.nhead_q + flat_row(a, token, head);
-                    a.out_lse[at] = lse2;
+                float* part_o = nullptr;
+                float* part_lse = nullptr;
+                if (shared_job) {
+                    part_o = tile_slot_o(a, slot_job) + t * kHeadDim;
+                    part_lse = tile_slot_lse(a, slot_job) + t;
+                } else if (a.out_o != nullptr) {
+                    const long long at = (long long)it.k * a.tokens * a.nhead_q + flat_row(a, token, head);
+                    part_o = a.out_o + at * kHeadDim;
+                    part_lse = a.out_lse + at;
+                }
+                if (has_row && part_o != nullptr) {
+                    *part_lse = lse2;
                     if (l_run > 0.0f) {
-                        float4* dst = reinterpret_cast<float4*>(a.out_o + at * kHeadDim);
+                        float4* dst = reinterpret_cast<float4*>(part_o);
 #pragma unroll
                         for (int c = 0; c < 16; ++c)
                             dst[c] = make_float4(val(4 * c), val(4 * c + 1), val(4 * c + 2), val(4 * c + 3));
                     }
+                } else if (has_row && a.part_n > 0) {
+                    // Under a prefix: its results belong to the row, too.
+                    for (int c = 0; c < 2; ++c)
+#pragma unroll
+                        for (int e = 0; e < 32; e += 4)
+                            finish_row4(a, token, head, c * 32 + e, lse2, l_run > 0.0f ? 1.0f : 0.0f,
+                                        make_float4(c ? val(32 + e) : val(e), c ? val(33 + e) : val(e + 1),
+                                                    c ? val(34 + e) : val(e + 2), c ? val(35 + e) : val(e + 3)),
+                                        c == 0 && e == 0);
                 } else if (has_row) {
                     uint4* dst = reinterpret_cast<uint4*>(o_row(a, token, head));
 #pragma unroll
@@ -501,28 +661,55 @@ fmha_paged_tile_kernel(const __grid_constant__ Args a) {
     }
 }
 
-// Final rows from part_n partial results: 16 threads per row, one float4 of
-// columns each.  Rows of sequences outside [min_rows, max_rows] belong to
-// another launch.
-__global__ void __launch_bounds__(256)
+// Folds the ranges of the jobs that several blocks shared into final rows: a
+// block looks after the slots blockIdx.x + i * gridDim.x; 16 threads per row,
+// four columns each, kBatch ranges in flight.
+constexpr int kCombineBlocks = 148;
+constexpr int kCombineThreads = 512;
+__global__ void __launch_bounds__(kCombineThreads)
 fmha_paged_combine(const __grid_constant__ Args a) {
+    constexpr int kEach = (kMaxTileSlots + kCombineBlocks - 1) / kCombineBlocks;
+    constexpr int kBatch = 4;
     griddep_wait();
-    const long long row = ((long long)blockIdx.x * 256 + threadIdx.x) >> 4;
-    if (row >= (long long)a.tokens * a.nhead_q) return;
-    const int c4 = threadIdx.x & 15;
-    const int token = (int)(row / a.nhead_q), head = (int)(row - (long long)token * a.nhead_q);
-    if (a.seqstart_q != nullptr) {
-        int lo = 0, hi = a.batch;
-        while (hi - lo > 1) {
-            const int mid = (lo + hi) >> 1;
-            if (a.seqstart_q[mid] <= token) lo = mid;
-            else hi = mid;
-        }
-        const Sequence s = load_sequence(a, lo);
-        const int rows = s.count * a.group;
-        if (token < s.first || token >= s.first + s.count || rows < a.min_rows || rows > a.max_rows) return;
+    TileHeader head[kEach];
+#pragma unroll
+    for (int i = 0; i < kEach; ++i) {
+        const int slot = blockIdx.x + i * kCombineBlocks;
+        head[i].parts = 0;
+        if (slot < a.max_slots) head[i] = tile_headers(a)[slot];
     }
-    finish_row4(a, token, head, c4 * 4, -INFINITY, 0.0f, make_float4(0.0f, 0.0f, 0.0f, 0.0f), c4 == 0);
+    const int c4 = threadIdx.x & 15;
+#pragma unroll
+    for (int i = 0; i < kEach; ++i) {
+        if (head[i].parts == 0) continue;
+        const int slot0 = blockIdx.x + i * kCombineBlocks;
+        const Sequence seq = load_sequence(a, head[i].b);
+        const int row0 = head[i].m * kTileM;
+        const int rows = min(kTileM, seq.count * a.group - row0);
+        for (int rt = threadIdx.x >> 4; rt < rows; rt += kCombineThreads / 16) {
+            float m = -INFINITY, l = 0.0f;
+            float4 o = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+            for (int k0 = 0; k0 < head[i].parts; k0 += kBatch) {
+                float m2[kBatch];
+                float4 x[kBatch];
+#pragma unroll
+                for (int u = 0; u < kBatch; ++u) {
+                    m2[u] = -INFINITY;
+                    x[u] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+                    if (k0 + u < head[i].parts) {
+                        const int slot = slot0 + (k0 + u) * a.nhead_k;
+                        m2[u] = tile_slot_lse(a, slot)[rt];
+                        x[u] = *reinterpret_cast<const float4*>(tile_slot_o(a, slot) + rt * kHeadDim + c4 * 4);
+                    }
+                }
+#pragma unroll
+                for (int u = 0; u < kBatch; ++u)
+                    if (m2[u] != -INFINITY) fold4(m, l, o, m2[u], 1.0f, x[u]);  // else O was not written
+            }
+            const int row = row0 + rt, t = row / a.group;
+            finish_row4(a, seq.first + t, head[i].h * a.group + row - t * a.group, c4 * 4, m, l, o, c4 == 0);
+        }
+    }
 }
 
 }  // namespace fmha_paged

@@ -37,7 +37,6 @@
 // many equal ranges, and take one range each (find_item); jobs of one range go
 // to the output, the others through scratch slots that fmha_paged_combine folds.
 #pragma once
-#include <climits>
 #include <type_traits>
 
 #include "paged_common.cuh"
@@ -53,7 +52,7 @@ constexpr int kTileBlocks = 2 * 148;            // resident blocks of the device
 constexpr uint32_t kTileTmemCols = 256;
 constexpr uint32_t kColS = 0, kColO = 128, kColP = 192;
 // setmaxnreg split of the launch's 256 x 128 registers.
-constexpr int kTileRegsSoftmax = 192, kTileRegsControl = 64;
+constexpr int kTileRegsSoftmax = 184, kTileRegsControl = 72;
 static_assert(128 * (kTileRegsSoftmax + kTileRegsControl) <= kTileThreads * 128, "register split");
 constexpr float kLazyLog2 = 8.0f;
 constexpr int kLongRange = 16;  // key tiles of a range from which blocks take two
@@ -62,7 +61,6 @@ constexpr int kPolyOf16 = 4;  // pairs of every 16 whose exponential runs on the
 struct alignas(1024) TileShared {
     uint8_t q[kTileBytes];
     uint8_t kv[kTileStages][kTileBytes];
-    uint64_t bar_q;                   // Q staged (128 arrivals)
     uint64_t bar_full[kTileStages];
     uint64_t bar_empty[kTileStages];
     uint64_t bar_s;                   // S written (commit)
@@ -72,14 +70,13 @@ struct alignas(1024) TileShared {
     uint64_t bar_drain;
     uint32_t tmem_base;
     int abort_flag;
-    long long scan_keys[8];
-    int scan_a[8], scan_b[8];
-    int item[5];
+    int scan_a[8], scan_b[8], item[8];
 };
 
 // Scratch of the jobs that several blocks share.
 constexpr int kMaxTileSlots = 4 * kTileBlocks;
 constexpr int kMaxPlanned = 8000;  // row tiles and sequences up to which find_item plans
+constexpr int kMostCounted = 0x7fffffff / kMaxPlanned;  // key tiles of a row tile that a plan counts
 struct TileHeader {
     int b, m, h;  // the job
     int parts;    // its ranges, in the slots from this one on, nhead_k apart; 0: no job begins here
@@ -95,50 +92,32 @@ __device__ __forceinline__ TileHeader* tile_headers(const Args& a) {
     return reinterpret_cast<TileHeader*>(a.slots + (size_t)a.max_slots * tile_slot_floats());
 }
 
-// 2^x for a pair on the FMA and integer pipes: x = n + f, n = round(x), and a
-// degree-4 minimax polynomial for 2^f on [-1/2, 1/2] (relative error 3e-6,
-// csrc/fit_exp2_poly.py with deg = 4), scaled by 2^n in the exponent field.
-// x is finite and clamped from below.
-__device__ __forceinline__ float2 exp2_poly4(float2 x) {
-    constexpr float kRound = 12582912.0f;  // 1.5 * 2^23
-    x.x = fmaxf(x.x, -120.0f);
-    x.y = fmaxf(x.y, -120.0f);
-    const float2 t = fadd2(x, make_float2(kRound, kRound));
-    const float2 n = fadd2(t, make_float2(-kRound, -kRound));
-    const float2 f = ffma2(n, make_float2(-1.0f, -1.0f), x);
-    float2 p = ffma2(make_float2(9.570101276e-03f, 9.570101276e-03f), f, make_float2(5.591786280e-02f, 5.591786280e-02f));
-    p = ffma2(p, f, make_float2(2.402474433e-01f, 2.402474433e-01f));
-    p = ffma2(p, f, make_float2(6.931217909e-01f, 6.931217909e-01f));
-    p = ffma2(p, f, make_float2(9.999992847e-01f, 9.999992847e-01f));
-    return make_float2(__uint_as_float(__float_as_uint(p.x) + (__float_as_uint(t.x) << 23)),
-                       __uint_as_float(__float_as_uint(p.y) + (__float_as_uint(t.y) << 23)));
-}
-
 // A block's work: range k of `parts` of the keys of row tile m of sequence b.
 static_assert((2 * kMaxPlanned + 1) * 4 <= kTileStages * kTileBytes, "find_item's integers fit the ring");
+static_assert(kMaxPlanned + 2 * kTileBlocks < 32768 && 4 * kTileBlocks < 65536, "find_item's packed sums");
 struct Item {
     int b, m, k, parts;
     int slot;  // scratch slot of the job's first range (where parts > 1), for head 0
 };
 
 // Exclusive scan of `mine` over the block; `total` = the sum.
-template <typename T>
-__device__ __forceinline__ T block_scan(T mine, T (&warp_sums)[8], T& total) {
+__device__ __forceinline__ int block_scan(int mine, int (&warp_sums)[8], int& total) {
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    T incl = mine;
+    int incl = mine;
 #pragma unroll
     for (int d = 1; d < 32; d <<= 1) {
-        const T v = __shfl_up_sync(0xffffffffu, incl, d);
+        const int v = __shfl_up_sync(0xffffffffu, incl, d);
         if (lane >= d) incl += v;
     }
     if (lane == 31) warp_sums[warp] = incl;
     __syncthreads();
-    T before = incl - mine;
+    int before = incl - mine;
     total = 0;
 #pragma unroll
     for (int w = 0; w < 8; ++w) {
-        if (w < warp) before += warp_sums[w];
-        total += warp_sums[w];
+        const int v = warp_sums[w];
+        if (w < warp) before += v;
+        total += v;
     }
     return before;
 }
@@ -152,26 +131,29 @@ __device__ __forceinline__ int tile_kv_end(const Args& a, const Sequence& s, int
     return max(0, key_limit(a, s, (row_end - 1) / a.group));
 }
 
-// Item `y` of the grid, tiles of later tokens (the ones with more keys) first.
-// All threads; `ints` is shared memory for 2 * kMaxPlanned + 1 integers.
-// False: past the last one.
-__device__ __forceinline__ bool find_item(const Args& a, TileShared& sm, int* ints, int y, Item& it) {
+// Item `y` of the grid and its sequence, tiles of later tokens (the ones with
+// more keys) first.  All threads; `ints` is shared memory for 2 * kMaxPlanned + 1
+// integers.  False: past the last one.
+__device__ __forceinline__ bool find_item(const Args& a, TileShared& sm, int* ints, int y, Item& it, Sequence& seq) {
     const bool packed = a.seqstart_q != nullptr;
+    const int tid = threadIdx.x;
+    const int per_seq = packed ? 1 : (a.seqlen_q * a.group + kTileM - 1) / kTileM;
     if (!a.plan) {
-        // Every tile whole (or cut as the host said), without a look at the lengths.
-        it.k = y % a.splits;
+        // Every tile whole, or cut as the host said, without a look at the lengths.
+        const int x = y / a.splits;
+        it.k = y - x * a.splits;
         it.parts = a.splits;
         it.slot = 0;
-        const int x = y / a.splits;
         if (!packed) {
-            const int tiles = (a.seqlen_q * a.group + kTileM - 1) / kTileM;
-            it.m = tiles - 1 - x / a.batch;
-            it.b = x % a.batch;
-            return it.m >= 0;
+            const int back = x / a.batch;
+            it.m = per_seq - 1 - back;
+            it.b = x - back * a.batch;
+            if (it.m < 0) return false;
+            seq = load_sequence(a, it.b);
+            return true;
         }
     }
     // First row tile of every sequence.
-    const int tid = threadIdx.x;
     int* first = ints;
     int tiles;
     if (packed) {
@@ -196,6 +178,7 @@ __device__ __forceinline__ bool find_item(const Args& a, TileShared& sm, int* in
             __syncthreads();
             it.b = sm.item[0];
             it.m = sm.item[1];
+            seq = load_sequence(a, it.b);
             return true;
         }
         for (int b = b0; b < b1; ++b) {
@@ -205,74 +188,95 @@ __device__ __forceinline__ bool find_item(const Args& a, TileShared& sm, int* in
         if (tid == 0) first[a.batch] = tiles;
         __syncthreads();
     } else {
-        tiles = a.batch * ((a.seqlen_q * a.group + kTileM - 1) / kTileM);
+        tiles = a.batch * per_seq;
     }
     tiles = min(tiles, kMaxPlanned);  // more only if the prefix sums overlap
-    const int per_seq = packed ? 1 : tiles / a.batch;
-    auto sequence_of = [&](int t, int& m) {
-        if (!packed) {
-            m = t % per_seq;
-            return t / per_seq;
-        }
-        int lo = 0, hi = a.batch;  // the last one with first <= t
-        while (hi - lo > 1) {
-            const int mid = (lo + hi) >> 1;
-            if (first[mid] <= t) lo = mid;
-            else hi = mid;
-        }
-        m = t - first[lo];
-        return lo;
-    };
-    // Key tiles of every row tile, and the range length.
+    // Key tiles of this thread's row tiles t0 .. t1-1, and the range length.
     int* keys = ints + kMaxPlanned + 1;
     const int per = (tiles + kTileThreads - 1) / kTileThreads;
     const int t0 = min(tiles, tid * per), t1 = min(tiles, t0 + per);
-    long long mine = 0, total;
-    for (int t = t0; t < t1; ++t) {
-        int m;
-        const int b = sequence_of(t, m);
-        const int n = max(1, (tile_kv_end(a, load_sequence(a, b), m) + kTileN - 1) / kTileN);
-        keys[t] = n;
-        mine += n;
+    int b_first = 0, m_first = 0;
+    if (packed) {
+        int lo = 0, hi = a.batch;  // the last sequence with first <= t0
+        while (hi - lo > 1) {
+            const int mid = (lo + hi) >> 1;
+            if (first[mid] <= t0) lo = mid;
+            else hi = mid;
+        }
+        b_first = lo;
+        m_first = t0 - first[lo];
+    } else {
+        b_first = t0 / per_seq;
+        m_first = t0 - b_first * per_seq;
     }
-    block_scan(mine, sm.scan_keys, total);
-    total *= a.nhead_k;
+    // The next row tile after (b, m); empty sequences are passed over.
+    auto next_tile = [&](int& b, int& m, int t) {
+        ++m;
+        if (packed)
+            while (b + 1 < a.batch && first[b + 1] <= t) ++b, m = 0;
+        else if (m == per_seq)
+            ++b, m = 0;
+    };
+    int mine = 0, total;
+    {
+        int b = b_first, m = m_first, have = -1;
+        Sequence s{0, 0, 0};
+        for (int t = t0; t < t1; ++t) {
+            if (b != have) s = load_sequence(a, have = b);
+            const int n = max(1, (tile_kv_end(a, s, m) + kTileN - 1) / kTileN);
+            keys[t] = n;
+            mine += min(n, kMostCounted);
+            next_tile(b, m, t + 1);
+        }
+    }
+    block_scan(mine, sm.scan_a, total);
     // One range per resident block while ranges are short, two beyond.
-    long long len = (total + kTileBlocks - 1) / kTileBlocks;
-    if (len > kLongRange) len = max((long long)kLongRange, (total + 2 * kTileBlocks - 1) / (2 * kTileBlocks));
-    const int most = (int)min(len, (long long)INT_MAX);
-    auto parts_of = [&](int n) { return (n + most - 1) / most; };
-    int items_mine = 0, split_mine = 0;
+    const long long all = (long long)total * a.nhead_k;
+    long long len = (all + kTileBlocks - 1) / kTileBlocks;
+    if (len > kLongRange) len = max((long long)kLongRange, (all + 2 * kTileBlocks - 1) / (2 * kTileBlocks));
+    const unsigned most = (unsigned)min(len, 0x7fffffffll);
+    auto parts_of = [&](int n) { return (int)(((unsigned)min(n, kMostCounted) + most - 1) / most); };
+    int both = 0;  // items in the upper half, those of split jobs in the lower
     for (int t = t0; t < t1; ++t) {
         const int p = parts_of(keys[t]);
-        items_mine += p;
-        if (p > 1) split_mine += p;
+        both += p << 16 | (p > 1 ? p : 0);
     }
-    int items, split;
-    int items_before = block_scan(items_mine, sm.scan_a, items);
-    int split_before = block_scan(split_mine, sm.scan_b, split);
+    int sum;
+    const int before = block_scan(both, sm.scan_b, sum);
+    const int split = sum & 0xffff;
     // No job begins in the slots that stay unused.
-    if (blockIdx.x % a.nhead_k == 0)
-        for (int i = split * a.nhead_k + (int)(blockIdx.x / a.nhead_k) * kTileThreads + tid; i < a.max_slots;
-             i += (int)(gridDim.x / a.nhead_k) * kTileThreads)
-            tile_headers(a)[i].parts = 0;
-    const int x = items - 1 - y;
+    for (int i = split * a.nhead_k + (int)blockIdx.x * kTileThreads + tid; i < a.max_slots;
+         i += (int)gridDim.x * kTileThreads)
+        tile_headers(a)[i].parts = 0;
+    const int x = (sum >> 16) - 1 - y;
     if (x < 0) return false;
-    if (x >= items_before && x < items_before + items_mine)
+    int items_before = before >> 16, split_before = before & 0xffff;
+    if (x >= items_before && x < items_before + (both >> 16)) {
+        int b = b_first, m = m_first;
         for (int t = t0; t < t1; ++t) {
             const int p = parts_of(keys[t]);
             if (x < items_before + p) {
-                sm.item[0] = sequence_of(t, sm.item[1]);
+                const Sequence s = load_sequence(a, b);
+                sm.item[0] = b;
+                sm.item[1] = m;
                 sm.item[2] = x - items_before;
                 sm.item[3] = p;
-                sm.item[4] = split_before;
+                sm.item[4] = split_before * a.nhead_k;
+                sm.item[5] = s.first;
+                sm.item[6] = s.count;
+                sm.item[7] = s.keys;
                 break;
             }
             items_before += p;
             if (p > 1) split_before += p;
+            next_tile(b, m, t + 1);
         }
+    }
+    // The ring goes to the copies next: what was written there comes before them.
+    asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
     __syncthreads();
-    it = Item{sm.item[0], sm.item[1], sm.item[2], sm.item[3], sm.item[4] * a.nhead_k};
+    it = Item{sm.item[0], sm.item[1], sm.item[2], sm.item[3], sm.item[4]};
+    seq = Sequence{sm.item[5], sm.item[6], sm.item[7]};
     return true;
 }
 
@@ -292,16 +296,17 @@ fmha_paged_tile_kernel(const __grid_constant__ Args a) {
     // neighbouring lines of memory at the same time.
     const int kvh = blockIdx.x % a.nhead_k;
     Item it;
-    if (!find_item(a, sm, reinterpret_cast<int*>(sm.kv[0]), blockIdx.x / a.nhead_k, it)) return;
-    const Sequence seq = load_sequence(a, it.b);
+    Sequence seq;
+    if (!find_item(a, sm, reinterpret_cast<int*>(sm.kv[0]), blockIdx.x / a.nhead_k, it, seq)) return;
     const int rows = seq.count * a.group;
     const int row0 = it.m * kTileM;
     if (rows < a.min_rows || rows > a.max_rows || row0 >= rows) return;
     const int row_end = min(rows, row0 + kTileM);
     const int kv_end = tile_kv_end(a, seq, it.m);
     const int all = (kv_end + kTileN - 1) / kTileN;
-    const int j0 = (int)((long long)all * it.k / it.parts);
-    const int n = (int)((long long)all * (it.k + 1) / it.parts) - j0;
+    const int each = all / it.parts, more = all - each * it.parts;
+    const int j0 = it.k * each + min(it.k, more);
+    const int n = each + (it.k < more);
     const bool shared_job = a.plan && it.parts > 1;  // through a scratch slot
     const int slot_job = it.slot + it.k * a.nhead_k + kvh;
     if (shared_job && it.k == 0 && threadIdx.x == 0)
@@ -312,72 +317,96 @@ fmha_paged_tile_kernel(const __grid_constant__ Args a) {
     const bool has_tail = n > 0 && tail < kTileN;
     const int active = (row_end - row0 + 31) / 32;    // softmax warps with rows
 
-    if (threadIdx.x == 0) {
-        mbar_init(smem_u32(&sm.bar_q), 128);
-        for (int s = 0; s < kTileStages; ++s) {
-            mbar_init(smem_u32(&sm.bar_full[s]), 1);
-            mbar_init(smem_u32(&sm.bar_empty[s]), 1);
+    // K_j is load 2j, V_j load 2j + 1 of the ring.
+    auto slot_of = [](int i) { return i % kTileStages; };
+    auto phase_of = [](int i) { return (uint32_t)((i / kTileStages) & 1); };
+
+    // Softmax warps: the thread's row.
+    const int row = row0 + (int)threadIdx.x;
+    const bool has_row = row < row_end;  // (warps 0-3)
+    const int tok = has_row ? row / a.group : 0;
+    const int token = seq.first + tok, head = kvh * a.group + (has_row ? row - tok * a.group : 0);
+
+    // Load warp: box_rows keys of one page per box, lane i loads box i of a tile.
+    const uint64_t policy = l2_policy_evict_last();
+    const int box_rows = min(1 << a.page_shift, kTileN);
+    auto page_of = [&](int j) {
+        const int key = (j0 + j) * kTileN + lane * box_rows;
+        return lane * box_rows < kTileN && key < kv_end
+                   ? __ldg(a.page_table + it.b * a.table_stride + (key >> a.page_shift)) : 0;
+    };
+    auto issue_load = [&](int i, int page) {
+        const int key0 = (j0 + (i >> 1)) * kTileN, slot = slot_of(i);
+        const int boxes = (min(kTileN, kv_end - key0) + box_rows - 1) / box_rows;
+        const uint32_t bar = smem_u32(&sm.bar_full[slot]);
+        if (lane == 0) mbar_arrive_expect_tx(bar, boxes * box_rows * kHeadDim * 2);
+        __syncwarp();
+        if (lane < boxes) {
+            if (page < 0 || page >= a.num_pages) flag_index_error(a.err_word);
+            load_page_box(smem_u32(sm.kv[slot]) + lane * box_rows * kHeadDim * 2, (i & 1) ? &a.tm_v : &a.tm_k, bar,
+                          (key0 + lane * box_rows) & ((1 << a.page_shift) - 1), kvh, page, policy);
         }
-        mbar_init(smem_u32(&sm.bar_s), 1);
-        mbar_init(smem_u32(&sm.bar_sfree), 32 * active);
-        mbar_init(smem_u32(&sm.bar_p), 32 * active);
-        mbar_init(smem_u32(&sm.bar_pv), 1);
-        mbar_init(smem_u32(&sm.bar_drain), 1);
-        sm.abort_flag = 0;
-        fence_barrier_init();
-    }
-    if (warp == 5) {
+    };
+    constexpr int kAhead = kTileStages / 2;  // tiles loaded before the block starts
+    int page = 0;
+
+    // Start, the roles side by side: barriers and the first copies, tensor
+    // memory, and Q (its 16-byte chunks swizzled by row mod 8).
+    if (warp == 4) {
+        page = page_of(0);
+        if (lane == 0) {
+            for (int s = 0; s < kTileStages; ++s) {
+                mbar_init(smem_u32(&sm.bar_full[s]), 1);
+                mbar_init(smem_u32(&sm.bar_empty[s]), 1);
+            }
+            mbar_init(smem_u32(&sm.bar_s), 1);
+            mbar_init(smem_u32(&sm.bar_sfree), 32 * active);
+            mbar_init(smem_u32(&sm.bar_p), 32 * active);
+            mbar_init(smem_u32(&sm.bar_pv), 1);
+            mbar_init(smem_u32(&sm.bar_drain), 1);
+            sm.abort_flag = 0;
+            fence_barrier_init();
+        }
+        __syncwarp();
+        for (int j = 0; j < min(n, kAhead); ++j) {
+            const int next = j + 1 < n ? page_of(j + 1) : 0;
+            issue_load(2 * j, page);
+            issue_load(2 * j + 1, page);
+            page = next;
+        }
+    } else if (warp == 5) {
         tmem_alloc(smem_u32(&sm.tmem_base), kTileTmemCols);
         tmem_relinquish();
+    } else if (warp < 4 && n > 0) {
+        uint4 x[8];
+        const uint4* src = has_row ? reinterpret_cast<const uint4*>(q_row(a, token, head)) : nullptr;
+#pragma unroll
+        for (int c = 0; c < 8; ++c) x[c] = src ? __ldg(src + c) : make_uint4(0, 0, 0, 0);
+        uint4* dst = reinterpret_cast<uint4*>(sm.q) + threadIdx.x * 8;
+#pragma unroll
+        for (int c = 0; c < 8; ++c) dst[c ^ (threadIdx.x & 7)] = x[c];
+        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
     }
-    // find_item used the K/V ring: ordered before the first TMA write there.
-    asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
     tc_fence_before();
     __syncthreads();
     tc_fence_after();
     const uint32_t tmem = sm.tmem_base;
 
-    // K_j is load 2j, V_j load 2j + 1 of the ring.
-    auto slot_of = [](int i) { return i % kTileStages; };
-    auto phase_of = [](int i) { return (uint32_t)((i / kTileStages) & 1); };
-
     if (warp >= 4) {
         regs_dec<kTileRegsControl>();
         if (warp == 4 && n > 0) {
             // ---------------------------------------------------- loads
-            if (lane == 0) {
-                tma_prefetch_desc(&a.tm_k);
-                tma_prefetch_desc(&a.tm_v);
-            }
-            const uint64_t policy = l2_policy_evict_last();
-            const int box_rows = min(1 << a.page_shift, kTileN);
-            const int32_t* table = a.page_table + it.b * a.table_stride;
-            // Lane i loads box i of a tile: box_rows keys of one page.
-            auto page_of = [&](int j) {
-                const int key = (j0 + j) * kTileN + lane * box_rows;
-                return lane * box_rows < kTileN && key < kv_end ? __ldg(table + (key >> a.page_shift)) : 0;
-            };
-            int page = page_of(0);
             bool ok = true;
-            int issued = 0;
-            for (int j = 0; j < n && ok; ++j) {
+            int issued = 2 * min(n, kAhead);
+            for (int j = kAhead; j < n && ok; ++j) {
                 const int next = j + 1 < n ? page_of(j + 1) : 0;
-                const int key0 = (j0 + j) * kTileN;
-                const int boxes = (min(kTileN, kv_end - key0) + box_rows - 1) / box_rows;
-                if (lane < boxes && (page < 0 || page >= a.num_pages)) flag_index_error(a.err_word);
 #pragma unroll
                 for (int v = 0; v < 2; ++v) {
-                    const int i = 2 * j + v, slot = slot_of(i);
-                    ok = wait_phase(smem_u32(&sm.bar_empty[slot]), phase_of(i) ^ 1, abort_flag, a);
+                    const int i = 2 * j + v;
+                    ok = wait_phase(smem_u32(&sm.bar_empty[slot_of(i)]), phase_of(i) ^ 1, abort_flag, a);
                     ok = __all_sync(0xffffffffu, ok);
                     if (!ok) break;
-                    const uint32_t bar = smem_u32(&sm.bar_full[slot]);
-                    if (lane == 0) mbar_arrive_expect_tx(bar, boxes * box_rows * kHeadDim * 2);
-                    __syncwarp();
-                    if (lane < boxes)
-                        load_page_box(smem_u32(sm.kv[slot]) + lane * box_rows * kHeadDim * 2,
-                                      v ? &a.tm_v : &a.tm_k, bar, (key0 + lane * box_rows) & ((1 << a.page_shift) - 1),
-                                      kvh, page, policy);
+                    issue_load(i, page);
                     issued = i + 1;
                 }
                 page = next;
@@ -420,7 +449,7 @@ fmha_paged_tile_kernel(const __grid_constant__ Args a) {
                         mma_ts(tmem + kColO, tmem + kColP + kk * 8, db + (uint64_t)(kk * 128), idesc_pv, 1u);
                 }
             };
-            bool ok = wait_all(&sm.bar_q, 0) && wait_all(&sm.bar_full[0], 0);
+            bool ok = wait_all(&sm.bar_full[0], 0);
             if (ok) {
                 tc_fence_after();
                 issue_s(0);
@@ -462,22 +491,6 @@ fmha_paged_tile_kernel(const __grid_constant__ Args a) {
         regs_inc<kTileRegsSoftmax>();
         // -------------------------------------------------------- softmax
         const int t = threadIdx.x;
-        const int row = row0 + t;
-        const bool has_row = row < row_end;
-        const int tok = has_row ? row / a.group : 0;
-        const int token = seq.first + tok, head = kvh * a.group + (has_row ? row - tok * a.group : 0);
-        if (n > 0) {
-            // Stage Q: the thread's row, 16-byte chunks swizzled by row mod 8.
-            uint4 x[8];
-            const uint4* src = has_row ? reinterpret_cast<const uint4*>(q_row(a, token, head)) : nullptr;
-#pragma unroll
-            for (int c = 0; c < 8; ++c) x[c] = src ? __ldg(src + c) : make_uint4(0, 0, 0, 0);
-            uint4* dst = reinterpret_cast<uint4*>(sm.q) + t * 8;
-#pragma unroll
-            for (int c = 0; c < 8; ++c) dst[c ^ (t & 7)] = x[c];
-            asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-            mbar_arrive(smem_u32(&sm.bar_q));
-        }
         if (warp < active) {
             const uint32_t lane_base = (uint32_t)(warp * 32) << 16;
             const uint32_t tS = tmem + lane_base + kColS, tO = tmem + lane_base + kColO,
@@ -548,7 +561,7 @@ fmha_paged_tile_kernel(const __grid_constant__ Args a) {
                                 make_float2(__uint_as_float(r[c][e]), __uint_as_float(r[c][e + 1])), scale2, neg2);
                             float2 pp;
                             if (kPoly && (pr + 1) * kPolyOf16 / 16 > pr * kPolyOf16 / 16)
-                                pp = exp2_poly4(x);
+                                pp = exp2_poly2(x);
                             else
                                 pp = make_float2(ex2_approx(x.x), ex2_approx(x.y));
                             sum[pr & 3] = fadd2(sum[pr & 3], pp);

@@ -50,7 +50,10 @@ struct Plan {
     bool planned;             // it plans its key ranges by the lengths
     long long prefix_tiles;   // row tiles against the prefix, and their key ranges
     int prefix_splits;
-    size_t pieces, slots, part;  // bytes: the two kernels' scratch; one partial result of all rows
+    // Bytes: the two kernels' scratch; under a prefix, what the rows kernel says of
+    // the sequences, and one partial result of all rows.
+    size_t pieces, slots, info, part;
+    int parts;                // partial results: the prefix's, then the rows kernel's
     size_t total;
 };
 
@@ -78,7 +81,7 @@ bool make_plan(int batch, int seqlen_q, int total_q, bool packed, int nhead_q, i
     z.tokens = packed ? total_q : (long long)batch * seqlen_q;
     z.group = nhead_q / nhead_k;
     const long long max_rows = (long long)(packed ? std::min(seqlen_q, total_q) : seqlen_q) * z.group;
-    if (z.tokens * nhead_q > INT_MAX || nhead_q > 65535) return false;
+    if (z.tokens * nhead_q > INT_MAX || nhead_q > 65535 || (z.tokens > 0 && max_rows == 0)) return false;
     z.max_rows = (int)max_rows;
     z.tile = max_rows > kMostRows;
     z.rows = packed || !z.tile;
@@ -99,8 +102,10 @@ bool make_plan(int batch, int seqlen_q, int total_q, bool packed, int nhead_q, i
         z.prefix_tiles = (z.tokens * z.group + kTileM - 1) / kTileM;
         z.prefix_splits = pick_splits(std::max(1ll, z.prefix_tiles * nhead_k), (prefix_len + kTileN - 1) / kTileN);
         z.part = (size_t)z.tokens * nhead_q * (kHeadDim + 1) * sizeof(float);
+        z.parts = z.prefix_splits + (z.rows ? 1 : 0);
+        z.info = round16(batch * sizeof(int2));
     }
-    z.total = z.pieces + z.slots + z.part * z.prefix_splits;
+    z.total = z.pieces + z.slots + z.info + z.part * z.parts;
     return true;
 }
 
@@ -151,7 +156,7 @@ int check(const FmhaPagedParams* p, bool prefix, Plan& z) {
         !stride_ok(p->nhead_stride_v, p->nhead_k) || !stride_ok(p->page_stride_v, p->num_pages))
         return FMHA_ERR_ARG;
     // Units of 32 keys over the whole batch are counted in 31 bits.
-    if ((long long)p->batch * (((long long)p->max_pages << shift) / kUnit + 2) > INT_MAX) return FMHA_ERR_ARG;
+    if ((long long)p->batch * (((long long)p->max_pages << shift) / kUnit + 1 + kSeqCost) > INT_MAX) return FMHA_ERR_ARG;
     if (!(p->scale > 0.0f) || p->scale > 1e30f) return FMHA_ERR_ARG;
     if (z.tokens > 0 && (p->workspace == nullptr || !aligned16(p->workspace) ||
                          p->workspace_bytes < (long long)z.total))
@@ -214,9 +219,9 @@ int launch_dependent(Kernel kernel, dim3 grid, int threads, size_t smem, cudaStr
     return cudaLaunchKernelEx(&cfg, kernel, a) == cudaSuccess ? FMHA_OK : FMHA_ERR_LAUNCH;
 }
 
-// The rows kernel (after = it follows another kernel of the call) and the merge
-// of the sequences that cross its blocks.
-int launch_rows(const Args& a, bool after, int device, cudaStream_t stream) {
+// The rows kernel (after = it follows another kernel of the call), then the merge
+// of the sequences that cross its blocks or, under a prefix, of all partial results.
+int launch_rows(const Args& a, const Args* finish, bool after, int device, cudaStream_t stream) {
     constexpr size_t smem = sizeof(RowsShared) + 1024;
     static std::atomic<unsigned long long> ready{0};
     if (!allow_smem(ready, device, reinterpret_cast<const void*>(fmha_paged_rows_kernel), smem))
@@ -227,6 +232,10 @@ int launch_rows(const Args& a, bool after, int device, cudaStream_t stream) {
     } else {
         fmha_paged_rows_kernel<<<kMaxRowBlocks, kRowThreadsTotal, smem, stream>>>(a);
         if (cudaGetLastError() != cudaSuccess) return FMHA_ERR_LAUNCH;
+    }
+    if (finish != nullptr) {
+        const long long threads = (long long)a.tokens * a.nhead_q * 16;
+        return launch_dependent(fmha_prefix_finish, dim3((unsigned)((threads + 255) / 256)), 256, 0, stream, *finish);
     }
     return launch_dependent(fmha_paged_rows_merge, dim3(kMaxRowBlocks, (a.nhead_k * a.row_cap + 3) / 4), 256, 0, stream,
                             a);
@@ -253,8 +262,9 @@ int run(const FmhaPagedParams* p, bool prefix, cudaStream_t stream) {
     uint8_t* scratch = static_cast<uint8_t*>(p->workspace);
     a.pieces = reinterpret_cast<float*>(scratch);
     a.slots = reinterpret_cast<float*>(scratch + z.pieces);
-    float* part_o = reinterpret_cast<float*>(scratch + z.pieces + z.slots);
-    float* part_lse = part_o + (size_t)z.tokens * p->nhead_q * kHeadDim * z.prefix_splits;
+    const size_t part_rows = (size_t)z.tokens * p->nhead_q;
+    float* part_o = reinterpret_cast<float*>(scratch + z.pieces + z.slots + z.info);
+    float* part_lse = part_o + part_rows * kHeadDim * z.parts;
     a.splits = 1;
     if (z.tile || prefix) {
         Args t = a;
@@ -275,7 +285,7 @@ int run(const FmhaPagedParams* p, bool prefix, cudaStream_t stream) {
             if ((st = launch_tile(b, z.prefix_tiles * z.prefix_splits, ctx.device, stream)) != FMHA_OK) return st;
             a.part_o = t.part_o = part_o;
             a.part_lse = t.part_lse = part_lse;
-            a.part_n = t.part_n = z.prefix_splits;
+            t.part_n = z.prefix_splits;
         }
         if (z.tile) {
             t.min_rows = kMostRows + 1;
@@ -290,10 +300,19 @@ int run(const FmhaPagedParams* p, bool prefix, cudaStream_t stream) {
         a.row_cap = z.row_cap;
         if (z.tile) a.max_rows = kMostRows;
         if ((st = cache_maps(ctx, a, p, kUnit)) != FMHA_OK) return st;
-        if ((st = launch_rows(a, z.tile || prefix, ctx.device, stream)) != FMHA_OK) return st;
+        Args finish = a;
+        if (prefix) {
+            finish.part_n = z.prefix_splits;
+            a.seq_parts = finish.seq_parts = reinterpret_cast<int2*>(scratch + z.pieces + z.slots);
+            a.out_o = part_o + part_rows * kHeadDim * z.prefix_splits;
+            a.out_lse = part_lse + part_rows * z.prefix_splits;
+        }
+        st = launch_rows(a, prefix ? &finish : nullptr, z.tile || prefix, ctx.device, stream);
+        if (st != FMHA_OK) return st;
     }
     if (z.tile && z.planned) {
         a.max_slots = kMaxTileSlots;
+        a.part_n = z.prefix_splits;
         st = launch_dependent(fmha_paged_combine, dim3(kCombineBlocks), kCombineThreads, 0, stream, a);
     }
     return st;

@@ -51,8 +51,8 @@ struct Args {
     const float* part_o;
     const float* part_lse;
     int part_n;
-    // Where a tile launch that makes such partial results puts its own (split s
-    // into slot s); null: it writes final rows.
+    // Where a launch that makes such partial results puts its own (a prefix's
+    // split s into slot s); null: it writes final rows.
     float* out_o;
     float* out_lse;
     int splits;                 // tile kernel, plan == 0: key ranges per row tile
@@ -60,6 +60,8 @@ struct Args {
     float* slots;               // and the scratch of the jobs that blocks share
     int max_slots;
     float* pieces;              // rows kernel: scratch between its blocks
+    int2* seq_parts;            // rows kernel under a prefix: per sequence its first block and, if
+                                // it crosses blocks, how many share it
     int* err_word;
     unsigned long long wait_limit_ns;
 };
@@ -149,11 +151,19 @@ __device__ __forceinline__ void fold4(float& m, float& l, float4& o, float m2, f
     o.w = o.w * f.keep + o2.w * f.take;
 }
 
-// The final row's four columns [c, c+4): folds the other launches' partial
-// results in, then writes O and, once per row (`first`), the LSE.  O is
-// rounded once, to nearest even.
-__device__ __forceinline__ void finish_row4(const Args& a, int token, int head, int c, float m,
-                                            float l, float4 o, bool first) {
+// The final row's four columns [c, c+4) of O and, once per row (`first`), the
+// LSE.  O is rounded once, to nearest even.
+__device__ __forceinline__ void write_row4(const Args& a, int token, int head, int c, float m, float l, float4 o,
+                                           bool first) {
+    const float inv = l > 0.0f ? 1.0f / l : 0.0f;
+    *reinterpret_cast<uint2*>(o_row(a, token, head) + c) =
+        make_uint2(pack_bf16_rne(o.x * inv, o.y * inv), pack_bf16_rne(o.z * inv, o.w * inv));
+    if (first && a.lse != nullptr) *lse_at(a, token, head) = l > 0.0f ? (m + __log2f(l)) * kLn2 : -INFINITY;
+}
+
+// The same after folding in the part_n partial results of other launches.
+__device__ __forceinline__ void finish_row4(const Args& a, int token, int head, int c, float m, float l, float4 o,
+                                            bool first) {
     const long long row = flat_row(a, token, head);
     const long long rows = (long long)a.tokens * a.nhead_q;
     constexpr int kBatch = 4;  // partial results in flight
@@ -173,12 +183,7 @@ __device__ __forceinline__ void finish_row4(const Args& a, int token, int head, 
         for (int u = 0; u < kBatch; ++u)
             if (m2[u] != -INFINITY) fold4(m, l, o, m2[u], 1.0f, x[u]);  // else O was not written
     }
-    const float inv = l > 0.0f ? 1.0f / l : 0.0f;
-    o.x *= inv, o.y *= inv, o.z *= inv, o.w *= inv;
-    const float lse2 = l > 0.0f ? m + __log2f(l) : -INFINITY;
-    *reinterpret_cast<uint2*>(o_row(a, token, head) + c) =
-        make_uint2(pack_bf16_rne(o.x, o.y), pack_bf16_rne(o.z, o.w));
-    if (first && a.lse != nullptr) *lse_at(a, token, head) = lse2 * kLn2;
+    write_row4(a, token, head, c, m, l, o, first);
 }
 
 // Bounded wait on an mbarrier phase; false once the block's abort flag is up

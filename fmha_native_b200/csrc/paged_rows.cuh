@@ -44,6 +44,9 @@ constexpr int kMaxRowBlocks = 148;    // one block per SM
 
 constexpr int kMostRows = 16;         // rows of a K/V head that a warp holds
 constexpr int kRowStages = 3;
+// A sequence's start and end in a block cost about as much time as this many
+// units (its first loads, Q, the results); the shares count them.
+constexpr int kSeqCost = 2;
 
 // A (sequence, head) result of a block: where it goes.
 struct Target {
@@ -63,7 +66,7 @@ struct alignas(1024) RowsShared {
     int piece_job[kRowWarps][2];      // segment of the block * heads + head, -1: none
     int scan[kRowWarps];
     int run[2 * kRowWarps + 1];
-    int start_b, start_u;
+    int start_b, start_x;
     int abort_flag;
 };
 
@@ -94,6 +97,7 @@ struct RowSeq {
     int first, count, keys;
     int kv_end;      // keys that any of its rows sees
     int units;       // 0: not ours; a sequence that sees no key counts one (empty) unit
+    __device__ int cost() const { return units > 0 ? units + kSeqCost : 0; }
 };
 __device__ __forceinline__ RowSeq load_row_seq(const Args& a, int b) {
     const Sequence s = load_sequence(a, b);
@@ -137,9 +141,16 @@ __device__ __forceinline__ void fence_async_smem() {
 // block's scratch.
 __device__ __forceinline__ void emit_row4(const Args& a, const Target& to, int rt, int c4, float m, float l,
                                           float4 o) {
-    if (to.slot < 0) {
-        const int t = rt / a.group;
-        finish_row4(a, to.first + t, to.h * a.group + rt - t * a.group, c4 * 4, m, l, o, c4 == 0);
+    const int t = rt / a.group, token = to.first + t, head = to.h * a.group + rt - t * a.group;
+    if (to.slot < 0 && a.out_o == nullptr) {
+        write_row4(a, token, head, c4 * 4, m, l, o, c4 == 0);
+    } else if (to.slot < 0) {
+        // Under a prefix: one more partial result of the row.
+        const float inv = l > 0.0f ? 1.0f / l : 0.0f;
+        const long long row = flat_row(a, token, head);
+        *reinterpret_cast<float4*>(a.out_o + row * kHeadDim + c4 * 4) =
+            make_float4(o.x * inv, o.y * inv, o.z * inv, o.w * inv);
+        if (c4 == 0) a.out_lse[row] = l > 0.0f ? m + __log2f(l) : -INFINITY;
     } else {
         const long long row = piece_row(a, to.slot, to.h, rt);
         *reinterpret_cast<float4*>(piece_o(a, row) + c4 * 4) = o;
@@ -182,7 +193,7 @@ fmha_paged_rows_kernel(const __grid_constant__ Args a) {
     const int per = (a.batch + kRowThreadsTotal - 1) / kRowThreadsTotal;
     const int b0 = min(a.batch, (int)threadIdx.x * per), b1 = min(a.batch, b0 + per);
     int mine = 0;
-    for (int b = b0; b < b1; ++b) mine += load_row_seq(a, b).units;
+    for (int b = b0; b < b1; ++b) mine += load_row_seq(a, b).cost();
     int incl = mine;
 #pragma unroll
     for (int d = 1; d < 32; d <<= 1) {
@@ -211,10 +222,10 @@ fmha_paged_rows_kernel(const __grid_constant__ Args a) {
     if (beg >= before && beg < before + mine) {
         unsigned p = before;
         for (int b = b0; b < b1; ++b) {
-            const unsigned n = load_row_seq(a, b).units;
+            const unsigned n = load_row_seq(a, b).cost();
             if (beg < p + n) {
                 sm.start_b = b;
-                sm.start_u = (int)(beg - p);
+                sm.start_x = (int)(beg - p);
                 break;
             }
             p += n;
@@ -227,19 +238,28 @@ fmha_paged_rows_kernel(const __grid_constant__ Args a) {
     // n) in this block), head, unit.  Two cursors: `p` issues loads, `c` computes.
     struct Cursor {
         RowSeq x;
-        int b, seg, left;  // left: units of the block from this segment on
+        int b, seg;
+        int left, cost;  // cost of the block from this segment on, and of the segment
         int unit0, n, h, u;
     };
-    auto next_seq = [&](Cursor& k) {
-        k.left -= k.n;
-        k.unit0 = k.n = 0;
-        if (k.left <= 0) return false;
+    // Sets the segment of sequence k.b that starts `off` into the sequence's cost.
+    auto set_segment = [&](Cursor& k, int off) {
+        k.cost = min(k.x.cost() - off, k.left);
+        k.unit0 = max(0, off - kSeqCost);
+        k.n = max(0, off + k.cost - kSeqCost) - k.unit0;
+    };
+    auto next_segment = [&](Cursor& k) {
         do {
-            if (++k.b >= a.batch) return false;
-            k.x = load_row_seq(a, k.b);
-        } while (k.x.units == 0);
-        ++k.seg;
-        k.n = min(k.x.units, k.left);
+            k.left -= k.cost;
+            k.cost = k.n = 0;
+            if (k.left <= 0) return false;
+            do {
+                if (++k.b >= a.batch) return false;
+                k.x = load_row_seq(a, k.b);
+            } while (k.x.units == 0);
+            ++k.seg;
+            set_segment(k, 0);
+        } while (k.n == 0);
         return true;
     };
     auto advance = [&](Cursor& k) {
@@ -247,39 +267,47 @@ fmha_paged_rows_kernel(const __grid_constant__ Args a) {
         k.u = 0;
         if (++k.h < a.nhead_k) return;
         k.h = 0;
-        next_seq(k);
+        next_segment(k);
     };
-    const unsigned long long tiles = (unsigned long long)(end - beg) * a.nhead_k;
-    const unsigned long long from = tiles * warp / kRowWarps;
-    const long long count = (long long)(tiles * (warp + 1) / kRowWarps - from);
+    Cursor c;
+    c.b = sm.start_b;
+    c.x = load_row_seq(a, c.b);
+    c.seg = 0;
+    c.left = (int)(end - beg);
+    c.h = c.u = 0;
+    set_segment(c, sm.start_x);
+    bool any = c.n > 0 || next_segment(c);
+    // The block's tiles (unit x head), and what it has to say of its sequences.
     RowsHeader header{0, 0, 0, 0};
-    bool waited = false;
-    if (count > 0 || warp == 0) {
-        Cursor c;
-        c.b = sm.start_b;
-        c.x = load_row_seq(a, c.b);
-        c.seg = 0;
-        c.left = (int)(end - beg);
-        c.unit0 = sm.start_u;
-        c.n = min(c.x.units - c.unit0, c.left);
-        if (warp == 0) {
-            // The block's last segment, if its sequence begins here and goes on.
-            Cursor k = c;
-            while (k.left > k.n && next_seq(k)) {}
-            const int after = k.x.units - k.unit0 - k.n;
-            if (k.unit0 == 0 && after > 0) {
+    unsigned long long tiles = 0;
+    {
+        Cursor k = c;
+        for (bool more = any; more; more = next_segment(k)) {
+            tiles += (unsigned long long)k.n * a.nhead_k;
+            if (k.unit0 != 0) continue;
+            int parts = 0;
+            if (k.n < k.x.units) {
+                // Only a last segment goes on; its cost ends that far past the block's.
+                parts = (int)(ranges.owner(end + (k.x.units - k.n) - 1) - blockIdx.x) + 1;
                 header.first = k.x.first;
                 header.rows = k.x.count * a.group;
-                header.parts = (int)(ranges.owner(end + after - 1) - blockIdx.x) + 1;
+                header.parts = parts;
             }
+            if (a.seq_parts != nullptr && threadIdx.x == 0) a.seq_parts[k.b] = make_int2(blockIdx.x, parts);
         }
+    }
+    const unsigned long long from = tiles * warp / kRowWarps;
+    const long long count = (long long)(tiles * (warp + 1) / kRowWarps - from);
+    if (count > 0) {
         unsigned long long x = from;
         while (x >= (unsigned long long)c.n * a.nhead_k) {
             x -= (unsigned long long)c.n * a.nhead_k;
-            if (!next_seq(c)) break;
+            if (!next_segment(c)) break;
         }
-        c.h = c.n > 0 ? (int)((unsigned)x / (unsigned)c.n) : 0;
-        c.u = (int)x - c.h * c.n;
+        if (c.n > 0) {
+            c.h = x >> 32 ? (int)(x / (unsigned)c.n) : (int)((unsigned)x / (unsigned)c.n);
+            c.u = (int)(x - (unsigned long long)c.h * c.n);
+        }
         Cursor p = c;
         long long to_issue = count;
         int issued = 0, done = 0;
@@ -501,8 +529,6 @@ fmha_paged_rows_kernel(const __grid_constant__ Args a) {
                     __syncwarp();
                 }
                 if (all) {
-                    if (!waited) griddep_wait();  // a launch before this one may hold partial results
-                    waited = true;
                     for (int rt = lane >> 4; rt < rows; rt += 2) {
                         float mr = -INFINITY, lr = 0.0f;
                         float4 y = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
@@ -529,7 +555,7 @@ fmha_paged_rows_kernel(const __grid_constant__ Args a) {
     }
 
     // --------------------------------------------- the block's fold of pieces
-    if (!waited) griddep_wait();
+    griddep_wait();  // the grid ends after the launch before it
     if (threadIdx.x == 0) piece_headers(a)[blockIdx.x] = header;
     __syncthreads();
     if (*abort_flag) return;
@@ -614,6 +640,63 @@ fmha_paged_rows_merge(const __grid_constant__ Args a) {
         fold4(m, l, o, other_ml[slot][c4].x, other_ml[slot][c4].y, other_o[slot][c4]);
         emit_row4(a, Target{hd.first, rows, h, -1}, rt, c4, m, l, o);
     }
+}
+
+// The end of a prefix call: every row's partial results of the prefix and of
+// its own keys (one, or the pieces of a sequence that crossed blocks), folded
+// into the final row.  16 threads per row, four columns each.
+__global__ void __launch_bounds__(256)
+fmha_prefix_finish(const __grid_constant__ Args a) {
+    constexpr int kBatch = 8;
+    griddep_wait();
+    const long long row = ((long long)blockIdx.x * 256 + threadIdx.x) >> 4;
+    const long long all_rows = (long long)a.tokens * a.nhead_q;
+    if (row >= all_rows) return;
+    const int c4 = threadIdx.x & 15;
+    const int token = (int)(row / a.nhead_q), head = (int)(row - (long long)token * a.nhead_q);
+    int b = token / a.row_div;
+    if (a.seqstart_q != nullptr) {
+        b = 0;
+        for (int hi = a.batch; hi - b > 1;) {
+            const int mid = (b + hi) >> 1;
+            if (a.seqstart_q[mid] <= token) b = mid;
+            else hi = mid;
+        }
+    }
+    const Sequence s = load_sequence(a, b);
+    const int rows = s.count * a.group;
+    if (token < s.first || token >= s.first + s.count || rows < a.min_rows || rows > a.max_rows) return;
+    const int h = head / a.group, rt = (token - s.first) * a.group + head - h * a.group;
+    if (rt >= a.row_cap) return;  // more tokens than the call said
+    const int2 parts = a.seq_parts[b];  // its first block, and how many share it
+    const int own = max(1, parts.y);
+    float m = -INFINITY, l = 0.0f;
+    float4 o = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+    for (int k0 = 0; k0 < a.part_n + own; k0 += kBatch) {
+        float2 ml[kBatch];
+        float4 x[kBatch];
+#pragma unroll
+        for (int u = 0; u < kBatch; ++u) {
+            const int k = k0 + u, piece = k - a.part_n;
+            ml[u] = make_float2(-INFINITY, 1.0f);
+            x[u] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+            if (k >= a.part_n + own) continue;
+            const float* src;
+            if (piece >= 0 && parts.y > 0) {
+                const long long at = piece_row(a, 2 * (parts.x + piece) + (piece == 0), h, rt);
+                ml[u] = *reinterpret_cast<const float2*>(piece_ml(a, at));
+                src = piece_o(a, at);
+            } else {  // the prefix's parts, then the sequence's own
+                ml[u].x = a.part_lse[k * all_rows + row];
+                src = a.part_o + (k * all_rows + row) * kHeadDim;
+            }
+            x[u] = *reinterpret_cast<const float4*>(src + c4 * 4);
+        }
+#pragma unroll
+        for (int u = 0; u < kBatch; ++u)
+            if (ml[u].x != -INFINITY) fold4(m, l, o, ml[u].x, ml[u].y, x[u]);  // else O may be unwritten
+    }
+    write_row4(a, token, head, c4 * 4, m, l, o, c4 == 0);
 }
 
 }  // namespace fmha_paged

@@ -313,46 +313,51 @@ fmha_paged_rows_kernel(const __grid_constant__ Args a) {
         int issued = 0, done = 0;
 
         // Page ids: lane i holds entry win + i of sequence win_b's table row.
-        const int box_rows = min(1 << a.page_shift, kUnit);
-        const int boxes = kUnit / box_rows;
+        const int box_shift = min(a.page_shift, 5);  // keys of a box, at most a unit's 32
+        const int page_mask = (1 << a.page_shift) - 1;
         int win_b = -1, win = 0, ids = 0, ids_next = 0;
         auto load_ids = [&](int first, int pages) {
             const int i = first + lane;
             return i < pages ? __ldg(a.page_table + win_b * a.table_stride + i) : 0;
         };
         const uint64_t policy = l2_policy_evict_first();
+        const uint32_t ring0 = smem_u32(sm.ring[warp]), bar0 = smem_u32(sm.bar[warp]);
+        int fill = 0;  // slot of the next load
+        const bool leader = elect_one();
         auto produce = [&]() {
             while (to_issue > 0 && issued - done < kRowStages) {
                 if (p.x.kv_end > 0) {
                     const int key0 = (p.unit0 + p.u) * kUnit;
-                    const int pages = (p.x.keys + (1 << a.page_shift) - 1) >> a.page_shift;
                     const int page0 = key0 >> a.page_shift;
-                    if (win_b != p.b || page0 < win || page0 >= win + 64) {
-                        win_b = p.b;
-                        win = page0 & ~3;
-                        ids = load_ids(win, pages);
-                        ids_next = load_ids(win + 32, pages);
-                    } else if (page0 >= win + 32) {
-                        win += 32;
-                        ids = ids_next;
+                    if (win_b != p.b || (unsigned)(page0 - win) >= 32u) {
+                        const int pages = (p.x.keys + page_mask) >> a.page_shift;
+                        if (win_b == p.b && page0 - win >= 32 && page0 - win < 64) {
+                            win += 32;
+                            ids = ids_next;
+                        } else {
+                            win_b = p.b;
+                            win = page0 & ~3;
+                            ids = load_ids(win, pages);
+                        }
                         ids_next = load_ids(win + 32, pages);
                     }
-                    const int nbox = min(boxes, (p.x.kv_end - key0 + box_rows - 1) / box_rows);
-                    const int slot = issued % kRowStages;
-                    const uint32_t bar = smem_u32(&sm.bar[warp][slot]);
-                    if (lane == 0) mbar_arrive_expect_tx(bar, 2 * nbox * box_rows * kHeadDim * 2);
-                    __syncwarp();
-                    // Lanes 0..nbox-1 load K boxes, the next nbox V boxes.
-                    const int box = lane < nbox ? lane : lane - nbox;
-                    const int id = __shfl_sync(0xffffffffu, ids, (page0 + box - win) & 31);
-                    if (lane < 2 * nbox) {
-                        if (id < 0 || id >= a.num_pages) flag_index_error(a.err_word);
-                        const bool is_v = lane >= nbox;
-                        load_page_box(smem_u32(&sm.ring[warp][slot][is_v][box * box_rows * kHeadDim * 2]),
-                                      is_v ? &a.tm_v : &a.tm_k, bar, key0 & ((1 << a.page_shift) - 1), p.h,
-                                      id, policy);
+                    const int nbox = (min(kUnit, p.x.kv_end - key0) + (1 << box_shift) - 1) >> box_shift;
+                    const uint32_t bar = bar0 + fill * 8;
+                    if (leader) mbar_arrive_expect_tx(bar, (2 * nbox) << (box_shift + 7));
+                    // One elected lane issues the boxes: the copy instruction takes its
+                    // operands from uniform registers, so lanes side by side would be
+                    // taken one after the other, at several times the cost.
+                    for (int box = 0; box < nbox; ++box) {
+                        const int id = __shfl_sync(0xffffffffu, ids, page0 + box - win);
+                        const uint32_t dst = ring0 + fill * (2 * kUnitBytes) + (box << (box_shift + 7));
+                        if (leader) {
+                            if ((unsigned)id >= (unsigned)a.num_pages) flag_index_error(a.err_word);
+                            load_page_box(dst, &a.tm_k, bar, key0 & page_mask, p.h, id, policy);
+                            load_page_box(dst + kUnitBytes, &a.tm_v, bar, key0 & page_mask, p.h, id, policy);
+                        }
                     }
                     ++issued;
+                    fill = fill == kRowStages - 1 ? 0 : fill + 1;
                 }
                 advance(p);
                 --to_issue;

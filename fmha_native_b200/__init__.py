@@ -148,7 +148,7 @@ def load_library(path: str = LIB_PATH) -> ctypes.CDLL:
     for name in ("fmha_rope_d64_bf16", "fmha_paged_append_d64_bf16", "fmha_paged_fwd_d64_bf16",
                  "fmha_prefix_fwd_d64_bf16"):
         fn = getattr(lib, name)
-        fn.argtypes = [ctypes.c_char_p, ctypes.c_void_p]  # the packed parameter block, the stream
+        fn.argtypes = [ctypes.c_void_p, ctypes.c_void_p]  # byref(FmhaRopeParams / FmhaPagedParams), the stream
         fn.restype = ctypes.c_int
     lib.fmha_paged_workspace_bytes.argtypes = [ctypes.c_int] * 6
     lib.fmha_paged_workspace_bytes.restype = ctypes.c_size_t

@@ -81,6 +81,34 @@ def build_trace_library(force: bool = False) -> str:
     return TRACE_LIB_PATH
 
 
+BINDING_SRC = os.path.join(PKG_DIR, "host", "torch_binding.cpp")
+BINDING_PATH = os.path.join(PKG_DIR, "_torch_binding.so")
+
+
+def build_torch_binding(force: bool = False) -> str:
+    """The torch binding of the serving operators (a CPython module against
+    torch's C++ headers; calls the C ABI through pointers, links no CUDA code)."""
+    deps = [BINDING_SRC, os.path.join(REPO_DIR, "include", "fmha_paged.h"), os.path.join(REPO_DIR, "include", "fmha_fwd.h")]
+    if not force and not _stale(BINDING_PATH, deps):
+        return BINDING_PATH
+    import sysconfig
+
+    import torch
+
+    root = os.path.dirname(torch.__file__)
+    cuda = os.path.dirname(os.path.dirname(nvcc_path()))
+    inc = [os.path.join(REPO_DIR, "include"), os.path.join(root, "include"),
+           os.path.join(root, "include", "torch", "csrc", "api", "include"), os.path.join(cuda, "include"),
+           sysconfig.get_paths()["include"]]
+    subprocess.run(["g++", "-std=c++17", "-O2", "-fPIC", "-shared", "-fvisibility=hidden",
+                    f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}",
+                    *(x for i in inc for x in ("-isystem" if i != inc[0] else "-I", i)), BINDING_SRC,
+                    "-o", BINDING_PATH + ".tmp", "-L", os.path.join(root, "lib"),
+                    "-ltorch_python", "-ltorch", "-ltorch_cpu", "-lc10", "-lc10_cuda"], check=True)
+    os.replace(BINDING_PATH + ".tmp", BINDING_PATH)
+    return BINDING_PATH
+
+
 CLI_SRC = os.path.join(PKG_DIR, "host", "bench_fmha_fwd.cpp")
 CLI_PATH = os.path.join(PKG_DIR, "bench_fmha_fwd")
 
@@ -148,6 +176,7 @@ def build_cpp_tests(force: bool = False) -> str | None:
 
 if __name__ == "__main__":
     build_library(force="--force" in sys.argv, verbose="-v" in sys.argv)
+    build_torch_binding(force="--force" in sys.argv)
     build_cli(force="--force" in sys.argv)
     build_trace_library(force="--force" in sys.argv)
     build_test_lib(force="--force" in sys.argv)

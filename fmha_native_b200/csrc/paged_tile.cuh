@@ -47,13 +47,15 @@ constexpr int kTileM = 128;
 constexpr int kTileN = 128;
 constexpr int kTileStages = 4;
 constexpr int kTileBytes = 128 * kHeadDim * 2;  // 16 KB: Q, K or V tile
-constexpr int kTileThreads = 256;
+constexpr int kTileThreads = 384;
+constexpr int kTileWarps = kTileThreads / 32;
+constexpr int kSoftmaxWarps = 8, kWarpLoad = 8, kWarpMma = 9;
 constexpr int kTileBlocks = 2 * 148;            // resident blocks of the device
 constexpr uint32_t kTileTmemCols = 256;
 constexpr uint32_t kColS = 0, kColO = 128, kColP = 192;
-// setmaxnreg split of the launch's 256 x 128 registers.
-constexpr int kTileRegsSoftmax = 184, kTileRegsControl = 72;
-static_assert(128 * (kTileRegsSoftmax + kTileRegsControl) <= kTileThreads * 128, "register split");
+// setmaxnreg split of the launch's 384 x 80 registers.
+constexpr int kTileRegsSoftmax = 96, kTileRegsControl = 48;
+static_assert(256 * kTileRegsSoftmax + 128 * kTileRegsControl <= kTileThreads * 80, "register split");
 constexpr float kLazyLog2 = 8.0f;
 constexpr int kLongRange = 16;  // key tiles of a range from which blocks take two
 constexpr int kPolyOf16 = 4;  // pairs of every 16 whose exponential runs on the FMA pipe
@@ -70,7 +72,9 @@ struct alignas(1024) TileShared {
     uint64_t bar_drain;
     uint32_t tmem_base;
     int abort_flag;
-    int scan_a[8], scan_b[8], item[8];
+    int scan_a[kTileWarps], scan_b[kTileWarps], item[8];
+    float half_max[2][kTileM], half_sum[2][kTileM];  // between the two threads of a row
+    int half_ok[kSoftmaxWarps];
 };
 
 // Scratch of the jobs that several blocks share.
@@ -92,6 +96,19 @@ __device__ __forceinline__ TileHeader* tile_headers(const Args& a) {
     return reinterpret_cast<TileHeader*>(a.slots + (size_t)a.max_slots * tile_slot_floats());
 }
 
+// Named barriers of `threads` threads: plain, and with an OR over a predicate.
+__device__ __forceinline__ void bar_sync(int id, int threads) {
+    asm volatile("barrier.cta.sync.aligned %0, %1;" ::"r"(id), "r"(threads) : "memory");
+}
+__device__ __forceinline__ bool bar_or(int id, int threads, bool p) {
+    uint32_t r;
+    asm volatile(
+        "{\n\t.reg .pred p, q;\n\tsetp.ne.u32 p, %3, 0;\n\t"
+        "barrier.cta.red.or.aligned.pred q, %1, %2, p;\n\tselp.u32 %0, 1, 0, q;\n\t}"
+        : "=r"(r) : "r"(id), "r"(threads), "r"((uint32_t)p) : "memory");
+    return r != 0;
+}
+
 // A block's work: range k of `parts` of the keys of row tile m of sequence b.
 static_assert((2 * kMaxPlanned + 1) * 4 <= kTileStages * kTileBytes, "find_item's integers fit the ring");
 static_assert(kMaxPlanned + 2 * kTileBlocks < 32768 && 4 * kTileBlocks < 65536, "find_item's packed sums");
@@ -101,7 +118,7 @@ struct Item {
 };
 
 // Exclusive scan of `mine` over the block; `total` = the sum.
-__device__ __forceinline__ int block_scan(int mine, int (&warp_sums)[8], int& total) {
+__device__ __forceinline__ int block_scan(int mine, int (&warp_sums)[kTileWarps], int& total) {
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     int incl = mine;
 #pragma unroll
@@ -114,7 +131,7 @@ __device__ __forceinline__ int block_scan(int mine, int (&warp_sums)[8], int& to
     int before = incl - mine;
     total = 0;
 #pragma unroll
-    for (int w = 0; w < 8; ++w) {
+    for (int w = 0; w < kTileWarps; ++w) {
         const int v = warp_sums[w];
         if (w < warp) before += v;
         total += v;
@@ -321,9 +338,10 @@ fmha_paged_tile_kernel(const __grid_constant__ Args a) {
     auto slot_of = [](int i) { return i % kTileStages; };
     auto phase_of = [](int i) { return (uint32_t)((i / kTileStages) & 1); };
 
-    // Softmax warps: the thread's row.
-    const int row = row0 + (int)threadIdx.x;
-    const bool has_row = row < row_end;  // (warps 0-3)
+    // Softmax warps: the thread's row and its half of the columns.
+    const int t = threadIdx.x & (kTileM - 1), half = (int)threadIdx.x >> 7;
+    const int row = row0 + t;
+    const bool has_row = row < row_end;
     const int tok = has_row ? row / a.group : 0;
     const int token = seq.first + tok, head = kvh * a.group + (has_row ? row - tok * a.group : 0);
 
@@ -352,7 +370,7 @@ fmha_paged_tile_kernel(const __grid_constant__ Args a) {
 
     // Start, the roles side by side: barriers and the first copies, tensor
     // memory, and Q (its 16-byte chunks swizzled by row mod 8).
-    if (warp == 4) {
+    if (warp == kWarpLoad) {
         page = page_of(0);
         if (lane == 0) {
             for (int s = 0; s < kTileStages; ++s) {
@@ -360,8 +378,8 @@ fmha_paged_tile_kernel(const __grid_constant__ Args a) {
                 mbar_init(smem_u32(&sm.bar_empty[s]), 1);
             }
             mbar_init(smem_u32(&sm.bar_s), 1);
-            mbar_init(smem_u32(&sm.bar_sfree), 32 * active);
-            mbar_init(smem_u32(&sm.bar_p), 32 * active);
+            mbar_init(smem_u32(&sm.bar_sfree), 64 * active);
+            mbar_init(smem_u32(&sm.bar_p), 64 * active);
             mbar_init(smem_u32(&sm.bar_pv), 1);
             mbar_init(smem_u32(&sm.bar_drain), 1);
             sm.abort_flag = 0;
@@ -374,17 +392,17 @@ fmha_paged_tile_kernel(const __grid_constant__ Args a) {
             issue_load(2 * j + 1, page);
             page = next;
         }
-    } else if (warp == 5) {
+    } else if (warp == kWarpMma) {
         tmem_alloc(smem_u32(&sm.tmem_base), kTileTmemCols);
         tmem_relinquish();
-    } else if (warp < 4 && n > 0) {
-        uint4 x[8];
-        const uint4* src = has_row ? reinterpret_cast<const uint4*>(q_row(a, token, head)) : nullptr;
+    } else if (warp < kSoftmaxWarps && n > 0) {
+        uint4 x[4];
+        const uint4* src = has_row ? reinterpret_cast<const uint4*>(q_row(a, token, head)) + half * 4 : nullptr;
 #pragma unroll
-        for (int c = 0; c < 8; ++c) x[c] = src ? __ldg(src + c) : make_uint4(0, 0, 0, 0);
-        uint4* dst = reinterpret_cast<uint4*>(sm.q) + threadIdx.x * 8;
+        for (int c = 0; c < 4; ++c) x[c] = src ? __ldg(src + c) : make_uint4(0, 0, 0, 0);
+        uint4* dst = reinterpret_cast<uint4*>(sm.q) + t * 8;
 #pragma unroll
-        for (int c = 0; c < 8; ++c) dst[c ^ (threadIdx.x & 7)] = x[c];
+        for (int c = 0; c < 4; ++c) dst[(half * 4 + c) ^ (t & 7)] = x[c];
         asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
     }
     tc_fence_before();
@@ -392,9 +410,9 @@ fmha_paged_tile_kernel(const __grid_constant__ Args a) {
     tc_fence_after();
     const uint32_t tmem = sm.tmem_base;
 
-    if (warp >= 4) {
+    if (warp >= kSoftmaxWarps) {
         regs_dec<kTileRegsControl>();
-        if (warp == 4 && n > 0) {
+        if (warp == kWarpLoad && n > 0) {
             // ---------------------------------------------------- loads
             bool ok = true;
             int issued = 2 * min(n, kAhead);
@@ -415,7 +433,7 @@ fmha_paged_tile_kernel(const __grid_constant__ Args a) {
                 for (int i = max(0, issued - kTileStages); i < issued; ++i)
                     drain_phase(smem_u32(&sm.bar_full[slot_of(i)]), phase_of(i), a);
             __syncwarp();
-        } else if (warp == 5 && n > 0) {
+        } else if (warp == kWarpMma && n > 0) {
             // ---------------------------------------------------- products
             const bool leader = elect_one();
             constexpr uint32_t idesc_qk = idesc_bf16_f32(kTileM, kTileN, 0, 0);
@@ -490,29 +508,27 @@ fmha_paged_tile_kernel(const __grid_constant__ Args a) {
     } else {
         regs_inc<kTileRegsSoftmax>();
         // -------------------------------------------------------- softmax
-        const int t = threadIdx.x;
-        if (warp < active) {
-            const uint32_t lane_base = (uint32_t)(warp * 32) << 16;
-            const uint32_t tS = tmem + lane_base + kColS, tO = tmem + lane_base + kColO,
-                           tP = tmem + lane_base + kColP;
+        if ((warp & 3) < active) {
+            const uint32_t lane_base = (uint32_t)((warp & 3) * 32) << 16;
+            const uint32_t tS = tmem + lane_base + kColS + half * 64, tO = tmem + lane_base + kColO + half * 32,
+                           tP = tmem + lane_base + kColP + half * 32;
+            const int pair_bar = 1 + (warp & 3);  // named barrier of the warps w and w + 4
             const float scale = a.scale;
-            const int lim = has_row ? key_limit(a, seq, tok) : kv_end;
+            const int lim = (has_row ? key_limit(a, seq, tok) : kv_end) - half * 64;
             const int lim_min = key_limit(a, seq, row0 / a.group);  // of the tile's first token
             float m_run = -INFINITY, l_run = 0.0f;
             bool ok = true;
             for (int j = 0; j < n; ++j) {
                 bool got = wait_phase(smem_u32(&sm.bar_s), j & 1, abort_flag, a);
-                if (!__all_sync(0xffffffffu, got)) {
-                    ok = false;
-                    break;
-                }
+                got = __all_sync(0xffffffffu, got);
+                if (!got) ok = false;
                 tc_fence_after();
-                uint32_t r[4][32];
-#pragma unroll
-                for (int c = 0; c < 4; ++c) tmem_ld32(tS + c * 32, r[c]);
+                uint32_t r[2][32];
+                tmem_ld32(tS, r[0]);
+                tmem_ld32(tS + 32, r[1]);
                 tmem_wait_ld();
-#pragma unroll
-                for (int c = 0; c < 4; ++c) reg_fence(r[c]);
+                reg_fence(r[0]);
+                reg_fence(r[1]);
                 tc_fence_before();
                 mbar_arrive(smem_u32(&sm.bar_sfree));
 
@@ -520,14 +536,14 @@ fmha_paged_tile_kernel(const __grid_constant__ Args a) {
                 const bool masked = k0 + kTileN > lim_min;
                 if (masked) {
 #pragma unroll
-                    for (int c = 0; c < 4; ++c)
+                    for (int c = 0; c < 2; ++c)
 #pragma unroll
                         for (int e = 0; e < 32; ++e)
                             if (k0 + c * 32 + e >= lim) r[c][e] = __float_as_uint(-INFINITY);
                 }
-                float mx[8];
+                float mx[4];
 #pragma unroll
-                for (int q = 0; q < 8; ++q) {
+                for (int q = 0; q < 4; ++q) {
                     const uint32_t* rr = &r[q >> 1][(q & 1) * 16];
                     mx[q] = __uint_as_float(rr[0]);
 #pragma unroll
@@ -535,25 +551,34 @@ fmha_paged_tile_kernel(const __grid_constant__ Args a) {
                         mx[q] = fmax3(mx[q], __uint_as_float(rr[e]), __uint_as_float(rr[e + 1]));
                     mx[q] = fmaxf(mx[q], __uint_as_float(rr[15]));
                 }
-                const float row_max = fmax3(fmax3(mx[0], mx[1], mx[2]), fmax3(mx[3], mx[4], mx[5]),
-                                            fmaxf(mx[6], mx[7]));
-                const float m_new = fmaxf(m_run, row_max);
-                const bool upd = (m_new - m_run) * scale > kLazyLog2;
+                const float half_max = fmax3(mx[0], mx[1], fmaxf(mx[2], mx[3]));
+                // Does either half of any of the 32 rows outgrow the reference (or
+                // did either warp give up)?  Seldom after the first tile.
+                const bool grew = (half_max - m_run) * scale > kLazyLog2;
                 float alpha = 1.0f;
-                if (upd) {
-                    alpha = ex2_approx((m_run - m_new) * scale);
-                    m_run = m_new;
+                bool any = bar_or(pair_bar, 64, grew || !ok);
+                if (any) {
+                    sm.half_max[half][t] = half_max;
+                    if (lane == 0) sm.half_ok[warp] = ok;
+                    bar_sync(pair_bar, 64);
+                    const float other = sm.half_max[half ^ 1][t];
+                    ok = sm.half_ok[warp] && sm.half_ok[warp ^ 4];  // the same for both warps
+                    if (!ok) break;
+                    const float m_new = fmaxf(half_max, other);
+                    if ((m_new - m_run) * scale > kLazyLog2) {
+                        alpha = ex2_approx((m_run - m_new) * scale);
+                        m_run = m_new;
+                    }
                 }
                 const float neg = m_run == -INFINITY ? 0.0f : -m_run * scale;
                 const float2 scale2 = make_float2(scale, scale), neg2 = make_float2(neg, neg);
-                float2 sum[4];
-#pragma unroll
-                for (int q = 0; q < 4; ++q) sum[q] = make_float2(0.0f, 0.0f);
-                uint32_t p[2][32];
+                float2 sum[2];
+                sum[0] = sum[1] = make_float2(0.0f, 0.0f);
+                uint32_t p[32];
                 auto exp_tile = [&](auto poly_tag) {
                     constexpr bool kPoly = decltype(poly_tag)::value;
 #pragma unroll
-                    for (int c = 0; c < 4; ++c)
+                    for (int c = 0; c < 2; ++c)
 #pragma unroll
                         for (int e = 0; e < 32; e += 2) {
                             const int pr = e >> 1;
@@ -564,41 +589,35 @@ fmha_paged_tile_kernel(const __grid_constant__ Args a) {
                                 pp = exp2_poly2(x);
                             else
                                 pp = make_float2(ex2_approx(x.x), ex2_approx(x.y));
-                            sum[pr & 3] = fadd2(sum[pr & 3], pp);
-                            p[c >> 1][(c & 1) * 16 + pr] = pack_bf16_rne(pp.x, pp.y);
+                            sum[pr & 1] = fadd2(sum[pr & 1], pp);
+                            p[c * 16 + pr] = pack_bf16_rne(pp.x, pp.y);
                         }
                 };
                 if (masked) exp_tile(std::false_type{});  // may hold -inf
                 else exp_tile(std::true_type{});
-                const float2 s01 = fadd2(fadd2(sum[0], sum[1]), fadd2(sum[2], sum[3]));
+                const float2 s01 = fadd2(sum[0], sum[1]);
                 l_run = fmaf(l_run, alpha, s01.x + s01.y);
                 if (j > 0) {
-                    // P(j-1) consumed, O settled.
+                    // P(j-1) consumed, O settled.  (Giving up waits for the next
+                    // tile's agreement with the row's other warp.)
                     got = wait_phase(smem_u32(&sm.bar_pv), (j - 1) & 1, abort_flag, a);
-                    if (!__all_sync(0xffffffffu, got)) {
-                        ok = false;
-                        break;
-                    }
+                    if (!__all_sync(0xffffffffu, got)) ok = false;
                     tc_fence_after();
                 }
-                tmem_st32(tP, p[0]);
-                tmem_st32(tP + 32, p[1]);
-                if (j > 0 && __any_sync(0xffffffffu, upd)) {
+                tmem_st32(tP, p);
+                if (j > 0 && any && __any_sync(0xffffffffu, alpha != 1.0f)) {
                     const float2 a2 = make_float2(alpha, alpha);
+                    uint32_t o[32];
+                    tmem_ld32(tO, o);
+                    tmem_wait_ld();
+                    reg_fence(o);
 #pragma unroll
-                    for (int c = 0; c < 2; ++c) {
-                        uint32_t o[32];
-                        tmem_ld32(tO + c * 32, o);
-                        tmem_wait_ld();
-                        reg_fence(o);
-#pragma unroll
-                        for (int e = 0; e < 32; e += 2) {
-                            const float2 y = fmul2(make_float2(__uint_as_float(o[e]), __uint_as_float(o[e + 1])), a2);
-                            o[e] = __float_as_uint(y.x);
-                            o[e + 1] = __float_as_uint(y.y);
-                        }
-                        tmem_st32(tO + c * 32, o);
+                    for (int e = 0; e < 32; e += 2) {
+                        const float2 y = fmul2(make_float2(__uint_as_float(o[e]), __uint_as_float(o[e + 1])), a2);
+                        o[e] = __float_as_uint(y.x);
+                        o[e + 1] = __float_as_uint(y.y);
                     }
+                    tmem_st32(tO, o);
                 }
                 tmem_wait_st();
                 tc_fence_before();
@@ -609,20 +628,22 @@ fmha_paged_tile_kernel(const __grid_constant__ Args a) {
                 const bool got = wait_phase(smem_u32(&sm.bar_pv), (n - 1) & 1, abort_flag, a);
                 ok = __all_sync(0xffffffffu, got);
             }
+            // The row's sum, from both halves.
+            sm.half_sum[half][t] = l_run;
+            if (bar_or(pair_bar, 64, !ok)) ok = false;
+            l_run += sm.half_sum[half ^ 1][t];
             if (ok) {
-                uint32_t o[2][32];
+                uint32_t o[32];
                 if (n > 0) {
                     tc_fence_after();
-                    tmem_ld32(tO, o[0]);
-                    tmem_ld32(tO + 32, o[1]);
+                    tmem_ld32(tO, o);
                     tmem_wait_ld();
-                    reg_fence(o[0]);
-                    reg_fence(o[1]);
+                    reg_fence(o);
                 }
                 float inv = l_run > 0.0f ? 1.0f / l_run : 0.0f;
                 float lse2 = l_run > 0.0f ? fmaf(m_run, scale, __log2f(l_run)) : -INFINITY;
                 auto val = [&](int col) {
-                    return n > 0 ? __uint_as_float(o[col >> 5][col & 31]) * inv : 0.0f;
+                    return n > 0 ? __uint_as_float(o[col]) * inv : 0.0f;
                 };
                 float* part_o = nullptr;
                 float* part_lse = nullptr;
@@ -635,32 +656,30 @@ fmha_paged_tile_kernel(const __grid_constant__ Args a) {
                     part_lse = a.out_lse + at;
                 }
                 if (has_row && part_o != nullptr) {
-                    *part_lse = lse2;
+                    if (half == 0) *part_lse = lse2;
                     if (l_run > 0.0f) {
-                        float4* dst = reinterpret_cast<float4*>(part_o);
+                        float4* dst = reinterpret_cast<float4*>(part_o) + half * 8;
 #pragma unroll
-                        for (int c = 0; c < 16; ++c)
+                        for (int c = 0; c < 8; ++c)
                             dst[c] = make_float4(val(4 * c), val(4 * c + 1), val(4 * c + 2), val(4 * c + 3));
                     }
                 } else if (has_row && a.part_n > 0) {
                     // Under a prefix: its results belong to the row, too.
-                    for (int c = 0; c < 2; ++c)
 #pragma unroll
-                        for (int e = 0; e < 32; e += 4)
-                            finish_row4(a, token, head, c * 32 + e, lse2, l_run > 0.0f ? 1.0f : 0.0f,
-                                        make_float4(c ? val(32 + e) : val(e), c ? val(33 + e) : val(e + 1),
-                                                    c ? val(34 + e) : val(e + 2), c ? val(35 + e) : val(e + 3)),
-                                        c == 0 && e == 0);
+                    for (int c = 0; c < 8; ++c)
+                        finish_row4(a, token, head, half * 32 + c * 4, lse2, l_run > 0.0f ? 1.0f : 0.0f,
+                                    make_float4(val(4 * c), val(4 * c + 1), val(4 * c + 2), val(4 * c + 3)),
+                                    half == 0 && c == 0);
                 } else if (has_row) {
-                    uint4* dst = reinterpret_cast<uint4*>(o_row(a, token, head));
+                    uint4* dst = reinterpret_cast<uint4*>(o_row(a, token, head)) + half * 4;
 #pragma unroll
-                    for (int c = 0; c < 8; ++c) {
+                    for (int c = 0; c < 4; ++c) {
                         uint32_t pk[4];
 #pragma unroll
                         for (int e = 0; e < 4; ++e) pk[e] = pack_bf16_rne(val(8 * c + 2 * e), val(8 * c + 2 * e + 1));
                         dst[c] = make_uint4(pk[0], pk[1], pk[2], pk[3]);
                     }
-                    if (a.lse != nullptr) *lse_at(a, token, head) = lse2 * kLn2;
+                    if (half == 0 && a.lse != nullptr) *lse_at(a, token, head) = lse2 * kLn2;
                 }
             }
         }
@@ -668,7 +687,7 @@ fmha_paged_tile_kernel(const __grid_constant__ Args a) {
 
     tc_fence_before();
     __syncthreads();
-    if (warp == 5) {
+    if (warp == kWarpMma) {
         tc_fence_after();
         tmem_dealloc(tmem, kTileTmemCols);
     }

@@ -46,8 +46,15 @@ constexpr int kMostRows = 16;         // rows of a K/V head that a warp holds
 constexpr int kRowStages = 3;
 // A sequence's start and end in a block cost about as much time as this many
 // units (its first loads, Q, the results); the shares count them.
-constexpr int kSeqCost = 2;
+constexpr int kSeqCost = 5;
 
+// A sequence as this kernel takes it.
+struct RowSeq {
+    int first, count, keys;
+    int kv_end;      // keys that any of its rows sees
+    int units;       // 0: not ours; a sequence that sees no key counts one (empty) unit
+    __device__ int cost() const { return units > 0 ? units + kSeqCost : 0; }
+};
 // A (sequence, head) result of a block: where it goes.
 struct Target {
     int first, rows;  // the sequence's first token; its rows per K/V head
@@ -66,6 +73,7 @@ struct alignas(1024) RowsShared {
     int piece_job[kRowWarps][2];      // segment of the block * heads + head, -1: none
     int scan[kRowWarps];
     int run[2 * kRowWarps + 1];
+    RowSeq start_seq;                 // of the block's first segment
     int start_b, start_x;
     int abort_flag;
 };
@@ -92,13 +100,6 @@ __device__ __forceinline__ RowsHeader* piece_headers(const Args& a) {
     return reinterpret_cast<RowsHeader*>(a.pieces + 2ll * kMaxRowBlocks * a.nhead_k * a.row_cap * (kHeadDim + 2));
 }
 
-// A sequence as this kernel takes it.
-struct RowSeq {
-    int first, count, keys;
-    int kv_end;      // keys that any of its rows sees
-    int units;       // 0: not ours; a sequence that sees no key counts one (empty) unit
-    __device__ int cost() const { return units > 0 ? units + kSeqCost : 0; }
-};
 __device__ __forceinline__ RowSeq load_row_seq(const Args& a, int b) {
     const Sequence s = load_sequence(a, b);
     RowSeq x{s.first, s.count, s.keys, 0, 0};
@@ -115,6 +116,9 @@ __device__ __forceinline__ RowSeq load_row_seq(const Args& a, int b) {
     return x;
 }
 
+__device__ __forceinline__ void prefetch_l1(const void* p) {
+    asm volatile("prefetch.global.L1 [%0];" ::"l"(p));
+}
 __device__ __forceinline__ void ldsm4(uint32_t addr, uint32_t (&r)[4]) {
     asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];"
                  : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(addr) : "memory");
@@ -129,9 +133,6 @@ __device__ __forceinline__ void mma_16816(float (&d)[4], const uint32_t (&a)[4],
         "{%0,%1,%2,%3};"
         : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
         : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
-}
-__device__ __forceinline__ void prefetch_l1(const void* p) {
-    asm volatile("prefetch.global.L1 [%0];" ::"l"(p));
 }
 __device__ __forceinline__ void fence_async_smem() {
     asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
@@ -222,10 +223,17 @@ fmha_paged_rows_kernel(const __grid_constant__ Args a) {
     if (beg >= before && beg < before + mine) {
         unsigned p = before;
         for (int b = b0; b < b1; ++b) {
-            const unsigned n = load_row_seq(a, b).cost();
+            const RowSeq x = load_row_seq(a, b);
+            const unsigned n = x.cost();
             if (beg < p + n) {
                 sm.start_b = b;
                 sm.start_x = (int)(beg - p);
+                sm.start_seq = x;
+                // The first page ids that the block will want.
+                const int page0 = (max(0, (int)(beg - p) - kSeqCost) * kUnit) >> a.page_shift;
+                const int32_t* ids = a.page_table + b * a.table_stride + page0;
+                if (page0 < a.max_pages) prefetch_l1(ids);
+                if (page0 + 32 < a.max_pages) prefetch_l1(ids + 32);
                 break;
             }
             p += n;
@@ -271,30 +279,17 @@ fmha_paged_rows_kernel(const __grid_constant__ Args a) {
     };
     Cursor c;
     c.b = sm.start_b;
-    c.x = load_row_seq(a, c.b);
+    c.x = sm.start_seq;
     c.seg = 0;
     c.left = (int)(end - beg);
     c.h = c.u = 0;
     set_segment(c, sm.start_x);
     bool any = c.n > 0 || next_segment(c);
-    // The block's tiles (unit x head), and what it has to say of its sequences.
-    RowsHeader header{0, 0, 0, 0};
-    unsigned long long tiles = 0;
+    const Cursor c0 = c;
+    unsigned long long tiles = 0;  // of the block: units x heads
     {
         Cursor k = c;
-        for (bool more = any; more; more = next_segment(k)) {
-            tiles += (unsigned long long)k.n * a.nhead_k;
-            if (k.unit0 != 0) continue;
-            int parts = 0;
-            if (k.n < k.x.units) {
-                // Only a last segment goes on; its cost ends that far past the block's.
-                parts = (int)(ranges.owner(end + (k.x.units - k.n) - 1) - blockIdx.x) + 1;
-                header.first = k.x.first;
-                header.rows = k.x.count * a.group;
-                header.parts = parts;
-            }
-            if (a.seq_parts != nullptr && threadIdx.x == 0) a.seq_parts[k.b] = make_int2(blockIdx.x, parts);
-        }
+        for (bool more = any; more; more = next_segment(k)) tiles += (unsigned long long)k.n * a.nhead_k;
     }
     const unsigned long long from = tiles * warp / kRowWarps;
     const long long count = (long long)(tiles * (warp + 1) / kRowWarps - from);
@@ -559,6 +554,24 @@ fmha_paged_rows_kernel(const __grid_constant__ Args a) {
                 drain_phase(smem_u32(&sm.bar[warp][i % kRowStages]), (i / kRowStages) & 1, a);
     }
 
+    // What the block has to say of the sequences that begin in it.
+    RowsHeader header{0, 0, 0, 0};
+    if (threadIdx.x == 0) {
+        Cursor k = c0;
+        for (bool more = any; more; more = next_segment(k)) {
+            if (k.unit0 != 0) continue;
+            int parts = 0;
+            if (k.n < k.x.units) {
+                // Only a last segment goes on; its cost ends that far past the block's.
+                parts = (int)(ranges.owner(end + (k.x.units - k.n) - 1) - blockIdx.x) + 1;
+                header.first = k.x.first;
+                header.rows = k.x.count * a.group;
+                header.parts = parts;
+            }
+            if (a.seq_parts != nullptr) a.seq_parts[k.b] = make_int2(blockIdx.x, parts);
+        }
+    }
+
     // --------------------------------------------- the block's fold of pieces
     griddep_wait();  // the grid ends after the launch before it
     if (threadIdx.x == 0) piece_headers(a)[blockIdx.x] = header;
@@ -653,12 +666,11 @@ fmha_paged_rows_merge(const __grid_constant__ Args a) {
 __global__ void __launch_bounds__(256)
 fmha_prefix_finish(const __grid_constant__ Args a) {
     constexpr int kBatch = 8;
-    griddep_wait();
     const long long row = ((long long)blockIdx.x * 256 + threadIdx.x) >> 4;
     const long long all_rows = (long long)a.tokens * a.nhead_q;
-    if (row >= all_rows) return;
     const int c4 = threadIdx.x & 15;
-    const int token = (int)(row / a.nhead_q), head = (int)(row - (long long)token * a.nhead_q);
+    bool mine = row < all_rows;
+    const int token = mine ? (int)(row / a.nhead_q) : 0, head = mine ? (int)(row - (long long)token * a.nhead_q) : 0;
     int b = token / a.row_div;
     if (a.seqstart_q != nullptr) {
         b = 0;
@@ -670,36 +682,46 @@ fmha_prefix_finish(const __grid_constant__ Args a) {
     }
     const Sequence s = load_sequence(a, b);
     const int rows = s.count * a.group;
-    if (token < s.first || token >= s.first + s.count || rows < a.min_rows || rows > a.max_rows) return;
     const int h = head / a.group, rt = (token - s.first) * a.group + head - h * a.group;
-    if (rt >= a.row_cap) return;  // more tokens than the call said
+    mine = mine && token >= s.first && token < s.first + s.count && rows >= a.min_rows && rows <= a.max_rows &&
+           rt < a.row_cap;  // (past the cap: more tokens than the call said)
+    griddep_wait();  // every thread: the grid ends after the launches before it
+    if (!mine) return;
     const int2 parts = a.seq_parts[b];  // its first block, and how many share it
-    const int own = max(1, parts.y);
     float m = -INFINITY, l = 0.0f;
     float4 o = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-    for (int k0 = 0; k0 < a.part_n + own; k0 += kBatch) {
+    // The prefix's parts and the sequence's own, if one (what is read there
+    // otherwise stays out).
+    for (int k0 = 0; k0 <= a.part_n; k0 += kBatch) {
+        float m2[kBatch];
+        float4 x[kBatch];
+#pragma unroll
+        for (int u = 0; u < kBatch; ++u) {
+            m2[u] = -INFINITY;
+            x[u] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+            if (k0 + u > a.part_n) continue;
+            m2[u] = a.part_lse[(k0 + u) * all_rows + row];
+            x[u] = *reinterpret_cast<const float4*>(a.part_o + ((k0 + u) * all_rows + row) * kHeadDim + c4 * 4);
+        }
+#pragma unroll
+        for (int u = 0; u < kBatch; ++u)
+            if (m2[u] != -INFINITY && k0 + u < a.part_n + (parts.y == 0))  // -inf: O may be unwritten
+                fold4(m, l, o, m2[u], 1.0f, x[u]);
+    }
+    for (int k0 = 0; k0 < parts.y; k0 += kBatch) {
         float2 ml[kBatch];
         float4 x[kBatch];
 #pragma unroll
         for (int u = 0; u < kBatch; ++u) {
-            const int k = k0 + u, piece = k - a.part_n;
-            ml[u] = make_float2(-INFINITY, 1.0f);
+            ml[u] = make_float2(-INFINITY, 0.0f);
             x[u] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-            if (k >= a.part_n + own) continue;
-            const float* src;
-            if (piece >= 0 && parts.y > 0) {
-                const long long at = piece_row(a, 2 * (parts.x + piece) + (piece == 0), h, rt);
-                ml[u] = *reinterpret_cast<const float2*>(piece_ml(a, at));
-                src = piece_o(a, at);
-            } else {  // the prefix's parts, then the sequence's own
-                ml[u].x = a.part_lse[k * all_rows + row];
-                src = a.part_o + (k * all_rows + row) * kHeadDim;
-            }
-            x[u] = *reinterpret_cast<const float4*>(src + c4 * 4);
+            if (k0 + u >= parts.y) continue;
+            const long long at = piece_row(a, 2 * (parts.x + k0 + u) + (k0 + u == 0), h, rt);
+            ml[u] = *reinterpret_cast<const float2*>(piece_ml(a, at));
+            x[u] = *reinterpret_cast<const float4*>(piece_o(a, at) + c4 * 4);
         }
 #pragma unroll
-        for (int u = 0; u < kBatch; ++u)
-            if (ml[u].x != -INFINITY) fold4(m, l, o, ml[u].x, ml[u].y, x[u]);  // else O may be unwritten
+        for (int u = 0; u < kBatch; ++u) fold4(m, l, o, ml[u].x, ml[u].y, x[u]);
     }
     write_row4(a, token, head, c4 * 4, m, l, o, c4 == 0);
 }

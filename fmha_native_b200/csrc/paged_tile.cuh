@@ -32,8 +32,8 @@
 // Work split.  A shared prefix has one length, so the host cuts every row
 // tile's keys into `splits` equal ranges, a block each, and whatever ends the
 // call folds their results.  Sequences' own keys differ as they like: the
-// blocks themselves agree, from the lengths, on a range length that makes about
-// one or two ranges per resident block, cut each (row tile, head) job into that
+// blocks themselves agree, from the lengths, on a range length that keeps every
+// resident block busy, cut each (row tile, head) job into that
 // many equal ranges, and take one range each (find_item); jobs of one range go
 // to the output, the others through scratch slots that fmha_paged_combine folds.
 #pragma once
@@ -57,7 +57,8 @@ constexpr uint32_t kColS = 0, kColO = 128, kColP = 192;
 constexpr int kTileRegsSoftmax = 96, kTileRegsControl = 48;
 static_assert(256 * kTileRegsSoftmax + 128 * kTileRegsControl <= kTileThreads * 80, "register split");
 constexpr float kLazyLog2 = 8.0f;
-constexpr int kLongRange = 16;  // key tiles of a range from which blocks take two
+constexpr int kLongRange = 16;  // key tiles up to which a job is not worth cutting where jobs abound
+constexpr unsigned kMostParts = 64;  // ranges of a job (their fold is one block's work per 32 rows)
 constexpr int kPolyOf16 = 4;  // pairs of every 16 whose exponential runs on the FMA pipe
 
 struct alignas(1024) TileShared {
@@ -82,8 +83,10 @@ constexpr int kMaxTileSlots = 4 * kTileBlocks;
 constexpr int kMaxPlanned = 8000;  // row tiles and sequences up to which find_item plans
 constexpr int kMostCounted = 0x7fffffff / kMaxPlanned;  // key tiles of a row tile that a plan counts
 struct TileHeader {
-    int b, m, h;  // the job
-    int parts;    // its ranges, in the slots from this one on, nhead_k apart; 0: no job begins here
+    int first;         // the job: its sequence's first token, the tile's rows
+    int row0, rows, h; // row0 .. row0 + rows - 1 of K/V head h
+    int parts;         // its ranges, in the slots from this one on, nhead_k apart; 0: no job begins here
+    int pad[3];
 };
 __host__ __device__ constexpr size_t tile_slot_floats() { return (size_t)kTileM * (kHeadDim + 1); }
 __device__ __forceinline__ float* tile_slot_o(const Args& a, int slot) {
@@ -247,19 +250,29 @@ __device__ __forceinline__ bool find_item(const Args& a, TileShared& sm, int* in
         }
     }
     block_scan(mine, sm.scan_a, total);
-    // One range per resident block while ranges are short, two beyond.
+    // The range length.  Fewer jobs than resident blocks: the ranges that fill
+    // the device once; the shortest length that may do, or else (jobs round up)
+    // the one that surely does.  More jobs: cut only what is longer than half a
+    // block's share.
     const long long all = (long long)total * a.nhead_k;
+    const int jobs = tiles * a.nhead_k;
     long long len = (all + kTileBlocks - 1) / kTileBlocks;
-    if (len > kLongRange) len = max((long long)kLongRange, (all + 2 * kTileBlocks - 1) / (2 * kTileBlocks));
-    const unsigned most = (unsigned)min(len, 0x7fffffffll);
-    auto parts_of = [&](int n) { return (int)(((unsigned)min(n, kMostCounted) + most - 1) / most); };
-    int both = 0;  // items in the upper half, those of split jobs in the lower
-    for (int t = t0; t < t1; ++t) {
-        const int p = parts_of(keys[t]);
-        both += p << 16 | (p > 1 ? p : 0);
+    if (jobs >= kTileBlocks) len = max((long long)kLongRange, (all + 2 * kTileBlocks - 1) / (2 * kTileBlocks));
+    int both, before, sum;
+    unsigned most;
+    auto parts_of = [&](int n) { return (int)min(((unsigned)min(n, kMostCounted) + most - 1) / most, kMostParts); };
+    for (bool again = false;; again = true) {
+        most = (unsigned)min(max(len, 1ll), 0x7fffffffll);
+        both = 0;  // items in the upper half, those of split jobs in the lower
+        for (int t = t0; t < t1; ++t) {
+            const int p = parts_of(keys[t]);
+            both += p << 16 | (p > 1 ? p : 0);
+        }
+        before = block_scan(both, sm.scan_b, sum);
+        if (again || jobs >= kTileBlocks || (sum >> 16) * a.nhead_k <= kTileBlocks) break;
+        len = (all + kTileBlocks - jobs - 1) / (kTileBlocks - jobs);
+        __syncthreads();  // scan_b is written again
     }
-    int sum;
-    const int before = block_scan(both, sm.scan_b, sum);
     const int split = sum & 0xffff;
     // No job begins in the slots that stay unused.
     for (int i = split * a.nhead_k + (int)blockIdx.x * kTileThreads + tid; i < a.max_slots;
@@ -327,7 +340,7 @@ fmha_paged_tile_kernel(const __grid_constant__ Args a) {
     const bool shared_job = a.plan && it.parts > 1;  // through a scratch slot
     const int slot_job = it.slot + it.k * a.nhead_k + kvh;
     if (shared_job && it.k == 0 && threadIdx.x == 0)
-        tile_headers(a)[slot_job] = TileHeader{it.b, it.m, kvh, it.parts};
+        tile_headers(a)[slot_job] = TileHeader{seq.first, row0, row_end - row0, kvh, it.parts, {0, 0, 0}};
     else if (shared_job && threadIdx.x == 0)
         tile_headers(a)[slot_job].parts = 0;
     const int tail = kv_end - (j0 + n - 1) * kTileN;  // visible keys of the range's last tile
@@ -693,15 +706,15 @@ fmha_paged_tile_kernel(const __grid_constant__ Args a) {
     }
 }
 
-// Folds the ranges of the jobs that several blocks shared into final rows: a
-// block looks after the slots blockIdx.x + i * gridDim.x; 16 threads per row,
-// four columns each, kBatch ranges in flight.
+// Folds the ranges of the jobs that several blocks shared into final rows:
+// blockIdx.y takes 32 rows of the jobs that begin in the slots blockIdx.x + i *
+// gridDim.x; 16 threads per row, four columns each, kBatch ranges in flight.
 constexpr int kCombineBlocks = 148;
 constexpr int kCombineThreads = 512;
 __global__ void __launch_bounds__(kCombineThreads)
 fmha_paged_combine(const __grid_constant__ Args a) {
     constexpr int kEach = (kMaxTileSlots + kCombineBlocks - 1) / kCombineBlocks;
-    constexpr int kBatch = 4;
+    constexpr int kBatch = 8;
     griddep_wait();
     TileHeader head[kEach];
 #pragma unroll
@@ -710,37 +723,32 @@ fmha_paged_combine(const __grid_constant__ Args a) {
         head[i].parts = 0;
         if (slot < a.max_slots) head[i] = tile_headers(a)[slot];
     }
-    const int c4 = threadIdx.x & 15;
+    const int c4 = threadIdx.x & 15, rt = blockIdx.y * 32 + (int)(threadIdx.x >> 4);
 #pragma unroll
     for (int i = 0; i < kEach; ++i) {
-        if (head[i].parts == 0) continue;
+        if (rt >= head[i].rows || head[i].parts == 0) continue;
         const int slot0 = blockIdx.x + i * kCombineBlocks;
-        const Sequence seq = load_sequence(a, head[i].b);
-        const int row0 = head[i].m * kTileM;
-        const int rows = min(kTileM, seq.count * a.group - row0);
-        for (int rt = threadIdx.x >> 4; rt < rows; rt += kCombineThreads / 16) {
-            float m = -INFINITY, l = 0.0f;
-            float4 o = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-            for (int k0 = 0; k0 < head[i].parts; k0 += kBatch) {
-                float m2[kBatch];
-                float4 x[kBatch];
+        float m = -INFINITY, l = 0.0f;
+        float4 o = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+        for (int k0 = 0; k0 < head[i].parts; k0 += kBatch) {
+            float m2[kBatch];
+            float4 x[kBatch];
 #pragma unroll
-                for (int u = 0; u < kBatch; ++u) {
-                    m2[u] = -INFINITY;
-                    x[u] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-                    if (k0 + u < head[i].parts) {
-                        const int slot = slot0 + (k0 + u) * a.nhead_k;
-                        m2[u] = tile_slot_lse(a, slot)[rt];
-                        x[u] = *reinterpret_cast<const float4*>(tile_slot_o(a, slot) + rt * kHeadDim + c4 * 4);
-                    }
+            for (int u = 0; u < kBatch; ++u) {
+                m2[u] = -INFINITY;
+                x[u] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+                if (k0 + u < head[i].parts) {
+                    const int slot = slot0 + (k0 + u) * a.nhead_k;
+                    m2[u] = tile_slot_lse(a, slot)[rt];
+                    x[u] = *reinterpret_cast<const float4*>(tile_slot_o(a, slot) + rt * kHeadDim + c4 * 4);
                 }
-#pragma unroll
-                for (int u = 0; u < kBatch; ++u)
-                    if (m2[u] != -INFINITY) fold4(m, l, o, m2[u], 1.0f, x[u]);  // else O was not written
             }
-            const int row = row0 + rt, t = row / a.group;
-            finish_row4(a, seq.first + t, head[i].h * a.group + row - t * a.group, c4 * 4, m, l, o, c4 == 0);
+#pragma unroll
+            for (int u = 0; u < kBatch; ++u)
+                if (m2[u] != -INFINITY) fold4(m, l, o, m2[u], 1.0f, x[u]);  // else O was not written
         }
+        const int row = head[i].row0 + rt, t = row / a.group;
+        finish_row4(a, head[i].first + t, head[i].h * a.group + row - t * a.group, c4 * 4, m, l, o, c4 == 0);
     }
 }
 

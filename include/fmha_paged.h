@@ -66,13 +66,13 @@ typedef struct FmhaRopeParams {
 
 /* q_out, k_out = rotated q, k.  q or k may be NULL.  A token whose position is
  * outside the angle table gets zero rows. */
-int fmha_rope_d64_bf16(const FmhaRopeParams* params, CUstream_st* stream);
+int fmha_rope_d64_bf16(const FmhaRopeParams* params, struct CUstream_st* stream);
 
 /* New K and V, K rotated, into the pages of the cache; q, if given, rotated
  * into q_out.  A token whose place is negative (a batch slot with fewer keys
  * than new tokens, such as an empty slot) is not stored, and its q_out row is
  * zero.  No two tokens of a call may name the same place. */
-int fmha_paged_append_d64_bf16(const FmhaRopeParams* params, CUstream_st* stream);
+int fmha_paged_append_d64_bf16(const FmhaRopeParams* params, struct CUstream_st* stream);
 
 typedef struct FmhaPagedParams {
     const uint16_t* q;       /* dense [batch, seqlen_q, nhead_q, 64] or packed [total_q, nhead_q, 64], any strides */
@@ -108,12 +108,12 @@ size_t fmha_paged_workspace_bytes(int batch, int seqlen_q, int total_q, int nhea
 
 /* O = softmax(scale * Q K^T + mask) V over each sequence's pages.  A row that
  * sees no key gets O = 0 and LSE = -inf. */
-int fmha_paged_fwd_d64_bf16(const FmhaPagedParams* params, CUstream_st* stream);
+int fmha_paged_fwd_d64_bf16(const FmhaPagedParams* params, struct CUstream_st* stream);
 
 /* The same where every sequence's keys are the prefix_len keys of
  * prefix_pages followed by its own seqlens_k[b] ones: the prefix is read once
  * for the whole batch.  prefix_len >= 1. */
-int fmha_prefix_fwd_d64_bf16(const FmhaPagedParams* params, CUstream_st* stream);
+int fmha_prefix_fwd_d64_bf16(const FmhaPagedParams* params, struct CUstream_st* stream);
 
 #ifdef __cplusplus
 }

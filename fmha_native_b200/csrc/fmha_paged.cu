@@ -47,12 +47,13 @@ struct Plan {
     bool rows, tile;          // which kernels serve the sequences' own keys
     int row_cap;              // max_rows for the rows kernel's sequences
     long long tiles;          // row tiles of the tile kernel (at most)
-    bool planned;             // it plans its key ranges by the lengths
+    int plan;                 // how its key ranges are found
+    long long ranges;         // and how many they are at most
     long long prefix_tiles;   // row tiles against the prefix, and their key ranges
     int prefix_splits;
-    // Bytes: the two kernels' scratch; under a prefix, what the rows kernel says of
-    // the sequences, and one partial result of all rows.
-    size_t pieces, slots, info, part;
+    // Bytes: the two kernels' scratch, the list of work; under a prefix, what the
+    // rows kernel says of the sequences, and one partial result of all rows.
+    size_t pieces, slots, list, info, part;
     int parts;                // partial results: the prefix's, then the rows kernel's
     size_t total;
 };
@@ -98,9 +99,12 @@ bool make_plan(int batch, int seqlen_q, int total_q, bool packed, int nhead_q, i
         z.tiles = packed ? all / kTileM + std::min<long long>(batch, all / (kMostRows + 1))
                          : (max_rows + kTileM - 1) / kTileM * batch;
         if ((z.tiles + 2 * kTileBlocks) * nhead_k > INT_MAX) return false;
-        z.planned = z.tiles <= kMaxPlanned && batch <= kMaxPlanned;
-        if (z.planned)
-            z.slots = round16(kMaxTileSlots * (tile_slot_floats() * sizeof(float) + sizeof(TileHeader)));
+        // A range per resident block, or per row tile and two per resident block.
+        const long long resident = (kTileBlocks + nhead_k - 1) / nhead_k;
+        z.plan = z.tiles * nhead_k < kTileBlocks ? kPlanHere : kPlanList;
+        z.ranges = z.plan == kPlanHere ? resident : z.tiles + 2 * resident;
+        z.slots = round16(kMaxTileSlots * (tile_slot_floats() * sizeof(float) + sizeof(TileHeader)));
+        if (z.plan == kPlanList) z.list = round16(z.ranges * sizeof(TileItem) + (batch + 2) * sizeof(int));
     }
     if (prefix_len > 0) {
         z.prefix_tiles = (z.tokens * z.group + kTileM - 1) / kTileM;
@@ -109,7 +113,7 @@ bool make_plan(int batch, int seqlen_q, int total_q, bool packed, int nhead_q, i
         z.parts = z.prefix_splits + (z.rows ? 1 : 0);
         z.info = round16(batch * sizeof(int2));
     }
-    z.total = z.pieces + z.slots + z.info + z.part * z.parts;
+    z.total = z.pieces + z.slots + z.list + z.info + z.part * z.parts;
     return true;
 }
 
@@ -245,13 +249,15 @@ int launch_rows(const Args& a, const Args* finish, bool after, int device, cudaS
                             a);
 }
 
-// `ranges`: row tiles and, cut by the plan or the host, their key ranges.
-int launch_tile(const Args& a, long long ranges, int device, cudaStream_t stream) {
+// `ranges`: key ranges of row tiles; after: right behind the kernel that lists them.
+int launch_tile(const Args& a, long long ranges, bool after, int device, cudaStream_t stream) {
     constexpr size_t smem = sizeof(TileShared) + 1024;
     static std::atomic<unsigned long long> ready{0};
     if (!allow_smem(ready, device, reinterpret_cast<const void*>(fmha_paged_tile_kernel), smem))
         return FMHA_ERR_LAUNCH;
-    fmha_paged_tile_kernel<<<(unsigned)(ranges * a.nhead_k), kTileThreads, smem, stream>>>(a);
+    const dim3 grid((unsigned)(ranges * a.nhead_k));
+    if (after) return launch_dependent(fmha_paged_tile_kernel, grid, kTileThreads, smem, stream, a);
+    fmha_paged_tile_kernel<<<grid, kTileThreads, smem, stream>>>(a);
     return cudaGetLastError() == cudaSuccess ? FMHA_OK : FMHA_ERR_LAUNCH;
 }
 
@@ -267,12 +273,24 @@ int run(const FmhaPagedParams* p, bool prefix, cudaStream_t stream) {
     a.pieces = reinterpret_cast<float*>(scratch);
     a.slots = reinterpret_cast<float*>(scratch + z.pieces);
     const size_t part_rows = (size_t)z.tokens * p->nhead_q;
-    float* part_o = reinterpret_cast<float*>(scratch + z.pieces + z.slots + z.info);
+    uint8_t* list = scratch + z.pieces + z.slots;
+    int2* info = reinterpret_cast<int2*>(list + z.list);
+    float* part_o = reinterpret_cast<float*>(list + z.list + z.info);
     float* part_lse = part_o + part_rows * kHeadDim * z.parts;
-    a.splits = 1;
     if (z.tile || prefix) {
         Args t = a;
         if ((st = cache_maps(ctx, t, p, kTileN)) != FMHA_OK) return st;
+        t.min_rows = kMostRows + 1;
+        t.max_slots = kMaxTileSlots;
+        if (z.tile && z.plan == kPlanList) {
+            t.items = reinterpret_cast<TileItem*>(list);
+            t.max_items = (int)z.ranges;
+            t.max_tiles = (int)z.tiles;
+            t.item_count = reinterpret_cast<int*>(t.items + z.ranges);
+            t.tile_first = t.item_count + 1;
+            fmha_paged_plan<<<1, kPlanThreads, 0, stream>>>(t);
+            if (cudaGetLastError() != cudaSuccess) return FMHA_ERR_LAUNCH;
+        }
         if (prefix) {
             // Every token's rows against the prefix, as one sequence without mask.
             Args b = t;
@@ -283,25 +301,20 @@ int run(const FmhaPagedParams* p, bool prefix, cudaStream_t stream) {
             b.batch = 1;
             b.seqlen_q = a.tokens;
             b.causal = 0;
+            b.min_rows = 1;
             b.splits = z.prefix_splits;
             b.out_o = part_o;
             b.out_lse = part_lse;
-            if ((st = launch_tile(b, z.prefix_tiles * z.prefix_splits, ctx.device, stream)) != FMHA_OK) return st;
+            st = launch_tile(b, z.prefix_tiles * z.prefix_splits, false, ctx.device, stream);
+            if (st != FMHA_OK) return st;
             a.part_o = t.part_o = part_o;
             a.part_lse = t.part_lse = part_lse;
             t.part_n = z.prefix_splits;
         }
         if (z.tile) {
-            t.min_rows = kMostRows + 1;
-            t.plan = z.planned;
-            t.max_slots = kMaxTileSlots;
-            // What a plan makes at most (find_item): a range per resident block, or
-            // two and one per row tile.
-            const long long resident = (kTileBlocks + p->nhead_k - 1) / p->nhead_k;
-            const long long ranges = !z.planned                                  ? z.tiles
-                                     : z.tiles * p->nhead_k < kTileBlocks ? resident
-                                                                                 : z.tiles + 2 * resident;
-            if ((st = launch_tile(t, ranges, ctx.device, stream)) != FMHA_OK) return st;
+            t.plan = z.plan;
+            st = launch_tile(t, z.ranges, z.plan == kPlanList && !prefix, ctx.device, stream);
+            if (st != FMHA_OK) return st;
         }
     }
     if (z.rows) {
@@ -311,14 +324,14 @@ int run(const FmhaPagedParams* p, bool prefix, cudaStream_t stream) {
         Args finish = a;
         if (prefix) {
             finish.part_n = z.prefix_splits;
-            a.seq_parts = finish.seq_parts = reinterpret_cast<int2*>(scratch + z.pieces + z.slots);
+            a.seq_parts = finish.seq_parts = info;
             a.out_o = part_o + part_rows * kHeadDim * z.prefix_splits;
             a.out_lse = part_lse + part_rows * z.prefix_splits;
         }
         st = launch_rows(a, prefix ? &finish : nullptr, z.tile || prefix, ctx.device, stream);
         if (st != FMHA_OK) return st;
     }
-    if (z.tile && z.planned) {
+    if (z.tile) {
         a.max_slots = kMaxTileSlots;
         a.part_n = z.prefix_splits;
         st = launch_dependent(fmha_paged_combine, dim3(kCombineBlocks, (std::min(z.max_rows, kTileM) + 31) / 32), kCombineThreads, 0, stream, a);

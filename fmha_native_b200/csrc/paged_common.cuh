@@ -22,6 +22,9 @@ constexpr float kLn2 = 0.69314718055994531f;
 // rows of a sequence are (token, query head of the group), group fastest:
 // row r is token r / group, query head kvh * group + r % group, so all rows
 // that read the same keys sit in one tile.
+enum : int { kPlanNone, kPlanHere, kPlanList };
+struct TileItem;
+
 struct Args {
     CUtensorMap tm_k;
     CUtensorMap tm_v;
@@ -55,9 +58,13 @@ struct Args {
     // split s into slot s); null: it writes final rows.
     float* out_o;
     float* out_lse;
-    int splits;                 // tile kernel, plan == 0: key ranges per row tile
-    int plan;                   // tile kernel: ranges by the lengths (find_item)
-    float* slots;               // and the scratch of the jobs that blocks share
+    int plan;                   // tile kernel: where its blocks' work comes from
+    int splits;                 // kPlanNone: key ranges per row tile
+    TileItem* items;            // kPlanList: the list, its length, and scratch to make it
+    int* item_count;
+    int* tile_first;
+    int max_tiles, max_items;
+    float* slots;               // scratch of the jobs that blocks share
     int max_slots;
     float* pieces;              // rows kernel: scratch between its blocks
     int2* seq_parts;            // rows kernel under a prefix: per sequence its first block and, if

@@ -31,11 +31,13 @@
 //
 // Work split.  A shared prefix has one length, so the host cuts every row
 // tile's keys into `splits` equal ranges, a block each, and whatever ends the
-// call folds their results.  Sequences' own keys differ as they like: the
-// blocks themselves agree, from the lengths, on a range length that keeps every
-// resident block busy, cut each (row tile, head) job into that
-// many equal ranges, and take one range each (find_item); jobs of one range go
-// to the output, the others through scratch slots that fmha_paged_combine folds.
+// call folds their results (kPlanNone).  Sequences' own keys differ as they
+// like, and their lengths are on the device: with fewer (row tile, head) jobs
+// than resident blocks, every block works out for itself the ranges that keep
+// all of them busy (kPlanHere); with more, a first kernel writes the list of
+// whole tiles, cutting only what is far longer than the rest (kPlanList).  Jobs
+// of one range go to the output, the others through scratch slots that
+// fmha_paged_combine folds.
 #pragma once
 #include <type_traits>
 
@@ -58,8 +60,32 @@ constexpr int kTileRegsSoftmax = 96, kTileRegsControl = 48;
 static_assert(256 * kTileRegsSoftmax + 128 * kTileRegsControl <= kTileThreads * 80, "register split");
 constexpr float kLazyLog2 = 8.0f;
 constexpr int kLongRange = 16;  // key tiles up to which a job is not worth cutting where jobs abound
-constexpr unsigned kMostParts = 64;  // ranges of a job (their fold is one block's work per 32 rows)
+constexpr int kMostParts = 64;  // ranges of a job (their fold is one block's work per 32 rows)
 constexpr int kPolyOf16 = 4;  // pairs of every 16 whose exponential runs on the FMA pipe
+
+// A block's work (for one K/V head): range k of the keys of a row tile.
+struct alignas(16) TileItem {
+    int b, first, count, keys;    // the sequence
+    int row0, row_end;            // the tile's rows
+    int kv_end, j0, n;            // keys that any of them sees; the range's key tiles
+    int k, parts;                 // which range of how many
+    int slot;                     // scratch slot of the job's first range (parts > 1), for head 0; -1: none
+};
+__device__ __forceinline__ TileItem make_item(const Args& a, int b, const Sequence& s, int m, int k, int parts,
+                                              int slot) {
+    TileItem it;
+    it.b = b, it.first = s.first, it.count = s.count, it.keys = s.keys;
+    it.row0 = m * kTileM;
+    it.row_end = min(s.count * a.group, it.row0 + kTileM);
+    it.kv_end = max(0, key_limit(a, s, (it.row_end - 1) / a.group));
+    const int all = (it.kv_end + kTileN - 1) / kTileN;
+    const int each = all / parts, more = all - each * parts;
+    it.j0 = k * each + min(k, more);
+    it.n = each + (k < more);
+    it.k = k, it.parts = parts;
+    it.slot = slot;
+    return it;
+}
 
 struct alignas(1024) TileShared {
     uint8_t q[kTileBytes];
@@ -73,15 +99,16 @@ struct alignas(1024) TileShared {
     uint64_t bar_drain;
     uint32_t tmem_base;
     int abort_flag;
-    int scan_a[kTileWarps], scan_b[kTileWarps], item[8];
+    int scan[kTileWarps];
+    long long scan64[kTileWarps];
+    TileItem item;
+    int2 tile_of[kTileThreads];
     float half_max[2][kTileM], half_sum[2][kTileM];  // between the two threads of a row
     int half_ok[kSoftmaxWarps];
 };
 
 // Scratch of the jobs that several blocks share.
 constexpr int kMaxTileSlots = 4 * kTileBlocks;
-constexpr int kMaxPlanned = 8000;  // row tiles and sequences up to which find_item plans
-constexpr int kMostCounted = 0x7fffffff / kMaxPlanned;  // key tiles of a row tile that a plan counts
 struct TileHeader {
     int first;         // the job: its sequence's first token, the tile's rows
     int row0, rows, h; // row0 .. row0 + rows - 1 of K/V head h
@@ -112,33 +139,27 @@ __device__ __forceinline__ bool bar_or(int id, int threads, bool p) {
     return r != 0;
 }
 
-// A block's work: range k of `parts` of the keys of row tile m of sequence b.
-static_assert((2 * kMaxPlanned + 1) * 4 <= kTileStages * kTileBytes, "find_item's integers fit the ring");
-static_assert(kMaxPlanned + 2 * kTileBlocks < 32768 && 4 * kTileBlocks < 65536, "find_item's packed sums");
-struct Item {
-    int b, m, k, parts;
-    int slot;  // scratch slot of the job's first range (where parts > 1), for head 0
-};
-
-// Exclusive scan of `mine` over the block; `total` = the sum.
-__device__ __forceinline__ int block_scan(int mine, int (&warp_sums)[kTileWarps], int& total) {
+// Exclusive scan of `mine` over a block of kWarps warps; `total` = the sum.
+template <int kWarps, typename T>
+__device__ __forceinline__ T block_scan(T mine, T (&warp_sums)[kWarps], T& total) {
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    int incl = mine;
+    T incl = mine;
 #pragma unroll
     for (int d = 1; d < 32; d <<= 1) {
-        const int v = __shfl_up_sync(0xffffffffu, incl, d);
+        const T v = __shfl_up_sync(0xffffffffu, incl, d);
         if (lane >= d) incl += v;
     }
     if (lane == 31) warp_sums[warp] = incl;
     __syncthreads();
-    int before = incl - mine;
+    T before = incl - mine;
     total = 0;
 #pragma unroll
-    for (int w = 0; w < kTileWarps; ++w) {
-        const int v = warp_sums[w];
+    for (int w = 0; w < kWarps; ++w) {
+        const T v = warp_sums[w];
         if (w < warp) before += v;
         total += v;
     }
+    __syncthreads();  // warp_sums may be used again
     return before;
 }
 
@@ -146,74 +167,105 @@ __device__ __forceinline__ int tile_count(const Args& a, const Sequence& s) {
     const int rows = s.count * a.group;
     return rows < a.min_rows || rows > a.max_rows ? 0 : (rows + kTileM - 1) / kTileM;
 }
-__device__ __forceinline__ int tile_kv_end(const Args& a, const Sequence& s, int m) {
+// Key tiles of row tile m, at least one.
+__device__ __forceinline__ int key_tiles(const Args& a, const Sequence& s, int m) {
     const int row_end = min(s.count * a.group, (m + 1) * kTileM);
-    return max(0, key_limit(a, s, (row_end - 1) / a.group));
+    return max(1, (key_limit(a, s, (row_end - 1) / a.group) + kTileN - 1) / kTileN);
+}
+__device__ __forceinline__ int parts_of(int n, long long len) {
+    return n <= len ? 1 : min((n + (int)len - 1) / (int)len, kMostParts);
 }
 
-// Item `y` of the grid and its sequence, tiles of later tokens (the ones with
-// more keys) first.  All threads; `ints` is shared memory for 2 * kMaxPlanned + 1
-// integers.  False: past the last one.
-__device__ __forceinline__ bool find_item(const Args& a, TileShared& sm, int* ints, int y, Item& it, Sequence& seq) {
-    const bool packed = a.seqstart_q != nullptr;
+// The plan for fewer jobs (row tile, head) than resident blocks, by every block
+// for itself: the shortest range length whose ranges all fit the device at
+// once.  All threads; false: no item for this block.
+__device__ __forceinline__ bool plan_here(const Args& a, TileShared& sm, int y, TileItem& it) {
     const int tid = threadIdx.x;
-    const int per_seq = packed ? 1 : (a.seqlen_q * a.group + kTileM - 1) / kTileM;
-    if (!a.plan) {
-        // Every tile whole, or cut as the host said, without a look at the lengths.
-        const int x = y / a.splits;
-        it.k = y - x * a.splits;
-        it.parts = a.splits;
-        it.slot = 0;
-        if (!packed) {
-            const int back = x / a.batch;
-            it.m = per_seq - 1 - back;
-            it.b = x - back * a.batch;
-            if (it.m < 0) return false;
-            seq = load_sequence(a, it.b);
-            return true;
-        }
-    }
-    // First row tile of every sequence.
-    int* first = ints;
-    int tiles;
-    if (packed) {
+    // Row tiles in order, one per thread.
+    int tiles, b = 0, m = 0;
+    if (a.seqstart_q != nullptr) {
         const int per = (a.batch + kTileThreads - 1) / kTileThreads;
         const int b0 = min(a.batch, tid * per), b1 = min(a.batch, b0 + per);
         int mine = 0;
-        for (int b = b0; b < b1; ++b) mine += tile_count(a, load_sequence(a, b));
-        int p = block_scan(mine, sm.scan_a, tiles);
-        if (!a.plan) {
-            const int x = tiles - 1 - y / a.splits;
-            if (x < 0) return false;
-            if (x >= p && x < p + mine)
-                for (int b = b0; b < b1; ++b) {
-                    const int n = tile_count(a, load_sequence(a, b));
-                    if (x < p + n) {
-                        sm.item[0] = b;
-                        sm.item[1] = x - p;
-                        break;
-                    }
-                    p += n;
-                }
-            __syncthreads();
-            it.b = sm.item[0];
-            it.m = sm.item[1];
-            seq = load_sequence(a, it.b);
-            return true;
+        for (int i = b0; i < b1; ++i) mine += tile_count(a, load_sequence(a, i));
+        int at = block_scan(mine, sm.scan, tiles);
+        tiles = min(tiles, kTileThreads);  // more only if the prefix sums overlap
+        for (int i = b0; i < b1 && mine > 0; ++i) {
+            const int c = tile_count(a, load_sequence(a, i));
+            for (int k = 0; k < c && at < tiles; ++k, ++at) sm.tile_of[at] = make_int2(i, k);
         }
+        __syncthreads();
+        if (tid < tiles) b = sm.tile_of[tid].x, m = sm.tile_of[tid].y;
+    } else {
+        const int per_seq = (a.seqlen_q * a.group + kTileM - 1) / kTileM;
+        tiles = a.batch * per_seq;
+        b = tid / per_seq;
+        m = tid - b * per_seq;
+    }
+    Sequence s{0, 0, 0};
+    int n = 0;
+    if (tid < tiles) {
+        s = load_sequence(a, b);
+        n = key_tiles(a, s, m);
+    }
+    long long total;
+    block_scan((long long)n, sm.scan64, total);
+    // The shortest length that may do, or else (jobs round up) one that surely does.
+    const long long all = total * a.nhead_k;
+    const int jobs = tiles * a.nhead_k;
+    long long len = (all + kTileBlocks - 1) / kTileBlocks;
+    int parts, before, sum;
+    for (bool again = false;; again = true) {
+        parts = tid < tiles ? parts_of(n, len) : 0;
+        // Items in the upper half, those of split jobs in the lower.
+        before = block_scan(parts << 16 | (parts > 1 ? parts : 0), sm.scan, sum);
+        if (again || jobs >= kTileBlocks || (sum >> 16) * a.nhead_k <= kTileBlocks) break;
+        len = (all + kTileBlocks - jobs - 1) / (kTileBlocks - jobs);
+    }
+    if ((sum & 0xffff) * a.nhead_k > a.max_slots) return false;  // (overlapping prefix sums)
+    // No job begins in the slots that stay unused.
+    for (int i = (sum & 0xffff) * a.nhead_k + (int)blockIdx.x * kTileThreads + tid; i < a.max_slots;
+         i += (int)gridDim.x * kTileThreads)
+        tile_headers(a)[i].parts = 0;
+    const int x = (sum >> 16) - 1 - y;  // tiles of later tokens (the ones with more keys) first
+    if (x < 0) return false;
+    const int k = x - (before >> 16);
+    if (k >= 0 && k < parts) sm.item = make_item(a, b, s, m, k, parts, parts > 1 ? (before & 0xffff) * a.nhead_k : -1);
+    __syncthreads();
+    it = sm.item;
+    return true;
+}
+
+// The plan for more jobs than that, once for all blocks: writes the list of
+// items and their number, tiles of later tokens first.  Whole tiles, except
+// that what is longer than half a resident block's share is cut into such
+// lengths.  One block; a.tile_first is scratch for batch + 1 integers.
+constexpr int kPlanThreads = 1024;
+__global__ void __launch_bounds__(kPlanThreads, 1)
+fmha_paged_plan(const __grid_constant__ Args a) {
+    __shared__ int scan[kPlanThreads / 32];
+    __shared__ long long scan64[kPlanThreads / 32];
+    griddep_launch_dependents();
+    const int tid = threadIdx.x;
+    const bool packed = a.seqstart_q != nullptr;
+    const int per_seq = packed ? 1 : (a.seqlen_q * a.group + kTileM - 1) / kTileM;
+    int* first = a.tile_first;
+    int tiles = a.batch * per_seq;
+    if (packed) {
+        const int per = (a.batch + kPlanThreads - 1) / kPlanThreads;
+        const int b0 = min(a.batch, tid * per), b1 = min(a.batch, b0 + per);
+        int mine = 0;
+        for (int b = b0; b < b1; ++b) mine += tile_count(a, load_sequence(a, b));
+        int at = block_scan(mine, scan, tiles);
         for (int b = b0; b < b1; ++b) {
-            first[b] = p;
-            p += tile_count(a, load_sequence(a, b));
+            first[b] = at;
+            at += tile_count(a, load_sequence(a, b));
         }
         if (tid == 0) first[a.batch] = tiles;
         __syncthreads();
-    } else {
-        tiles = a.batch * per_seq;
     }
-    tiles = min(tiles, kMaxPlanned);  // more only if the prefix sums overlap
-    // Key tiles of this thread's row tiles t0 .. t1-1, and the range length.
-    int* keys = ints + kMaxPlanned + 1;
-    const int per = (tiles + kTileThreads - 1) / kTileThreads;
+    tiles = min(tiles, a.max_tiles);  // more only if the prefix sums overlap
+    const int per = (tiles + kPlanThreads - 1) / kPlanThreads;
     const int t0 = min(tiles, tid * per), t1 = min(tiles, t0 + per);
     int b_first = 0, m_first = 0;
     if (packed) {
@@ -229,85 +281,42 @@ __device__ __forceinline__ bool find_item(const Args& a, TileShared& sm, int* in
         b_first = t0 / per_seq;
         m_first = t0 - b_first * per_seq;
     }
-    // The next row tile after (b, m); empty sequences are passed over.
-    auto next_tile = [&](int& b, int& m, int t) {
-        ++m;
-        if (packed)
-            while (b + 1 < a.batch && first[b + 1] <= t) ++b, m = 0;
-        else if (m == per_seq)
-            ++b, m = 0;
-    };
-    int mine = 0, total;
-    {
+    // f(b, sequence, m) for the thread's row tiles.
+    auto each_tile = [&](auto f) {
         int b = b_first, m = m_first, have = -1;
         Sequence s{0, 0, 0};
         for (int t = t0; t < t1; ++t) {
             if (b != have) s = load_sequence(a, have = b);
-            const int n = max(1, (tile_kv_end(a, s, m) + kTileN - 1) / kTileN);
-            keys[t] = n;
-            mine += min(n, kMostCounted);
-            next_tile(b, m, t + 1);
+            f(b, s, m);
+            ++m;
+            if (packed)
+                while (b + 1 < a.batch && first[b + 1] <= t + 1) ++b, m = 0;
+            else if (m == per_seq)
+                ++b, m = 0;
         }
-    }
-    block_scan(mine, sm.scan_a, total);
-    // The range length.  Fewer jobs than resident blocks: the ranges that fill
-    // the device once; the shortest length that may do, or else (jobs round up)
-    // the one that surely does.  More jobs: cut only what is longer than half a
-    // block's share.
-    const long long all = (long long)total * a.nhead_k;
-    const int jobs = tiles * a.nhead_k;
-    long long len = (all + kTileBlocks - 1) / kTileBlocks;
-    if (jobs >= kTileBlocks) len = max((long long)kLongRange, (all + 2 * kTileBlocks - 1) / (2 * kTileBlocks));
-    int both, before, sum;
-    unsigned most;
-    auto parts_of = [&](int n) { return (int)min(((unsigned)min(n, kMostCounted) + most - 1) / most, kMostParts); };
-    for (bool again = false;; again = true) {
-        most = (unsigned)min(max(len, 1ll), 0x7fffffffll);
-        both = 0;  // items in the upper half, those of split jobs in the lower
-        for (int t = t0; t < t1; ++t) {
-            const int p = parts_of(keys[t]);
-            both += p << 16 | (p > 1 ? p : 0);
+    };
+    long long mine = 0, total;
+    each_tile([&](int, const Sequence& s, int m) { mine += key_tiles(a, s, m); });
+    block_scan(mine, scan64, total);
+    const long long len = max((long long)kLongRange, (total * a.nhead_k + 2 * kTileBlocks - 1) / (2 * kTileBlocks));
+    long long both = 0, sum;  // items in the upper half, those of split jobs in the lower
+    each_tile([&](int, const Sequence& s, int m) {
+        const int p = parts_of(key_tiles(a, s, m), len);
+        both += (long long)p << 32 | (p > 1 ? p : 0);
+    });
+    const long long before = block_scan(both, scan64, sum);
+    const int items = (int)(sum >> 32), split = (int)sum;
+    int at = (int)(before >> 32), slot = (int)before;
+    each_tile([&](int b, const Sequence& s, int m) {
+        const int p = parts_of(key_tiles(a, s, m), len);
+        for (int k = 0; k < p; ++k, ++at) {
+            const int x = items - 1 - at;
+            if (x >= 0 && x < a.max_items) a.items[x] = make_item(a, b, s, m, k, p, p > 1 ? slot * a.nhead_k : -1);
         }
-        before = block_scan(both, sm.scan_b, sum);
-        if (again || jobs >= kTileBlocks || (sum >> 16) * a.nhead_k <= kTileBlocks) break;
-        len = (all + kTileBlocks - jobs - 1) / (kTileBlocks - jobs);
-        __syncthreads();  // scan_b is written again
-    }
-    const int split = sum & 0xffff;
-    // No job begins in the slots that stay unused.
-    for (int i = split * a.nhead_k + (int)blockIdx.x * kTileThreads + tid; i < a.max_slots;
-         i += (int)gridDim.x * kTileThreads)
-        tile_headers(a)[i].parts = 0;
-    const int x = (sum >> 16) - 1 - y;
-    if (x < 0) return false;
-    int items_before = before >> 16, split_before = before & 0xffff;
-    if (x >= items_before && x < items_before + (both >> 16)) {
-        int b = b_first, m = m_first;
-        for (int t = t0; t < t1; ++t) {
-            const int p = parts_of(keys[t]);
-            if (x < items_before + p) {
-                const Sequence s = load_sequence(a, b);
-                sm.item[0] = b;
-                sm.item[1] = m;
-                sm.item[2] = x - items_before;
-                sm.item[3] = p;
-                sm.item[4] = split_before * a.nhead_k;
-                sm.item[5] = s.first;
-                sm.item[6] = s.count;
-                sm.item[7] = s.keys;
-                break;
-            }
-            items_before += p;
-            if (p > 1) split_before += p;
-            next_tile(b, m, t + 1);
-        }
-    }
-    // The ring goes to the copies next: what was written there comes before them.
-    asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-    __syncthreads();
-    it = Item{sm.item[0], sm.item[1], sm.item[2], sm.item[3], sm.item[4]};
-    seq = Sequence{sm.item[5], sm.item[6], sm.item[7]};
-    return true;
+        if (p > 1) slot += p;
+    });
+    if (tid == 0) *a.item_count = split * a.nhead_k <= a.max_slots ? min(items, a.max_items) : 0;
+    for (int i = split * a.nhead_k + tid; i < a.max_slots; i += kPlanThreads) tile_headers(a)[i].parts = 0;
 }
 
 __global__ void __launch_bounds__(kTileThreads, 2)
@@ -318,31 +327,33 @@ fmha_paged_tile_kernel(const __grid_constant__ Args a) {
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     volatile int* abort_flag = &sm.abort_flag;
 
+    // Neighbouring blocks take the heads of one key range: they read
+    // neighbouring lines of memory at the same time.
+    const int kvh = blockIdx.x % a.nhead_k, y = blockIdx.x / a.nhead_k;
+    TileItem it;
+    if (a.plan == kPlanNone) {
+        // One sequence, every tile cut as the host said.
+        const int m = y / a.splits;
+        it = make_item(a, 0, load_sequence(a, 0), m, y - m * a.splits, a.splits, -1);
+    } else if (a.plan == kPlanHere) {
+        if (!plan_here(a, sm, y, it)) return;
+    } else {
+        griddep_wait();  // for the list
+        if (y >= *a.item_count) return;
+        it = a.items[y];
+    }
     // What follows on the stream may be scheduled as soon as this grid's last
     // blocks run; it waits for their results where it needs them.
     griddep_launch_dependents();
 
-    // Neighbouring blocks take the heads of one key range: they read
-    // neighbouring lines of memory at the same time.
-    const int kvh = blockIdx.x % a.nhead_k;
-    Item it;
-    Sequence seq;
-    if (!find_item(a, sm, reinterpret_cast<int*>(sm.kv[0]), blockIdx.x / a.nhead_k, it, seq)) return;
-    const int rows = seq.count * a.group;
-    const int row0 = it.m * kTileM;
-    if (rows < a.min_rows || rows > a.max_rows || row0 >= rows) return;
-    const int row_end = min(rows, row0 + kTileM);
-    const int kv_end = tile_kv_end(a, seq, it.m);
-    const int all = (kv_end + kTileN - 1) / kTileN;
-    const int each = all / it.parts, more = all - each * it.parts;
-    const int j0 = it.k * each + min(it.k, more);
-    const int n = each + (it.k < more);
-    const bool shared_job = a.plan && it.parts > 1;  // through a scratch slot
+    const Sequence seq{it.first, it.count, it.keys};
+    const int row0 = it.row0, row_end = it.row_end, kv_end = it.kv_end, j0 = it.j0, n = it.n;
+    const bool shared_job = it.slot >= 0;  // through scratch slots
     const int slot_job = it.slot + it.k * a.nhead_k + kvh;
-    if (shared_job && it.k == 0 && threadIdx.x == 0)
-        tile_headers(a)[slot_job] = TileHeader{seq.first, row0, row_end - row0, kvh, it.parts, {0, 0, 0}};
-    else if (shared_job && threadIdx.x == 0)
-        tile_headers(a)[slot_job].parts = 0;
+    if (shared_job && threadIdx.x == 0) {
+        if (it.k == 0) tile_headers(a)[slot_job] = TileHeader{seq.first, row0, row_end - row0, kvh, it.parts, {0, 0, 0}};
+        else tile_headers(a)[slot_job].parts = 0;
+    }
     const int tail = kv_end - (j0 + n - 1) * kTileN;  // visible keys of the range's last tile
     const bool has_tail = n > 0 && tail < kTileN;
     const int active = (row_end - row0 + 31) / 32;    // softmax warps with rows

@@ -240,7 +240,7 @@ __device__ __forceinline__ bool plan_here(const Args& a, TileShared& sm, int y, 
 // items and their number, tiles of later tokens first.  Whole tiles, except
 // that what is longer than half a resident block's share is cut into such
 // lengths.  One block; a.tile_first is scratch for batch + 1 integers.
-constexpr int kPlanThreads = 1024;
+constexpr int kPlanThreads = 256;
 __global__ void __launch_bounds__(kPlanThreads, 1)
 fmha_paged_plan(const __grid_constant__ Args a) {
     __shared__ int scan[kPlanThreads / 32];

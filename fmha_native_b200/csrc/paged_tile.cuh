@@ -327,6 +327,19 @@ fmha_paged_tile_kernel(const __grid_constant__ Args a) {
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     volatile int* abort_flag = &sm.abort_flag;
 
+    // Tensor memory first: the SM's second block does not start before the first
+    // has given the permit to allocate back (2-3 us later, if that waits for the
+    // block's work to be known).
+    if (warp == kWarpMma) {
+        tmem_alloc(smem_u32(&sm.tmem_base), kTileTmemCols);
+        tmem_relinquish();
+    }
+    auto leave = [&]() {  // a block without work
+        tc_fence_before();
+        __syncthreads();
+        tc_fence_after();
+        if (warp == kWarpMma) tmem_dealloc(sm.tmem_base, kTileTmemCols);
+    };
     // Neighbouring blocks take the heads of one key range: they read
     // neighbouring lines of memory at the same time.
     const int kvh = blockIdx.x % a.nhead_k, y = blockIdx.x / a.nhead_k;
@@ -336,10 +349,10 @@ fmha_paged_tile_kernel(const __grid_constant__ Args a) {
         const int m = y / a.splits;
         it = make_item(a, 0, load_sequence(a, 0), m, y - m * a.splits, a.splits, -1);
     } else if (a.plan == kPlanHere) {
-        if (!plan_here(a, sm, y, it)) return;
+        if (!plan_here(a, sm, y, it)) return leave();
     } else {
         griddep_wait();  // for the list
-        if (y >= *a.item_count) return;
+        if (y >= *a.item_count) return leave();
         it = a.items[y];
     }
     // What follows on the stream may be scheduled as soon as this grid's last
@@ -392,8 +405,8 @@ fmha_paged_tile_kernel(const __grid_constant__ Args a) {
     constexpr int kAhead = kTileStages / 2;  // tiles loaded before the block starts
     int page = 0;
 
-    // Start, the roles side by side: barriers and the first copies, tensor
-    // memory, and Q (its 16-byte chunks swizzled by row mod 8).
+    // Start, the roles side by side: barriers and the first copies, and Q (its
+    // 16-byte chunks swizzled by row mod 8).
     if (warp == kWarpLoad) {
         page = page_of(0);
         if (lane == 0) {
@@ -416,9 +429,6 @@ fmha_paged_tile_kernel(const __grid_constant__ Args a) {
             issue_load(2 * j + 1, page);
             page = next;
         }
-    } else if (warp == kWarpMma) {
-        tmem_alloc(smem_u32(&sm.tmem_base), kTileTmemCols);
-        tmem_relinquish();
     } else if (warp < kSoftmaxWarps && n > 0) {
         uint4 x[4];
         const uint4* src = has_row ? reinterpret_cast<const uint4*>(q_row(a, token, head)) + half * 4 : nullptr;

@@ -23,6 +23,7 @@ static_assert(sizeof(RowsShared) + 1024 <= 227 * 1024, "shared memory of a block
 static_assert(2 * (sizeof(TileShared) + 2048) <= 228 * 1024, "two tile blocks per SM");
 
 bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
+bool aligned4(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 3u) == 0; }
 
 // A stride of a dimension of one element is never used.
 bool stride_ok(long long s, long long extent) {
@@ -86,7 +87,7 @@ bool make_plan(int batch, int seqlen_q, int total_q, bool packed, int nhead_q, i
     z.tokens = packed ? total_q : (long long)batch * seqlen_q;
     z.group = nhead_q / nhead_k;
     const long long max_rows = (long long)(packed ? std::min(seqlen_q, total_q) : seqlen_q) * z.group;
-    if (z.tokens * nhead_q > INT_MAX || nhead_q > 65535 || (z.tokens > 0 && max_rows == 0)) return false;
+    if (z.tokens * nhead_q > INT_MAX || nhead_q > 8192 || prefix_len > kMostKeys || (z.tokens > 0 && max_rows == 0)) return false;
     z.max_rows = (int)max_rows;
     z.tile = max_rows > kMostRows;
     z.rows = packed || !z.tile;
@@ -150,6 +151,9 @@ int check(const FmhaPagedParams* p, bool prefix, Plan& z) {
                   prefix ? p->prefix_len : 0, z))
         return FMHA_ERR_ARG;
     if (!aligned16(p->q) || !aligned16(p->k_cache) || !aligned16(p->v_cache) || !aligned16(p->o))
+        return FMHA_ERR_ARG;
+    if (!aligned4(p->lse) || !aligned4(p->page_table) || !aligned4(p->seqlens_k) || !aligned4(p->seqstart_q) ||
+        !aligned4(p->prefix_pages))
         return FMHA_ERR_ARG;
     const int shift = log2_exact(p->page_size);
     if (shift < 3 || shift > 12 || p->num_pages < 0 || p->max_pages < 0 || p->table_stride < 0)

@@ -262,6 +262,9 @@ int check(const FmhaRopeParams* p, bool append, RopeArgs& a) {
     const long long batch = packed ? 1 : p->batch;
     const long long tokens = rows * batch;
     if (tokens > 0x7fffffffll) return FMHA_ERR_ARG;
+    for (const void* i : {(const void*)p->positions, (const void*)p->seqstart_q, (const void*)p->page_table,
+                          (const void*)p->seqlens_k})
+        if ((reinterpret_cast<uintptr_t>(i) & 3u) != 0) return FMHA_ERR_ARG;
     if (p->q != nullptr) {
         if (p->nhead_q <= 0 || p->q_out == nullptr || !aligned16(p->q) || !aligned16(p->q_out) ||
             !stride_ok(p->stride_q, rows, false) || !stride_ok(p->nhead_stride_q, p->nhead_q, false) ||

@@ -16,6 +16,7 @@ using namespace fmha_sm100;
 
 constexpr int kHeadDim = 64;
 constexpr float kLn2 = 0.69314718055994531f;
+constexpr int kMostKeys = 0x7fffffff - 4096;  // of a sequence: places are counted in 32 bits, tiles past them too
 
 // Rows.  The new tokens of a call are numbered f = 0 .. tokens-1 (dense:
 // batch * seqlen_q + index; packed: the packed index).  For one K/V head the
@@ -100,7 +101,7 @@ __device__ __forceinline__ Sequence load_sequence(const Args& a, int b) {
     }
     if (a.seqlens_k != nullptr) {
         s.keys = max(a.seqlens_k[b], 0);
-        const long long cap = (long long)a.max_pages << a.page_shift;
+        const long long cap = min((long long)a.max_pages << a.page_shift, (long long)kMostKeys);
         if (s.keys > cap) {
             flag_index_error(a.err_word);
             s.keys = (int)cap;

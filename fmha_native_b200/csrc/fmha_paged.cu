@@ -112,7 +112,7 @@ bool make_plan(int batch, int seqlen_q, int total_q, bool packed, int nhead_q, i
         z.prefix_splits = pick_splits(std::max(1ll, z.prefix_tiles * nhead_k), (prefix_len + kTileN - 1) / kTileN);
         z.part = (size_t)z.tokens * nhead_q * (kHeadDim + 1) * sizeof(float);
         z.parts = z.prefix_splits + (z.rows ? 1 : 0);
-        z.info = round16(batch * sizeof(int2));
+        z.info = round16((batch + 1ll) * sizeof(int2));
     }
     z.total = z.pieces + z.slots + z.list + z.info + z.part * z.parts;
     return true;

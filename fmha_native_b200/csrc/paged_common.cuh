@@ -68,8 +68,8 @@ struct Args {
     float* slots;               // scratch of the jobs that blocks share
     int max_slots;
     float* pieces;              // rows kernel: scratch between its blocks
-    int2* seq_parts;            // rows kernel under a prefix: per sequence its first block and, if
-                                // it crosses blocks, how many share it
+    int2* seq_parts;            // rows kernel under a prefix: per sequence its first block and, if it
+                                // crosses blocks, how many share it; last, its groups of blocks
     int* err_word;
     unsigned long long wait_limit_ns;
 };

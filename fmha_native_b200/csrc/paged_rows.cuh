@@ -45,7 +45,9 @@ constexpr int kMaxRowBlocks = 148;    // one block per SM
 constexpr int kMostRows = 16;         // rows of a K/V head that a warp holds
 constexpr int kRowStages = 3;
 // A sequence's start and end in a block cost about as much time as this many
-// units (its first loads, Q, the results); the shares count them.
+// units (its first loads, Q, the results).  The shares count them once there is
+// more than a unit or two per block (64 sequences of 100 to 4095 keys: 42 us
+// with, 48 without).
 constexpr int kSeqCost = 5;
 
 // A sequence as this kernel takes it.
@@ -53,7 +55,6 @@ struct RowSeq {
     int first, count, keys;
     int kv_end;      // keys that any of its rows sees
     int units;       // 0: not ours; a sequence that sees no key counts one (empty) unit
-    __device__ int cost() const { return units > 0 ? units + kSeqCost : 0; }
 };
 // A (sequence, head) result of a block: where it goes.
 struct Target {
@@ -71,7 +72,7 @@ struct alignas(1024) RowsShared {
     uint64_t bar[kRowWarps][kRowStages];
     Target piece_to[kRowWarps][2];
     int piece_job[kRowWarps][2];      // segment of the block * heads + head, -1: none
-    int scan[kRowWarps];
+    int2 scan[kRowWarps];
     int run[2 * kRowWarps + 1];
     RowSeq start_seq;                 // of the block's first segment
     int start_b, start_x;
@@ -84,7 +85,8 @@ struct alignas(1024) RowsShared {
 struct RowsHeader {
     int first, rows;  // a sequence that begins in this block and goes on: its first token, rows
     int parts;        // blocks that share it; 0: none
-    int pad;
+    int h0, heads;    // the block's K/V heads
+    int pad[3];
 };
 __host__ __device__ constexpr size_t rows_scratch_bytes(long long rows) {
     return kMaxRowBlocks * (2 * (size_t)rows * (kHeadDim + 2) * sizeof(float) + sizeof(RowsHeader));
@@ -193,44 +195,78 @@ fmha_paged_rows_kernel(const __grid_constant__ Args a) {
     // ------------------------------------------------- the block's range
     const int per = (a.batch + kRowThreadsTotal - 1) / kRowThreadsTotal;
     const int b0 = min(a.batch, (int)threadIdx.x * per), b1 = min(a.batch, b0 + per);
-    int mine = 0;
-    for (int b = b0; b < b1; ++b) mine += load_row_seq(a, b).cost();
+    int mine = 0, mine_n = 0;  // units; sequences
+    for (int b = b0; b < b1; ++b) {
+        const int n = load_row_seq(a, b).units;
+        mine += n;
+        mine_n += n > 0;
+    }
     int incl = mine;
 #pragma unroll
     for (int d = 1; d < 32; d <<= 1) {
         const int v = __shfl_up_sync(0xffffffffu, incl, d);
         if (lane >= d) incl += v;
     }
-    if (lane == 31) sm.scan[warp] = incl;
+    int incl_n;
+    if (per == 1) {
+        incl_n = __popc(__ballot_sync(0xffffffffu, mine_n > 0) & (0xffffffffu >> (31 - lane)));
+    } else {
+        incl_n = mine_n;
+#pragma unroll
+        for (int d = 1; d < 32; d <<= 1) {
+            const int v = __shfl_up_sync(0xffffffffu, incl_n, d);
+            if (lane >= d) incl_n += v;
+        }
+    }
+    if (lane == 31) sm.scan[warp] = make_int2(incl, incl_n);
     __syncthreads();
-    unsigned before = incl - mine, total = 0;
+    unsigned before = incl - mine, before_n = incl_n - mine_n, total = 0, total_n = 0;
 #pragma unroll
     for (int w = 0; w < kRowWarps; ++w) {
-        if (w < warp) before += sm.scan[w];
-        total += sm.scan[w];
+        const int2 v = sm.scan[w];
+        if (w < warp) before += v.x, before_n += v.y;
+        total += v.x;
+        total_n += v.y;
     }
+    const int seq_cost = total > 2 * kMaxRowBlocks ? kSeqCost : 0;
+    auto cost_of = [&](int n) { return n > 0 ? n + seq_cost : 0; };
+    // Few units: groups of blocks share out the heads, too, at least 8 a block.
+    int groups = 1, group_blocks = gridDim.x, group = 0, index = blockIdx.x, head0 = 0, heads = a.nhead_k;
+    if (heads > kRowWarps && total > 0 && 2 * total <= gridDim.x) {
+        groups = min((heads + kRowWarps - 1) / kRowWarps, (int)(gridDim.x / total));
+        group_blocks = (int)gridDim.x / groups;
+        group = (int)blockIdx.x / group_blocks;
+        index = (int)blockIdx.x - group * group_blocks;
+        head0 = a.nhead_k * group / groups;
+        heads = a.nhead_k * (group + 1) / groups - head0;
+    }
+    const unsigned cost_mine = mine + mine_n * seq_cost;
+    before += before_n * seq_cost;
+    total += total_n * seq_cost;
     // As many blocks as give every warp a unit of some head.
-    const unsigned want = (unsigned)min(((unsigned long long)total * a.nhead_k + kRowWarps - 1) / kRowWarps,
+    const unsigned want = (unsigned)min(((unsigned long long)total * heads + kRowWarps - 1) / kRowWarps,
                                         (unsigned long long)total);
-    const unsigned blocks = min(gridDim.x, want);
-    if (blockIdx.x >= blocks) {
+    const unsigned blocks = min((unsigned)group_blocks, want);
+    if (a.seq_parts != nullptr && blockIdx.x == 0 && threadIdx.x == 0)
+        a.seq_parts[a.batch] = make_int2(groups, group_blocks);
+    if (group >= groups || index >= blocks) {
         griddep_wait();  // the grid ends after the launch before it
         if (threadIdx.x == 0) piece_headers(a)[blockIdx.x].parts = 0;
         return;
     }
     const Ranges ranges(total, blocks);
-    const unsigned beg = ranges.begin(blockIdx.x), end = ranges.begin(blockIdx.x + 1);
-    if (beg >= before && beg < before + mine) {
+    const unsigned beg = ranges.begin(index), end = ranges.begin(index + 1);
+    if (beg >= before && beg < before + cost_mine) {
         unsigned p = before;
         for (int b = b0; b < b1; ++b) {
             const RowSeq x = load_row_seq(a, b);
-            const unsigned n = x.cost();
+            const unsigned n = cost_of(x.units);
             if (beg < p + n) {
                 sm.start_b = b;
                 sm.start_x = (int)(beg - p);
                 sm.start_seq = x;
                 // The first page ids that the block will want.
-                const int page0 = (max(0, (int)(beg - p) - kSeqCost) * kUnit) >> a.page_shift;
+                const int page0 = (max(0, (int)(beg - p) - seq_cost) * kUnit) >> a.page_shift;
                 const int32_t* ids = a.page_table + b * a.table_stride + page0;
                 if (page0 < a.max_pages) prefetch_l1(ids);
                 if (page0 + 32 < a.max_pages) prefetch_l1(ids + 32);
@@ -243,7 +279,7 @@ fmha_paged_rows_kernel(const __grid_constant__ Args a) {
 
     // ------------------------------------------------------- the share
     // A place on the block's line: segment (a sequence's units [unit0, unit0 +
-    // n) in this block), head, unit.  Two cursors: `p` issues loads, `c` computes.
+    // n) in this block), head (of the block's), unit.  Two cursors: `p` issues loads, `c` computes.
     struct Cursor {
         RowSeq x;
         int b, seg;
@@ -252,9 +288,9 @@ fmha_paged_rows_kernel(const __grid_constant__ Args a) {
     };
     // Sets the segment of sequence k.b that starts `off` into the sequence's cost.
     auto set_segment = [&](Cursor& k, int off) {
-        k.cost = min(k.x.cost() - off, k.left);
-        k.unit0 = max(0, off - kSeqCost);
-        k.n = max(0, off + k.cost - kSeqCost) - k.unit0;
+        k.cost = min(cost_of(k.x.units) - off, k.left);
+        k.unit0 = max(0, off - seq_cost);
+        k.n = max(0, off + k.cost - seq_cost) - k.unit0;
     };
     auto next_segment = [&](Cursor& k) {
         do {
@@ -273,7 +309,7 @@ fmha_paged_rows_kernel(const __grid_constant__ Args a) {
     auto advance = [&](Cursor& k) {
         if (++k.u < k.n) return;
         k.u = 0;
-        if (++k.h < a.nhead_k) return;
+        if (++k.h < heads) return;
         k.h = 0;
         next_segment(k);
     };
@@ -289,14 +325,14 @@ fmha_paged_rows_kernel(const __grid_constant__ Args a) {
     unsigned long long tiles = 0;  // of the block: units x heads
     {
         Cursor k = c;
-        for (bool more = any; more; more = next_segment(k)) tiles += (unsigned long long)k.n * a.nhead_k;
+        for (bool more = any; more; more = next_segment(k)) tiles += (unsigned long long)k.n * heads;
     }
     const unsigned long long from = tiles * warp / kRowWarps;
     const long long count = (long long)(tiles * (warp + 1) / kRowWarps - from);
     if (count > 0) {
         unsigned long long x = from;
-        while (x >= (unsigned long long)c.n * a.nhead_k) {
-            x -= (unsigned long long)c.n * a.nhead_k;
+        while (x >= (unsigned long long)c.n * heads) {
+            x -= (unsigned long long)c.n * heads;
             if (!next_segment(c)) break;
         }
         if (c.n > 0) {
@@ -347,8 +383,8 @@ fmha_paged_rows_kernel(const __grid_constant__ Args a) {
                         const uint32_t dst = ring0 + fill * (2 * kUnitBytes) + (box << (box_shift + 7));
                         if (leader) {
                             if ((unsigned)id >= (unsigned)a.num_pages) flag_index_error(a.err_word);
-                            load_page_box(dst, &a.tm_k, bar, key0 & page_mask, p.h, id, policy);
-                            load_page_box(dst + kUnitBytes, &a.tm_v, bar, key0 & page_mask, p.h, id, policy);
+                            load_page_box(dst, &a.tm_k, bar, key0 & page_mask, head0 + p.h, id, policy);
+                            load_page_box(dst + kUnitBytes, &a.tm_v, bar, key0 & page_mask, head0 + p.h, id, policy);
                         }
                     }
                     ++issued;
@@ -361,7 +397,7 @@ fmha_paged_rows_kernel(const __grid_constant__ Args a) {
                     // one's page ids, will be wanted without delay.
                     if (lane < p.x.count * a.group) {
                         const int t = lane / a.group;
-                        prefetch_l1(q_row(a, p.x.first + t, p.h * a.group + lane - t * a.group));
+                        prefetch_l1(q_row(a, p.x.first + t, (head0 + p.h) * a.group + lane - t * a.group));
                     }
                     if (p.h == 0 && lane == 31 && p.b + 1 < a.batch)
                         prefetch_l1(a.page_table + (p.b + 1) * a.table_stride);
@@ -391,7 +427,7 @@ fmha_paged_rows_kernel(const __grid_constant__ Args a) {
                         const int t = r / a.group;
                         lim[hr] = key_limit(a, Sequence{c.x.first, c.x.count, c.x.keys}, t);
                         src = reinterpret_cast<const uint32_t*>(
-                            q_row(a, c.x.first + t, c.h * a.group + r - t * a.group));
+                            q_row(a, c.x.first + t, (head0 + c.h) * a.group + r - t * a.group));
                     }
 #pragma unroll
                     for (int kk = 0; kk < 4; ++kk) {
@@ -511,7 +547,7 @@ fmha_paged_rows_kernel(const __grid_constant__ Args a) {
                 float* po = all ? reinterpret_cast<float*>(sm.ring[warp][(done + kRowStages - 1) % kRowStages])
                           : last ? reinterpret_cast<float*>(sm.ring[warp]) : sm.first_o[warp];
                 float* pml = all || last ? po + kMostRows * kHeadDim : sm.first_ml[warp];
-                const Target to{c.x.first, rows, c.h,
+                const Target to{c.x.first, rows, head0 + c.h,
                                 c.unit0 == 0 && c.n == c.x.units ? -1 : 2 * (int)blockIdx.x + (c.unit0 == 0)};
                 if (!empty) {
 #pragma unroll
@@ -543,7 +579,7 @@ fmha_paged_rows_kernel(const __grid_constant__ Args a) {
                     __syncwarp();
                 } else if (lane == 0) {
                     sm.piece_to[warp][last] = to;
-                    sm.piece_job[warp][last] = c.seg * a.nhead_k + c.h;
+                    sm.piece_job[warp][last] = c.seg * heads + c.h;
                 }
             }
             produce();
@@ -555,7 +591,7 @@ fmha_paged_rows_kernel(const __grid_constant__ Args a) {
     }
 
     // What the block has to say of the sequences that begin in it.
-    RowsHeader header{0, 0, 0, 0};
+    RowsHeader header{0, 0, 0, head0, heads, {0, 0, 0}};
     if (threadIdx.x == 0) {
         Cursor k = c0;
         for (bool more = any; more; more = next_segment(k)) {
@@ -563,12 +599,12 @@ fmha_paged_rows_kernel(const __grid_constant__ Args a) {
             int parts = 0;
             if (k.n < k.x.units) {
                 // Only a last segment goes on; its cost ends that far past the block's.
-                parts = (int)(ranges.owner(end + (k.x.units - k.n) - 1) - blockIdx.x) + 1;
+                parts = (int)ranges.owner(end + (k.x.units - k.n) - 1) - index + 1;
                 header.first = k.x.first;
                 header.rows = k.x.count * a.group;
                 header.parts = parts;
             }
-            if (a.seq_parts != nullptr) a.seq_parts[k.b] = make_int2(blockIdx.x, parts);
+            if (a.seq_parts != nullptr && group == 0) a.seq_parts[k.b] = make_int2(index, parts);
         }
     }
 
@@ -621,8 +657,8 @@ fmha_paged_rows_merge(const __grid_constant__ Args a) {
     if (hd.parts == 0) return;
     const int rows = hd.rows;
     const int y = blockIdx.y * 4 + (int)(threadIdx.x >> 6);
-    const bool has_row = y < rows * a.nhead_k;
-    const int h = has_row ? y / rows : 0, rt = has_row ? y - h * rows : 0;
+    const bool has_row = y < rows * hd.heads;
+    const int h = has_row ? hd.h0 + y / rows : 0, rt = has_row ? y - y / rows * rows : 0;
     const int lane = threadIdx.x & 31, c4 = lane & 15;
     float m = -INFINITY, l = 0.0f;
     float4 o = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
@@ -687,7 +723,9 @@ fmha_prefix_finish(const __grid_constant__ Args a) {
            rt < a.row_cap;  // (past the cap: more tokens than the call said)
     griddep_wait();  // every thread: the grid ends after the launches before it
     if (!mine) return;
-    const int2 parts = a.seq_parts[b];  // its first block, and how many share it
+    int2 parts = a.seq_parts[b];  // its first block (of each group of heads), and how many share it
+    const int2 groups = a.seq_parts[a.batch];  // and the groups, and their blocks
+    parts.x += ((h + 1) * groups.x - 1) / a.nhead_k * groups.y;
     float m = -INFINITY, l = 0.0f;
     float4 o = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
     // The prefix's parts and the sequence's own, if one (what is read there

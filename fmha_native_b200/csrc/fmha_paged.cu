@@ -253,7 +253,7 @@ int launch_rows(const Args& a, const Args* finish, bool after, int device, cudaS
                             a);
 }
 
-// `ranges`: key ranges of row tiles; after: right behind the kernel that lists them.
+// `ranges`: key ranges of row tiles; after: it follows another kernel of the call.
 int launch_tile(const Args& a, long long ranges, bool after, int device, cudaStream_t stream) {
     constexpr size_t smem = sizeof(TileShared) + 1024;
     static std::atomic<unsigned long long> ready{0};
@@ -317,7 +317,7 @@ int run(const FmhaPagedParams* p, bool prefix, cudaStream_t stream) {
         }
         if (z.tile) {
             t.plan = z.plan;
-            st = launch_tile(t, z.ranges, z.plan == kPlanList && !prefix, ctx.device, stream);
+            st = launch_tile(t, z.ranges, z.plan == kPlanList || prefix, ctx.device, stream);
             if (st != FMHA_OK) return st;
         }
     }

@@ -335,6 +335,7 @@ fmha_paged_tile_kernel(const __grid_constant__ Args a) {
         tmem_relinquish();
     }
     auto leave = [&]() {  // a block without work
+        griddep_wait();   // (the grid ends after the launch before it)
         tc_fence_before();
         __syncthreads();
         tc_fence_after();
@@ -662,6 +663,7 @@ fmha_paged_tile_kernel(const __grid_constant__ Args a) {
                 const bool got = wait_phase(smem_u32(&sm.bar_pv), (n - 1) & 1, abort_flag, a);
                 ok = __all_sync(0xffffffffu, got);
             }
+            griddep_wait();  // a prefix's results may come from the launch before
             // The row's sum, from both halves.
             sm.half_sum[half][t] = l_run;
             if (bar_or(pair_bar, 64, !ok)) ok = false;

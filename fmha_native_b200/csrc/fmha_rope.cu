@@ -147,30 +147,43 @@ fmha_rope_d64_kernel(const __grid_constant__ RopeArgs a) {
             const int j0 = part * 8 + half * 4;
             const unsigned axes = a.axes4[part * 2 + half];
             const bool given = !kAppend || p.positions != nullptr;
-            const bool same = !given || axes == (axes & 3) * 0x55u;  // one axis turns the four pairs
-            int pos[4];
-            pos[0] = given ? p.positions[(axes & 3) * p.axis_stride + tok] : place;
-#pragma unroll
-            for (int e = 1; e < 4; ++e)
-                pos[e] = same ? pos[0] : p.positions[((axes >> (2 * e)) & 3) * p.axis_stride + tok];
-#pragma unroll
-            for (int e = 0; e < 4; ++e)
-                if ((unsigned)pos[e] >= (unsigned)p.max_pos) angle = false;
-            if (angle && same) {
-                const float* row = p.cos_sin + (long long)pos[0] * (2 * n) + j0;
-                const float4 c = *reinterpret_cast<const float4*>(row);
-                const float4 s = *reinterpret_cast<const float4*>(row + n);
-                cs[half * 4 + 0] = c.x, cs[half * 4 + 1] = c.y, cs[half * 4 + 2] = c.z, cs[half * 4 + 3] = c.w;
-                sn[half * 4 + 0] = s.x * sign, sn[half * 4 + 1] = s.y * sign;
-                sn[half * 4 + 2] = s.z * sign, sn[half * 4 + 3] = s.w * sign;
-            } else if (angle) {
-#pragma unroll
-                for (int e = 0; e < 4; ++e) {
-                    const float* row = p.cos_sin + (long long)pos[e] * (2 * n) + j0 + e;
-                    cs[half * 4 + e] = row[0];
-                    sn[half * 4 + e] = row[n] * sign;
+            // At most two axes turn the four pairs, unless axes alternate pair by
+            // pair: those of the first and of the last.
+            const unsigned ax0 = axes & 3, ax3 = axes >> 6, ax1 = (axes >> 2) & 3, ax2 = (axes >> 4) & 3;
+            const bool two = (ax1 == ax0 || ax1 == ax3) && (ax2 == ax0 || ax2 == ax3);
+            const int pos0 = given ? p.positions[ax0 * p.axis_stride + tok] : place;
+            int pos3 = pos0;
+            if (given && ax3 != ax0) pos3 = p.positions[ax3 * p.axis_stride + tok];
+            angle = angle && (unsigned)pos0 < (unsigned)p.max_pos && (unsigned)pos3 < (unsigned)p.max_pos;
+            float4 c, s;
+            if (angle) {
+                const float* row = p.cos_sin + (long long)pos0 * (2 * n) + j0;
+                c = *reinterpret_cast<const float4*>(row);
+                s = *reinterpret_cast<const float4*>(row + n);
+            }
+            if (given && axes != ax0 * 0x55u) {
+                if (angle) {
+                    const float* row = p.cos_sin + (long long)pos3 * (2 * n) + j0;
+                    const float4 c3 = *reinterpret_cast<const float4*>(row);
+                    const float4 s3 = *reinterpret_cast<const float4*>(row + n);
+                    if (ax1 != ax0) c.y = c3.y, s.y = s3.y;
+                    if (ax2 != ax0) c.z = c3.z, s.z = s3.z;
+                    c.w = ax3 != ax0 ? c3.w : c.w, s.w = ax3 != ax0 ? s3.w : s.w;
+                }
+                if (!two) {  // a third axis in the middle
+                    const int pos1 = p.positions[ax1 * p.axis_stride + tok], pos2 = p.positions[ax2 * p.axis_stride + tok];
+                    angle = angle && (unsigned)pos1 < (unsigned)p.max_pos && (unsigned)pos2 < (unsigned)p.max_pos;
+                    if (angle) {
+                        const float* row1 = p.cos_sin + (long long)pos1 * (2 * n) + j0 + 1;
+                        const float* row2 = p.cos_sin + (long long)pos2 * (2 * n) + j0 + 2;
+                        c.y = row1[0], s.y = row1[n];
+                        c.z = row2[0], s.z = row2[n];
+                    }
                 }
             }
+            cs[half * 4 + 0] = c.x, cs[half * 4 + 1] = c.y, cs[half * 4 + 2] = c.z, cs[half * 4 + 3] = c.w;
+            sn[half * 4 + 0] = s.x * sign, sn[half * 4 + 1] = s.y * sign;
+            sn[half * 4 + 2] = s.z * sign, sn[half * 4 + 3] = s.w * sign;
         }
     }
     // A row whose four threads do not all have their angles is not written in

@@ -88,12 +88,18 @@ struct Sequence {
 
 __device__ __forceinline__ Sequence load_sequence(const Args& a, int b) {
     Sequence s;
+    int past = 0;  // tokens beyond what the call said: only the ones before them are worked on
     if (a.seqstart_q != nullptr) {
         s.first = a.seqstart_q[b];
         s.count = a.seqstart_q[b + 1] - s.first;
         if (s.first < 0 || s.count < 0 || s.first > a.tokens - s.count) {
             flag_index_error(a.err_word);
             s.first = s.count = 0;
+        }
+        if (s.count > a.seqlen_q) {
+            flag_index_error(a.err_word);
+            past = s.count - a.seqlen_q;
+            s.count = a.seqlen_q;
         }
     } else {
         s.first = b * a.seqlen_q;
@@ -106,6 +112,7 @@ __device__ __forceinline__ Sequence load_sequence(const Args& a, int b) {
             flag_index_error(a.err_word);
             s.keys = (int)cap;
         }
+        s.keys = max(s.keys - past, 0);
     } else {
         s.keys = a.fixed_len;
     }

@@ -105,14 +105,8 @@ __device__ __forceinline__ RowsHeader* piece_headers(const Args& a) {
 __device__ __forceinline__ RowSeq load_row_seq(const Args& a, int b) {
     const Sequence s = load_sequence(a, b);
     RowSeq x{s.first, s.count, s.keys, 0, 0};
-    int rows = s.count * a.group;
+    const int rows = s.count * a.group;  // at most row_cap from here on
     if (rows < a.min_rows || rows > a.max_rows) return x;
-    if (rows > kMostRows || rows > a.row_cap) {  // more tokens than the call said: the first ones only
-        flag_index_error(a.err_word);
-        x.count = min(kMostRows, a.row_cap) / a.group;
-        if (x.count == 0) return x;
-        x.keys = max(0, min(s.keys, s.keys - s.count + x.count));
-    }
     x.kv_end = max(0, key_limit(a, Sequence{x.first, x.count, x.keys}, x.count - 1));
     x.units = max(1, (x.kv_end + kUnit - 1) / kUnit);
     return x;
@@ -719,8 +713,7 @@ fmha_prefix_finish(const __grid_constant__ Args a) {
     const Sequence s = load_sequence(a, b);
     const int rows = s.count * a.group;
     const int h = head / a.group, rt = (token - s.first) * a.group + head - h * a.group;
-    mine = mine && token >= s.first && token < s.first + s.count && rows >= a.min_rows && rows <= a.max_rows &&
-           rt < a.row_cap;  // (past the cap: more tokens than the call said)
+    mine = mine && token >= s.first && token < s.first + s.count && rows >= a.min_rows && rows <= a.max_rows;
     griddep_wait();  // every thread: the grid ends after the launches before it
     if (!mine) return;
     int2 parts = a.seq_parts[b];  // its first block (of each group of heads), and how many share it

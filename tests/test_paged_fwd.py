@@ -227,6 +227,18 @@ def test_more_tokens_than_said_is_reported():
     assert fm.status() == fm.FMHA_ERR_INDEX
 
 
+@pytest.mark.parametrize("new, said, prefix", [(9, 2, 0), (40, 9, 0), (300, 40, 0), (40, 9, 700)])
+def test_tokens_within_what_was_said_keep_their_results(new, said, prefix):
+    """A sequence of more tokens than said: reported, the first ones as they are."""
+    p = Problem([said, new, 1], [900, 1300, 800], 8, 2, packed=True, prefix=prefix)
+    o = p.run()
+    assert fm.status() == fm.FMHA_OK
+    few = p.run(max_seqlen_q=said)
+    assert fm.status() == fm.FMHA_ERR_INDEX
+    for at in (slice(0, 2 * said), slice(said + new, None)):
+        assert (o[at].double() - few[at].double()).abs().max() <= 2.0 ** -7 * o[at].double().abs().max()
+
+
 def test_refusals():
     p = Problem([1, 1], [40, 70], 4, 2)
     q, kc, vc, t, n = p.q, p.k_cache, p.v_cache, p.table, p.seqlens

@@ -249,8 +249,8 @@ int launch_rows(const Args& a, const Args* finish, bool after, int device, cudaS
         const long long threads = (long long)a.tokens * a.nhead_q * 16;
         return launch_dependent(fmha_prefix_finish, dim3((unsigned)((threads + 255) / 256)), 256, 0, stream, *finish);
     }
-    return launch_dependent(fmha_paged_rows_merge, dim3(kMaxRowBlocks, (a.nhead_k * a.row_cap + 3) / 4), 256, 0, stream,
-                            a);
+    return launch_dependent(fmha_paged_rows_merge,
+                            dim3(kMaxRowBlocks, std::min(kMergeBlocks, (a.nhead_k * a.row_cap + 3) / 4)), 256, 0, stream, a);
 }
 
 // `ranges`: key ranges of row tiles; after: it follows another kernel of the call.

@@ -348,7 +348,6 @@ fmha_paged_rows_kernel(const __grid_constant__ Args a) {
         const uint64_t policy = l2_policy_evict_first();
         const uint32_t ring0 = smem_u32(sm.ring[warp]), bar0 = smem_u32(sm.bar[warp]);
         int fill = 0;  // slot of the next load
-        const bool leader = elect_one();
         auto produce = [&]() {
             while (to_issue > 0 && issued - done < kRowStages) {
                 if (p.x.kv_end > 0) {
@@ -368,18 +367,14 @@ fmha_paged_rows_kernel(const __grid_constant__ Args a) {
                     }
                     const int nbox = (min(kUnit, p.x.kv_end - key0) + (1 << box_shift) - 1) >> box_shift;
                     const uint32_t bar = bar0 + fill * 8;
-                    if (leader) mbar_arrive_expect_tx(bar, (2 * nbox) << (box_shift + 7));
-                    // One elected lane issues the boxes: the copy instruction takes its
-                    // operands from uniform registers, so lanes side by side would be
-                    // taken one after the other, at several times the cost.
-                    for (int box = 0; box < nbox; ++box) {
-                        const int id = __shfl_sync(0xffffffffu, ids, page0 + box - win);
-                        const uint32_t dst = ring0 + fill * (2 * kUnitBytes) + (box << (box_shift + 7));
-                        if (leader) {
-                            if ((unsigned)id >= (unsigned)a.num_pages) flag_index_error(a.err_word);
-                            load_page_box(dst, &a.tm_k, bar, key0 & page_mask, head0 + p.h, id, policy);
-                            load_page_box(dst + kUnitBytes, &a.tm_v, bar, key0 & page_mask, head0 + p.h, id, policy);
-                        }
+                    const int id = __shfl_sync(0xffffffffu, ids, (page0 + lane - win) & 31);
+                    if (lane == 0) mbar_arrive_expect_tx(bar, (2 * nbox) << (box_shift + 7));
+                    __syncwarp();
+                    if (lane < nbox) {
+                        const uint32_t dst = ring0 + fill * (2 * kUnitBytes) + (lane << (box_shift + 7));
+                        if ((unsigned)id >= (unsigned)a.num_pages) flag_index_error(a.err_word);
+                        load_page_box(dst, &a.tm_k, bar, key0 & page_mask, head0 + p.h, id, policy);
+                        load_page_box(dst + kUnitBytes, &a.tm_v, bar, key0 & page_mask, head0 + p.h, id, policy);
                     }
                     ++issued;
                     fill = fill == kRowStages - 1 ? 0 : fill + 1;
@@ -639,8 +634,12 @@ fmha_paged_rows_kernel(const __grid_constant__ Args a) {
 }
 
 // Folds the pieces of the sequence that begins in block blockIdx.x and goes on
-// in the blocks after it.  64 threads per row: 16 cover the columns, the four
-// sixteens take every fourth piece, kBatch of them in flight.
+// in the blocks after it, four rows at a time.  64 threads per row: 16 cover the
+// columns, the four sixteens take every fourth piece, kBatch of them in flight.
+// kMergeBlocks per block of the rows kernel at most: a block without work costs
+// a nanosecond, and most have none (53 sequences of 11 to 46 tokens with 32 K/V
+// heads: 72 us with a block for every four rows, 59 with 16).
+constexpr int kMergeBlocks = 16;
 __global__ void __launch_bounds__(256)
 fmha_paged_rows_merge(const __grid_constant__ Args a) {
     constexpr int kBatch = 8;
@@ -650,43 +649,46 @@ fmha_paged_rows_merge(const __grid_constant__ Args a) {
     const RowsHeader hd = piece_headers(a)[blockIdx.x];
     if (hd.parts == 0) return;
     const int rows = hd.rows;
-    const int y = blockIdx.y * 4 + (int)(threadIdx.x >> 6);
-    const bool has_row = y < rows * hd.heads;
-    const int h = has_row ? hd.h0 + y / rows : 0, rt = has_row ? y - y / rows * rows : 0;
-    const int lane = threadIdx.x & 31, c4 = lane & 15;
-    float m = -INFINITY, l = 0.0f;
-    float4 o = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-    if (has_row)
-        for (int k0 = (threadIdx.x >> 4) & 3; k0 < hd.parts; k0 += 4 * kBatch) {
-            float2 ml[kBatch];
-            float4 z[kBatch];
+    for (int y0 = blockIdx.y * 4; y0 < rows * hd.heads; y0 += gridDim.y * 4) {
+        const int y = y0 + (int)(threadIdx.x >> 6);
+        const bool has_row = y < rows * hd.heads;
+        const int h = has_row ? hd.h0 + y / rows : 0, rt = has_row ? y - y / rows * rows : 0;
+        const int lane = threadIdx.x & 31, c4 = lane & 15;
+        float m = -INFINITY, l = 0.0f;
+        float4 o = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+        if (has_row)
+            for (int k0 = (threadIdx.x >> 4) & 3; k0 < hd.parts; k0 += 4 * kBatch) {
+                float2 ml[kBatch];
+                float4 z[kBatch];
 #pragma unroll
-            for (int u = 0; u < kBatch; ++u) {
-                const int k = k0 + 4 * u;
-                ml[u] = make_float2(-INFINITY, 0.0f);
-                z[u] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-                if (k < hd.parts) {
-                    const long long row = piece_row(a, 2 * ((int)blockIdx.x + k) + (k == 0), h, rt);
-                    ml[u] = *reinterpret_cast<const float2*>(piece_ml(a, row));
-                    z[u] = *reinterpret_cast<const float4*>(piece_o(a, row) + c4 * 4);
+                for (int u = 0; u < kBatch; ++u) {
+                    const int k = k0 + 4 * u;
+                    ml[u] = make_float2(-INFINITY, 0.0f);
+                    z[u] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+                    if (k < hd.parts) {
+                        const long long row = piece_row(a, 2 * ((int)blockIdx.x + k) + (k == 0), h, rt);
+                        ml[u] = *reinterpret_cast<const float2*>(piece_ml(a, row));
+                        z[u] = *reinterpret_cast<const float4*>(piece_o(a, row) + c4 * 4);
+                    }
                 }
-            }
 #pragma unroll
-            for (int u = 0; u < kBatch; ++u) fold4(m, l, o, ml[u].x, ml[u].y, z[u]);
+                for (int u = 0; u < kBatch; ++u) fold4(m, l, o, ml[u].x, ml[u].y, z[u]);
+            }
+        // Within the warp, then the row's second warp.
+        fold4(m, l, o, __shfl_xor_sync(0xffffffffu, m, 16), __shfl_xor_sync(0xffffffffu, l, 16),
+              make_float4(__shfl_xor_sync(0xffffffffu, o.x, 16), __shfl_xor_sync(0xffffffffu, o.y, 16),
+                          __shfl_xor_sync(0xffffffffu, o.z, 16), __shfl_xor_sync(0xffffffffu, o.w, 16)));
+        const int slot = threadIdx.x >> 6;
+        if ((threadIdx.x & 32) && lane < 16) {
+            other_o[slot][c4] = o;
+            other_ml[slot][c4] = make_float2(m, l);
         }
-    // Within the warp, then the row's second warp.
-    fold4(m, l, o, __shfl_xor_sync(0xffffffffu, m, 16), __shfl_xor_sync(0xffffffffu, l, 16),
-          make_float4(__shfl_xor_sync(0xffffffffu, o.x, 16), __shfl_xor_sync(0xffffffffu, o.y, 16),
-                      __shfl_xor_sync(0xffffffffu, o.z, 16), __shfl_xor_sync(0xffffffffu, o.w, 16)));
-    const int slot = threadIdx.x >> 6;
-    if ((threadIdx.x & 32) && lane < 16) {
-        other_o[slot][c4] = o;
-        other_ml[slot][c4] = make_float2(m, l);
-    }
-    __syncthreads();
-    if (has_row && !(threadIdx.x & 32) && lane < 16) {
-        fold4(m, l, o, other_ml[slot][c4].x, other_ml[slot][c4].y, other_o[slot][c4]);
-        emit_row4(a, Target{hd.first, rows, h, -1}, rt, c4, m, l, o);
+        __syncthreads();
+        if (has_row && !(threadIdx.x & 32) && lane < 16) {
+            fold4(m, l, o, other_ml[slot][c4].x, other_ml[slot][c4].y, other_o[slot][c4]);
+            emit_row4(a, Target{hd.first, rows, h, -1}, rt, c4, m, l, o);
+        }
+        __syncthreads();
     }
 }
 

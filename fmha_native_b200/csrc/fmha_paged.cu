@@ -17,6 +17,26 @@
 
 using namespace fmha_paged;
 
+// The end of a call: the merge of the sequences that cross the rows kernel's
+// blocks, by the first end_merge blocks, and the fold of the key ranges that
+// the tile kernel's blocks shared, by the others.  One kernel for both saves a
+// launch (50 sequences of 3 to 12 tokens: 20.2 -> 19.5 us); where there is only
+// the merge, the fold's registers would cost more (64 sequences of 100 to 4095
+// keys: 43.8 us with it, 42.4 without).
+constexpr int kEndThreads = 256;
+template <bool kMerge, bool kCombine>
+__global__ void __launch_bounds__(kEndThreads)
+fmha_paged_end(const __grid_constant__ Args a) {
+    griddep_wait();
+    const int x = blockIdx.x;
+    if (kMerge && (!kCombine || x < a.end_merge)) {
+        merge_pieces(a, x % kMaxRowBlocks, x / kMaxRowBlocks, a.end_merge / kMaxRowBlocks);
+    } else if (kCombine) {
+        const int y = x - (kMerge ? a.end_merge : 0);
+        combine_ranges(a, y % kCombineBlocks, y / kCombineBlocks * kCombineRows);
+    }
+}
+
 namespace {
 
 static_assert(sizeof(RowsShared) + 1024 <= 227 * 1024, "shared memory of a block");
@@ -231,26 +251,15 @@ int launch_dependent(Kernel kernel, dim3 grid, int threads, size_t smem, cudaStr
     return cudaLaunchKernelEx(&cfg, kernel, a) == cudaSuccess ? FMHA_OK : FMHA_ERR_LAUNCH;
 }
 
-// The rows kernel (after = it follows another kernel of the call), then the merge
-// of the sequences that cross its blocks or, under a prefix, of all partial results.
-int launch_rows(const Args& a, const Args* finish, bool after, int device, cudaStream_t stream) {
+// after: it follows another kernel of the call.
+int launch_rows(const Args& a, bool after, int device, cudaStream_t stream) {
     constexpr size_t smem = sizeof(RowsShared) + 1024;
     static std::atomic<unsigned long long> ready{0};
     if (!allow_smem(ready, device, reinterpret_cast<const void*>(fmha_paged_rows_kernel), smem))
         return FMHA_ERR_LAUNCH;
-    if (after) {
-        const int st = launch_dependent(fmha_paged_rows_kernel, dim3(kMaxRowBlocks), kRowThreadsTotal, smem, stream, a);
-        if (st != FMHA_OK) return st;
-    } else {
-        fmha_paged_rows_kernel<<<kMaxRowBlocks, kRowThreadsTotal, smem, stream>>>(a);
-        if (cudaGetLastError() != cudaSuccess) return FMHA_ERR_LAUNCH;
-    }
-    if (finish != nullptr) {
-        const long long threads = (long long)a.tokens * a.nhead_q * 16;
-        return launch_dependent(fmha_prefix_finish, dim3((unsigned)((threads + 255) / 256)), 256, 0, stream, *finish);
-    }
-    return launch_dependent(fmha_paged_rows_merge,
-                            dim3(kMaxRowBlocks, std::min(kMergeBlocks, (a.nhead_k * a.row_cap + 3) / 4)), 256, 0, stream, a);
+    if (after) return launch_dependent(fmha_paged_rows_kernel, dim3(kMaxRowBlocks), kRowThreadsTotal, smem, stream, a);
+    fmha_paged_rows_kernel<<<kMaxRowBlocks, kRowThreadsTotal, smem, stream>>>(a);
+    return cudaGetLastError() == cudaSuccess ? FMHA_OK : FMHA_ERR_LAUNCH;
 }
 
 // `ranges`: key ranges of row tiles; after: it follows another kernel of the call.
@@ -322,23 +331,38 @@ int run(const FmhaPagedParams* p, bool prefix, cudaStream_t stream) {
         }
     }
     if (z.rows) {
-        a.row_cap = z.row_cap;
-        if (z.tile) a.max_rows = kMostRows;
-        if ((st = cache_maps(ctx, a, p, kUnit)) != FMHA_OK) return st;
-        Args finish = a;
+        Args r = a;
+        r.row_cap = z.row_cap;
+        if (z.tile) r.max_rows = kMostRows;
+        if ((st = cache_maps(ctx, r, p, kUnit)) != FMHA_OK) return st;
         if (prefix) {
-            finish.part_n = z.prefix_splits;
-            a.seq_parts = finish.seq_parts = info;
-            a.out_o = part_o + part_rows * kHeadDim * z.prefix_splits;
-            a.out_lse = part_lse + part_rows * z.prefix_splits;
+            r.part_n = z.prefix_splits;
+            r.seq_parts = info;
+            r.out_o = part_o + part_rows * kHeadDim * z.prefix_splits;
+            r.out_lse = part_lse + part_rows * z.prefix_splits;
         }
-        st = launch_rows(a, prefix ? &finish : nullptr, z.tile || prefix, ctx.device, stream);
-        if (st != FMHA_OK) return st;
+        if ((st = launch_rows(r, z.tile || prefix, ctx.device, stream)) != FMHA_OK) return st;
+        if (prefix) {
+            const long long threads = part_rows * 16;
+            st = launch_dependent(fmha_prefix_finish, dim3((unsigned)((threads + 255) / 256)), 256, 0, stream, r);
+            if (st != FMHA_OK) return st;
+        }
+    }
+    unsigned blocks = 0;
+    if (z.rows && !prefix) {
+        a.row_cap = z.row_cap;
+        a.end_merge = kMaxRowBlocks * std::min(kMergeBlocks, (a.nhead_k * z.row_cap + 3) / 4);
+        blocks += a.end_merge;
     }
     if (z.tile) {
         a.max_slots = kMaxTileSlots;
         a.part_n = z.prefix_splits;
-        st = launch_dependent(fmha_paged_combine, dim3(kCombineBlocks, (std::min(z.max_rows, kTileM) + 31) / 32), kCombineThreads, 0, stream, a);
+        blocks += kCombineBlocks * ((std::min(z.max_rows, kTileM) + kCombineRows - 1) / kCombineRows);
+    }
+    if (blocks > 0) {
+        const auto end = !z.tile ? fmha_paged_end<true, false>
+                         : a.end_merge ? fmha_paged_end<true, true> : fmha_paged_end<false, true>;
+        st = launch_dependent(end, dim3(blocks), kEndThreads, 0, stream, a);
     }
     return st;
 }

@@ -70,6 +70,7 @@ struct Args {
     float* pieces;              // rows kernel: scratch between its blocks
     int2* seq_parts;            // rows kernel under a prefix: per sequence its first block and, if it
                                 // crosses blocks, how many share it; last, its groups of blocks
+    int end_merge;              // blocks of the call's last kernel that merge the rows kernel's pieces
     int* err_word;
     unsigned long long wait_limit_ns;
 };

@@ -17,7 +17,7 @@
 //                they like: every warp streams the same number of bytes.
 //                Pieces (m, l, O) of a head whose units went to several warps
 //                are folded through shared memory, those of a sequence that
-//                crosses blocks by fmha_paged_rows_merge.  The shares follow
+//                crosses blocks by fmha_paged_end.  The shares follow
 //                from the lengths alone, so results do not depend on timing.
 //   streaming    Each warp has its own ring of kRowStages units in shared memory,
 //                filled by TMA (one box per page) several units ahead, across
@@ -633,23 +633,22 @@ fmha_paged_rows_kernel(const __grid_constant__ Args a) {
     }
 }
 
-// Folds the pieces of the sequence that begins in block blockIdx.x and goes on
-// in the blocks after it, four rows at a time.  64 threads per row: 16 cover the
+// Folds the pieces of the sequence that begins in block `block` and goes on in
+// the blocks after it, four rows at a time (256 threads, the part-th of parts_y
+// blocks that share the rows).  64 threads per row: 16 cover the
 // columns, the four sixteens take every fourth piece, kBatch of them in flight.
 // kMergeBlocks per block of the rows kernel at most: a block without work costs
 // a nanosecond, and most have none (53 sequences of 11 to 46 tokens with 32 K/V
 // heads: 72 us with a block for every four rows, 59 with 16).
 constexpr int kMergeBlocks = 16;
-__global__ void __launch_bounds__(256)
-fmha_paged_rows_merge(const __grid_constant__ Args a) {
+__device__ __forceinline__ void merge_pieces(const Args& a, int block, int part, int parts_y) {
     constexpr int kBatch = 8;
     __shared__ float4 other_o[4][16];
     __shared__ float2 other_ml[4][16];
-    griddep_wait();
-    const RowsHeader hd = piece_headers(a)[blockIdx.x];
+    const RowsHeader hd = piece_headers(a)[block];
     if (hd.parts == 0) return;
     const int rows = hd.rows;
-    for (int y0 = blockIdx.y * 4; y0 < rows * hd.heads; y0 += gridDim.y * 4) {
+    for (int y0 = part * 4; y0 < rows * hd.heads; y0 += parts_y * 4) {
         const int y = y0 + (int)(threadIdx.x >> 6);
         const bool has_row = y < rows * hd.heads;
         const int h = has_row ? hd.h0 + y / rows : 0, rt = has_row ? y - y / rows * rows : 0;
@@ -666,7 +665,7 @@ fmha_paged_rows_merge(const __grid_constant__ Args a) {
                     ml[u] = make_float2(-INFINITY, 0.0f);
                     z[u] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
                     if (k < hd.parts) {
-                        const long long row = piece_row(a, 2 * ((int)blockIdx.x + k) + (k == 0), h, rt);
+                        const long long row = piece_row(a, 2 * (block + k) + (k == 0), h, rt);
                         ml[u] = *reinterpret_cast<const float2*>(piece_ml(a, row));
                         z[u] = *reinterpret_cast<const float4*>(piece_o(a, row) + c4 * 4);
                     }

@@ -37,7 +37,7 @@
 // all of them busy (kPlanHere); with more, a first kernel writes the list of
 // whole tiles, cutting only what is far longer than the rest (kPlanList).  Jobs
 // of one range go to the output, the others through scratch slots that
-// fmha_paged_combine folds.
+// fmha_paged_end folds.
 #pragma once
 #include <type_traits>
 
@@ -729,28 +729,26 @@ fmha_paged_tile_kernel(const __grid_constant__ Args a) {
     }
 }
 
-// Folds the ranges of the jobs that several blocks shared into final rows:
-// blockIdx.y takes 32 rows of the jobs that begin in the slots blockIdx.x + i *
-// gridDim.x; 16 threads per row, four columns each, kBatch ranges in flight.
+// Folds the ranges of the jobs that several blocks shared into final rows: 16
+// rows from row0 on of the jobs that begin in the slots first + i * kCombineBlocks;
+// 16 threads per row, four columns each, kBatch ranges in flight.
 constexpr int kCombineBlocks = 148;
-constexpr int kCombineThreads = 512;
-__global__ void __launch_bounds__(kCombineThreads)
-fmha_paged_combine(const __grid_constant__ Args a) {
+constexpr int kCombineRows = 16;
+__device__ __forceinline__ void combine_ranges(const Args& a, int first, int row0) {
     constexpr int kEach = (kMaxTileSlots + kCombineBlocks - 1) / kCombineBlocks;
     constexpr int kBatch = 8;
-    griddep_wait();
     TileHeader head[kEach];
 #pragma unroll
     for (int i = 0; i < kEach; ++i) {
-        const int slot = blockIdx.x + i * kCombineBlocks;
+        const int slot = first + i * kCombineBlocks;
         head[i].parts = 0;
         if (slot < a.max_slots) head[i] = tile_headers(a)[slot];
     }
-    const int c4 = threadIdx.x & 15, rt = blockIdx.y * 32 + (int)(threadIdx.x >> 4);
+    const int c4 = threadIdx.x & 15, rt = row0 + (int)(threadIdx.x >> 4);
 #pragma unroll
     for (int i = 0; i < kEach; ++i) {
         if (rt >= head[i].rows || head[i].parts == 0) continue;
-        const int slot0 = blockIdx.x + i * kCombineBlocks;
+        const int slot0 = first + i * kCombineBlocks;
         float m = -INFINITY, l = 0.0f;
         float4 o = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
         for (int k0 = 0; k0 < head[i].parts; k0 += kBatch) {

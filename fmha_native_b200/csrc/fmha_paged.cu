@@ -132,7 +132,7 @@ bool make_plan(int batch, int seqlen_q, int total_q, bool packed, int nhead_q, i
         z.prefix_splits = pick_splits(std::max(1ll, z.prefix_tiles * nhead_k), (prefix_len + kTileN - 1) / kTileN);
         z.part = (size_t)z.tokens * nhead_q * (kHeadDim + 1) * sizeof(float);
         z.parts = z.prefix_splits + (z.rows ? 1 : 0);
-        z.info = round16((batch + 1ll) * sizeof(int2));
+        z.info = round16((long long)batch * sizeof(int2));
     }
     z.total = z.pieces + z.slots + z.list + z.info + z.part * z.parts;
     return true;
@@ -331,8 +331,9 @@ int run(const FmhaPagedParams* p, bool prefix, cudaStream_t stream) {
         }
     }
     if (z.rows) {
+        a.row_cap = z.row_cap;
+        a.head_groups = head_groups(p->nhead_k, z.row_cap);
         Args r = a;
-        r.row_cap = z.row_cap;
         if (z.tile) r.max_rows = kMostRows;
         if ((st = cache_maps(ctx, r, p, kUnit)) != FMHA_OK) return st;
         if (prefix) {
@@ -350,8 +351,7 @@ int run(const FmhaPagedParams* p, bool prefix, cudaStream_t stream) {
     }
     unsigned blocks = 0;
     if (z.rows && !prefix) {
-        a.row_cap = z.row_cap;
-        a.end_merge = kMaxRowBlocks * std::min(kMergeBlocks, (a.nhead_k * z.row_cap + 3) / 4);
+        a.end_merge = kMaxRowBlocks * std::min(kMergeBlocks, (a.nhead_k / a.head_groups * z.row_cap + 3) / 4);
         blocks += a.end_merge;
     }
     if (z.tile) {

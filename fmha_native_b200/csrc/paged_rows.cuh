@@ -10,8 +10,9 @@
 //
 //   work split   The keys of all sequences are laid end to end in units of 32,
 //                and the blocks take equal contiguous ranges of that line, with
-//                all K/V heads: heads lie side by side in a token, so a block's
-//                warps read neighbouring lines of memory at the same time.
+//                several K/V heads (head_groups): heads lie side by side in a
+//                token, so a block's warps read neighbouring lines of memory at
+//                the same time.
 //                Inside a block the line (sequence, head, unit) of its range is
 //                cut into equal shares for the 8 warps.  Lengths may differ as
 //                they like: every warp streams the same number of bytes.
@@ -28,10 +29,20 @@
 //                second product as a sum of two bf16 (value and remainder), so
 //                O keeps fp32 accuracy until its one rounding at the end.
 //
+// Measured (in a graph): 4 sequences of 60 000 to 130 000 keys, 16 K/V heads,
+// 251 us for 1.62 GB (6.4 TB/s, a copy's rate); 64 sequences of 100 to 4095 keys,
+// 32 heads over 8, 41 us for 172 MB (4.2 TB/s: start, first loads and fold are
+// about 12 us of it); one sequence of 776 keys 9.3 us, which is two launches in
+// line.  Against the tile kernel, which could take these rows too: 282, 59 and
+// 11.3 us.  (A tensor map that promotes its reads to 256 bytes in L2 made it
+// fetch twice what it used.)
+//
 // Keys past a row's limit get weight 0 by selection, and value rows past the
 // tile's last visible key are zeroed in shared memory before use, so whatever
 // the page holds there (NaN included) stays out of O.
 #pragma once
+#include <algorithm>
+
 #include "paged_common.cuh"
 
 namespace fmha_paged {
@@ -42,13 +53,34 @@ constexpr int kRowThreadsTotal = 32 * kRowWarps;
 constexpr int kUnitBytes = kUnit * kHeadDim * 2;  // 4 KB of K, as much of V
 constexpr int kMaxRowBlocks = 148;    // one block per SM
 
-constexpr int kMostRows = 16;         // rows of a K/V head that a warp holds
+// Rows of a K/V head that a warp holds: two halves of the matrix instruction's M.
+// With 9 to 16 rows this kernel is still ahead of the tile kernel where the keys
+// are many (64 sequences of 1365 to 4096 keys, 8 heads of 16 rows: 83 against 95
+// us, 32 heads of one with 16384: 32 against 37), and even where they are few (64
+// of 100 to 300 keys, 8 heads: 23 and 23).
+constexpr int kMostRows = 16;
 constexpr int kRowStages = 3;
 // A sequence's start and end in a block cost about as much time as this many
 // units (its first loads, Q, the results).  The shares count them once there is
 // more than a unit or two per block (64 sequences of 100 to 4095 keys: 42 us
 // with, 48 without).
 constexpr int kSeqCost = 5;
+
+// Groups of blocks that share out the K/V heads: each group works on all keys.
+// More heads a block keep more neighbouring memory together, more groups make
+// longer ranges, and so fewer pieces to fold; what the pieces weigh depends on
+// the rows.  Per group about 8 heads for 1 or 2 rows (4 sequences of 60 000 to
+// 130 000 keys, 16 heads: 248 us, 265 with one group, 260 with 4 heads), 4 for up
+// to 8 (64 sequences of 100 to 4095 keys, 8 heads of 4 rows: 41.0 us, 42.3 with
+// one group), 2 beyond (one sequence of 16384 keys, 32 heads of 16 rows: 32 us, 87
+// with one group, 36 with 8 heads).
+constexpr int kMostGroups = 16;
+inline int head_groups(int nhead_k, int rows) {
+    const int least = rows <= 2 ? 8 : rows <= 8 ? 4 : 2;
+    int g = std::min(kMostGroups, (nhead_k + least - 1) / least);
+    while (nhead_k % g != 0) --g;
+    return g;
+}
 
 // A sequence as this kernel takes it.
 struct RowSeq {
@@ -73,6 +105,7 @@ struct alignas(1024) RowsShared {
     Target piece_to[kRowWarps][2];
     int piece_job[kRowWarps][2];      // segment of the block * heads + head, -1: none
     int2 scan[kRowWarps];
+    unsigned present[kRowWarps];      // bit per thread: its sequences have units
     int run[2 * kRowWarps + 1];
     RowSeq start_seq;                 // of the block's first segment
     int start_b, start_x;
@@ -201,9 +234,10 @@ fmha_paged_rows_kernel(const __grid_constant__ Args a) {
         const int v = __shfl_up_sync(0xffffffffu, incl, d);
         if (lane >= d) incl += v;
     }
+    const unsigned present = __ballot_sync(0xffffffffu, mine_n > 0);
     int incl_n;
     if (per == 1) {
-        incl_n = __popc(__ballot_sync(0xffffffffu, mine_n > 0) & (0xffffffffu >> (31 - lane)));
+        incl_n = __popc(present & (0xffffffffu >> (31 - lane)));
     } else {
         incl_n = mine_n;
 #pragma unroll
@@ -212,7 +246,7 @@ fmha_paged_rows_kernel(const __grid_constant__ Args a) {
             if (lane >= d) incl_n += v;
         }
     }
-    if (lane == 31) sm.scan[warp] = make_int2(incl, incl_n);
+    if (lane == 31) sm.scan[warp] = make_int2(incl, incl_n), sm.present[warp] = present;
     __syncthreads();
     unsigned before = incl - mine, before_n = incl_n - mine_n, total = 0, total_n = 0;
 #pragma unroll
@@ -222,18 +256,13 @@ fmha_paged_rows_kernel(const __grid_constant__ Args a) {
         total += v.x;
         total_n += v.y;
     }
+    const bool some_absent = total_n < a.batch;
     const int seq_cost = total > 2 * kMaxRowBlocks ? kSeqCost : 0;
     auto cost_of = [&](int n) { return n > 0 ? n + seq_cost : 0; };
-    // Few units: groups of blocks share out the heads, too, at least 8 a block.
-    int groups = 1, group_blocks = gridDim.x, group = 0, index = blockIdx.x, head0 = 0, heads = a.nhead_k;
-    if (heads > kRowWarps && total > 0 && 2 * total <= gridDim.x) {
-        groups = min((heads + kRowWarps - 1) / kRowWarps, (int)(gridDim.x / total));
-        group_blocks = (int)gridDim.x / groups;
-        group = (int)blockIdx.x / group_blocks;
-        index = (int)blockIdx.x - group * group_blocks;
-        head0 = a.nhead_k * group / groups;
-        heads = a.nhead_k * (group + 1) / groups - head0;
-    }
+    // Groups of blocks share out the heads.
+    const int groups = a.head_groups, group_blocks = (int)gridDim.x / groups;
+    const int group = (int)blockIdx.x / group_blocks, index = (int)blockIdx.x - group * group_blocks;
+    const int heads = a.nhead_k / groups, head0 = group * heads;
     const unsigned cost_mine = mine + mine_n * seq_cost;
     before += before_n * seq_cost;
     total += total_n * seq_cost;
@@ -241,8 +270,6 @@ fmha_paged_rows_kernel(const __grid_constant__ Args a) {
     const unsigned want = (unsigned)min(((unsigned long long)total * heads + kRowWarps - 1) / kRowWarps,
                                         (unsigned long long)total);
     const unsigned blocks = min((unsigned)group_blocks, want);
-    if (a.seq_parts != nullptr && blockIdx.x == 0 && threadIdx.x == 0)
-        a.seq_parts[a.batch] = make_int2(groups, group_blocks);
     if (group >= groups || index >= blocks) {
         griddep_wait();  // the grid ends after the launch before it
         if (threadIdx.x == 0) piece_headers(a)[blockIdx.x].parts = 0;
@@ -286,13 +313,29 @@ fmha_paged_rows_kernel(const __grid_constant__ Args a) {
         k.unit0 = max(0, off - seq_cost);
         k.n = max(0, off + k.cost - seq_cost) - k.unit0;
     };
+    // The first sequence from b on that may have units: those of the tile kernel are
+    // passed over (53 sequences, 44 of them such: 68 us with a look at each one, 60
+    // without; 111 of 111 here: 20.5 us with the search, 16.9 without).
+    auto next_present = [&](int b) {
+        if (b % per != 0 || b >= a.batch) return b;
+        int t = b / per;
+        unsigned bits = sm.present[t >> 5] >> (t & 31);
+        while (bits == 0) {
+            t = (t | 31) + 1;
+            if (t >= kRowThreadsTotal) return a.batch;
+            bits = sm.present[t >> 5];
+        }
+        return (t + __ffs(bits) - 1) * per;
+    };
     auto next_segment = [&](Cursor& k) {
         do {
             k.left -= k.cost;
             k.cost = k.n = 0;
             if (k.left <= 0) return false;
             do {
-                if (++k.b >= a.batch) return false;
+                ++k.b;
+                if (some_absent) k.b = next_present(k.b);
+                if (k.b >= a.batch) return false;
                 k.x = load_row_seq(a, k.b);
             } while (k.x.units == 0);
             ++k.seg;
@@ -638,8 +681,7 @@ fmha_paged_rows_kernel(const __grid_constant__ Args a) {
 // blocks that share the rows).  64 threads per row: 16 cover the
 // columns, the four sixteens take every fourth piece, kBatch of them in flight.
 // kMergeBlocks per block of the rows kernel at most: a block without work costs
-// a nanosecond, and most have none (53 sequences of 11 to 46 tokens with 32 K/V
-// heads: 72 us with a block for every four rows, 59 with 16).
+// a nanosecond, and most have none.
 constexpr int kMergeBlocks = 16;
 __device__ __forceinline__ void merge_pieces(const Args& a, int block, int part, int parts_y) {
     constexpr int kBatch = 8;
@@ -693,7 +735,9 @@ __device__ __forceinline__ void merge_pieces(const Args& a, int block, int part,
 
 // The end of a prefix call: every row's partial results of the prefix and of
 // its own keys (one, or the pieces of a sequence that crossed blocks), folded
-// into the final row.  16 threads per row, four columns each.
+// into the final row.  16 threads per row, four columns each, kBatch loads in
+// flight.  Bound by the partial results' bytes (192 tokens of 32 heads under
+// 24577 keys: 12 us; with 16 in flight it was slower).
 __global__ void __launch_bounds__(256)
 fmha_prefix_finish(const __grid_constant__ Args a) {
     constexpr int kBatch = 8;
@@ -718,8 +762,7 @@ fmha_prefix_finish(const __grid_constant__ Args a) {
     griddep_wait();  // every thread: the grid ends after the launches before it
     if (!mine) return;
     int2 parts = a.seq_parts[b];  // its first block (of each group of heads), and how many share it
-    const int2 groups = a.seq_parts[a.batch];  // and the groups, and their blocks
-    parts.x += ((h + 1) * groups.x - 1) / a.nhead_k * groups.y;
+    parts.x += h / (a.nhead_k / a.head_groups) * (kMaxRowBlocks / a.head_groups);
     float m = -INFINITY, l = 0.0f;
     float4 o = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
     // The prefix's parts and the sequence's own, if one (what is read there

@@ -202,6 +202,24 @@ def test_prefix_is_what_paged_gives():
     assert (o.double() - q.double()).abs().max() <= 2.0 ** -7 * q.double().abs().max()
 
 
+@pytest.mark.parametrize("hk", [5, 10, 12, 17, 24, 32])
+@pytest.mark.parametrize("new, group", [(1, 1), (1, 4), (2, 4), (5, 3)])
+def test_heads_shared_out_to_blocks(hk, new, group):
+    Problem([new] * 3, [5000, 37, 777], hk * group, hk, 32).check()
+
+
+def test_heads_shared_out_under_a_prefix():
+    Problem([1] * 5, [1500, 0, 33, 700, 1], 48, 24, 16, prefix=300).check()
+
+
+def test_sequences_of_both_kernels_mixed():
+    """More sequences than threads, most of them many-row ones."""
+    new = [1 if i % 7 == 3 else 20 + i % 5 for i in range(300)]
+    Problem(new, [n + (11 * i) % 150 for i, n in enumerate(new)], 4, 4, 16, packed=True).check()
+    new = [1 if 250 < i < 255 else 0 for i in range(300)]
+    Problem(new, [n + (11 * i) % 150 for i, n in enumerate(new)], 4, 4, 16, packed=True).check()
+
+
 # ------------------------------------------------------------ refusals
 
 def test_index_errors_are_reported():

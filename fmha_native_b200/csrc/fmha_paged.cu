@@ -332,7 +332,9 @@ int run(const FmhaPagedParams* p, bool prefix, cudaStream_t stream) {
     }
     if (z.rows) {
         a.row_cap = z.row_cap;
-        a.head_groups = head_groups(p->nhead_k, z.row_cap);
+        const int groups = head_groups(p->nhead_k, z.row_cap);
+        a.group_blocks = kMaxRowBlocks / groups;
+        a.group_heads = p->nhead_k / groups;
         Args r = a;
         if (z.tile) r.max_rows = kMostRows;
         if ((st = cache_maps(ctx, r, p, kUnit)) != FMHA_OK) return st;
@@ -351,7 +353,7 @@ int run(const FmhaPagedParams* p, bool prefix, cudaStream_t stream) {
     }
     unsigned blocks = 0;
     if (z.rows && !prefix) {
-        a.end_merge = kMaxRowBlocks * std::min(kMergeBlocks, (a.nhead_k / a.head_groups * z.row_cap + 3) / 4);
+        a.end_merge = kMaxRowBlocks * std::min(kMergeBlocks, (a.group_heads * z.row_cap + 3) / 4);
         blocks += a.end_merge;
     }
     if (z.tile) {

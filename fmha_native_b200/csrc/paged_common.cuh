@@ -68,7 +68,8 @@ struct Args {
     float* slots;               // scratch of the jobs that blocks share
     int max_slots;
     float* pieces;              // rows kernel: scratch between its blocks
-    int head_groups;            // rows kernel: groups of blocks that share out the K/V heads
+    int group_blocks;           // rows kernel: blocks of each group, the groups share out the K/V heads
+    int group_heads;
     int2* seq_parts;            // rows kernel under a prefix: per sequence its first block (of each
                                 // group) and, if it crosses blocks, how many share it
     int end_merge;              // blocks of the call's last kernel that merge the rows kernel's pieces

@@ -10,7 +10,7 @@
 //
 //   work split   The keys of all sequences are laid end to end in units of 32,
 //                and the blocks take equal contiguous ranges of that line, with
-//                several K/V heads (head_groups): heads lie side by side in a
+//                several K/V heads (group_heads): heads lie side by side in a
 //                token, so a block's warps read neighbouring lines of memory at
 //                the same time.
 //                Inside a block the line (sequence, head, unit) of its range is
@@ -260,9 +260,9 @@ fmha_paged_rows_kernel(const __grid_constant__ Args a) {
     const int seq_cost = total > 2 * kMaxRowBlocks ? kSeqCost : 0;
     auto cost_of = [&](int n) { return n > 0 ? n + seq_cost : 0; };
     // Groups of blocks share out the heads.
-    const int groups = a.head_groups, group_blocks = (int)gridDim.x / groups;
+    const int group_blocks = a.group_blocks, heads = a.group_heads;
     const int group = (int)blockIdx.x / group_blocks, index = (int)blockIdx.x - group * group_blocks;
-    const int heads = a.nhead_k / groups, head0 = group * heads;
+    const int head0 = group * heads;
     const unsigned cost_mine = mine + mine_n * seq_cost;
     before += before_n * seq_cost;
     total += total_n * seq_cost;
@@ -270,7 +270,7 @@ fmha_paged_rows_kernel(const __grid_constant__ Args a) {
     const unsigned want = (unsigned)min(((unsigned long long)total * heads + kRowWarps - 1) / kRowWarps,
                                         (unsigned long long)total);
     const unsigned blocks = min((unsigned)group_blocks, want);
-    if (group >= groups || index >= blocks) {
+    if (head0 >= a.nhead_k || index >= blocks) {
         griddep_wait();  // the grid ends after the launch before it
         if (threadIdx.x == 0) piece_headers(a)[blockIdx.x].parts = 0;
         return;
@@ -762,7 +762,7 @@ fmha_prefix_finish(const __grid_constant__ Args a) {
     griddep_wait();  // every thread: the grid ends after the launches before it
     if (!mine) return;
     int2 parts = a.seq_parts[b];  // its first block (of each group of heads), and how many share it
-    parts.x += h / (a.nhead_k / a.head_groups) * (kMaxRowBlocks / a.head_groups);
+    parts.x += h / a.group_heads * a.group_blocks;
     float m = -INFINITY, l = 0.0f;
     float4 o = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
     // The prefix's parts and the sequence's own, if one (what is read there

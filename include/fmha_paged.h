@@ -19,10 +19,16 @@
  *     new token i of a sequence with n new ones has place seqlens_k[b] - n + i.
  *   - Nothing is allocated, copied from the host or synchronised by a call
  *     (after the first on a device), so calls may be captured in CUDA graphs.
+ *   - Limits: tokens * nhead_q and the 32-key units of batch * max_pages pages
+ *     below 2^31; nhead_q at most 8192; strides below 2^39.
+ *   - seqstart_q should cover tokens 0 .. total_q - 1; a token outside every
+ *     sequence is not worked on: append reports it and zeroes its row of q_out,
+ *     the attention leaves its row of o unwritten.
  *   - Returns an FMHA_* status.  Bad values that only the device can see (a
  *     page id outside the cache, a length past the page table, a position
- *     outside the angle table) access no memory out of range and are reported
- *     by fmha_fwd_d64_status as FMHA_ERR_INDEX.
+ *     outside the angle table, prefix sums that decrease or leave the tokens, more
+ *     new tokens in a sequence than seqlen_q) access no memory out of range
+ *     and are reported once by fmha_fwd_d64_status as FMHA_ERR_INDEX.
  */
 #ifndef FMHA_PAGED_H
 #define FMHA_PAGED_H
@@ -101,7 +107,7 @@ typedef struct FmhaPagedParams {
 } FmhaPagedParams;
 
 /* Device scratch that a call with these sizes needs (16-byte aligned, any
- * contents); total_q 0 for dense tokens, prefix_len 0 for
+ * contents; calls that may overlap need one each); total_q 0 for dense tokens, prefix_len 0 for
  * fmha_paged_fwd_d64_bf16.  0 on invalid sizes. */
 size_t fmha_paged_workspace_bytes(int batch, int seqlen_q, int total_q, int nhead_q, int nhead_k,
                                   int prefix_len);

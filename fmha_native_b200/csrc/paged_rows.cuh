@@ -32,9 +32,8 @@
 // Measured (in a graph): 4 sequences of 60 000 to 130 000 keys, 16 K/V heads,
 // 251 us for 1.62 GB (6.4 TB/s, a copy's rate); 64 sequences of 100 to 4095 keys,
 // 32 heads over 8, 41 us for 172 MB (4.2 TB/s: start, first loads and fold are
-// about 12 us of it); one sequence of 776 keys 9.3 us, which is two launches in
-// line.  Against the tile kernel, which could take these rows too: 282, 59 and
-// 11.3 us.  (A tensor map that promotes its reads to 256 bytes in L2 made it
+// about 12 us of it); one sequence of 776 keys 9.1 us, which is two launches in
+// line.  The tile kernel, which could take these rows too: 282, 59 and 11.3 us.  (A tensor map that promotes its reads to 256 bytes in L2 made it
 // fetch twice what it used.)
 //
 // Keys past a row's limit get weight 0 by selection, and value rows past the
@@ -61,9 +60,9 @@ constexpr int kMaxRowBlocks = 148;    // one block per SM
 constexpr int kMostRows = 16;
 constexpr int kRowStages = 3;
 // A sequence's start and end in a block cost about as much time as this many
-// units (its first loads, Q, the results).  The shares count them once there is
-// more than a unit or two per block (64 sequences of 100 to 4095 keys: 42 us
-// with, 48 without).
+// units (its first loads, Q, the results), and the shares count them: 64 sequences
+// of 100 to 4095 keys 41 us, 43 without; 111 of none or one under a prefix of 335
+// 13 us, 17 without.
 constexpr int kSeqCost = 5;
 
 // Groups of blocks that share out the K/V heads: each group works on all keys.
@@ -257,15 +256,14 @@ fmha_paged_rows_kernel(const __grid_constant__ Args a) {
         total_n += v.y;
     }
     const bool some_absent = total_n < a.batch;
-    const int seq_cost = total > 2 * kMaxRowBlocks ? kSeqCost : 0;
-    auto cost_of = [&](int n) { return n > 0 ? n + seq_cost : 0; };
+    auto cost_of = [&](int n) { return n > 0 ? n + kSeqCost : 0; };
     // Groups of blocks share out the heads.
     const int group_blocks = a.group_blocks, heads = a.group_heads;
     const int group = (int)blockIdx.x / group_blocks, index = (int)blockIdx.x - group * group_blocks;
     const int head0 = group * heads;
-    const unsigned cost_mine = mine + mine_n * seq_cost;
-    before += before_n * seq_cost;
-    total += total_n * seq_cost;
+    const unsigned cost_mine = mine + mine_n * kSeqCost;
+    before += before_n * kSeqCost;
+    total += total_n * kSeqCost;
     // As many blocks as give every warp a unit of some head.
     const unsigned want = (unsigned)min(((unsigned long long)total * heads + kRowWarps - 1) / kRowWarps,
                                         (unsigned long long)total);
@@ -287,7 +285,7 @@ fmha_paged_rows_kernel(const __grid_constant__ Args a) {
                 sm.start_x = (int)(beg - p);
                 sm.start_seq = x;
                 // The first page ids that the block will want.
-                const int page0 = (max(0, (int)(beg - p) - seq_cost) * kUnit) >> a.page_shift;
+                const int page0 = (max(0, (int)(beg - p) - kSeqCost) * kUnit) >> a.page_shift;
                 const int32_t* ids = a.page_table + b * a.table_stride + page0;
                 if (page0 < a.max_pages) prefetch_l1(ids);
                 if (page0 + 32 < a.max_pages) prefetch_l1(ids + 32);
@@ -310,12 +308,12 @@ fmha_paged_rows_kernel(const __grid_constant__ Args a) {
     // Sets the segment of sequence k.b that starts `off` into the sequence's cost.
     auto set_segment = [&](Cursor& k, int off) {
         k.cost = min(cost_of(k.x.units) - off, k.left);
-        k.unit0 = max(0, off - seq_cost);
-        k.n = max(0, off + k.cost - seq_cost) - k.unit0;
+        k.unit0 = max(0, off - kSeqCost);
+        k.n = max(0, off + k.cost - kSeqCost) - k.unit0;
     };
     // The first sequence from b on that may have units: those of the tile kernel are
     // passed over (53 sequences, 44 of them such: 68 us with a look at each one, 60
-    // without; 111 of 111 here: 20.5 us with the search, 16.9 without).
+    // without).  Where none is absent the search itself would cost up to a fifth.
     auto next_present = [&](int b) {
         if (b % per != 0 || b >= a.batch) return b;
         int t = b / per;

@@ -34,8 +34,8 @@
 // hides in part.  Measured: 4 sequences of 2048 tokens, 16 heads over 4 K/V
 // heads, no mask, 557 TF/s from pages of 64 keys, 508 of 16 and 421 of 8 (the
 // dense kernel: 650); 6 prompt chunks of 513 to 2048 tokens over up to 8191
-// keys, 199 us, of them 202 for this kernel alone with cold caches: tensor pipe
-// 32 % busy, special functions 49 %, issue slots 56 %.  One thread per row took
+// keys, 198 us; the kernel alone, with cold caches, 204: tensor pipe
+// 30 % busy, special functions 49 %, issue slots 54 %.  One thread per row took
 // 216 us there instead of 209 with two, blocks of 64 keys a tile (three to an
 // SM) 280 to 315, an arrival per warp instead of per thread at the barriers of
 // S and P 4 to 6 % more.
@@ -46,7 +46,7 @@
 // like, and their lengths are on the device: with fewer (row tile, head) jobs
 // than resident blocks, every block works out for itself the ranges that keep
 // all of them busy (kPlanHere: 24 sequences of 5 tokens, 24 heads over 4, 200 to
-// 3001 keys 17 us, with a list 24); with more, a first kernel writes the list of
+// 3001 keys 17 us, with a list 26); with more, a first kernel writes the list of
 // whole tiles, cutting only what is far longer than the rest (kPlanList: the
 // prompt chunks 205 us, 213 with every block planning for itself).  Jobs of one
 // range go to the output, the others through scratch slots that fmha_paged_end
@@ -72,9 +72,12 @@ constexpr uint32_t kColS = 0, kColO = 128, kColP = 192;
 constexpr int kTileRegsSoftmax = 96, kTileRegsControl = 48;
 static_assert(256 * kTileRegsSoftmax + 128 * kTileRegsControl <= kTileThreads * 80, "register split");
 constexpr float kLazyLog2 = 8.0f;
-constexpr int kLongRange = 16;  // key tiles up to which a job is not worth cutting where jobs abound
-constexpr int kMostParts = 64;  // ranges of a job (their fold is one block's work per 32 rows)
-constexpr int kPolyOf16 = 4;  // pairs of every 16 whose exponential runs on the FMA pipe
+// Key tiles up to which a job is not worth cutting where jobs abound (prompt chunks:
+// 198 us; 220 with no job cut, however long; 198 with 8).
+constexpr int kLongRange = 16;
+constexpr int kMostParts = 64;  // ranges of a job (their fold is one block's work per 16 rows)
+// Pairs of every 16 whose exponential runs on the FMA pipe (prompt chunks: 201 us; 211 with 0, 206.5 with 6).
+constexpr int kPolyOf16 = 4;
 
 // A block's work (for one K/V head): range k of the keys of a row tile.
 struct alignas(16) TileItem {

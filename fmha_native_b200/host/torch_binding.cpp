@@ -186,10 +186,39 @@ Batch batch_of(const at::Tensor& table, const at::Tensor& lengths, const at::Ten
     return b;
 }
 
-CUstream_st* stream_of(PyObject* o, int device) {
-    if (o != Py_None) return reinterpret_cast<CUstream_st*>(static_cast<uintptr_t>(integer(o)));
-    return c10::cuda::getCurrentCUDAStream((c10::DeviceIndex)device).stream();
-}
+// The stream of a call: the current one, or the one that the caller names.  A
+// named stream is the current one while a CallStream lives, so that the scratch
+// and the results come from memory that is this stream's to use: the allocator
+// hands a block that was freed on one stream to that stream's next request at
+// once, whatever other streams still do with it.  given(): a result goes back to
+// a caller on another stream, who may drop it while that stream still reads it.
+class CallStream {
+public:
+    CallStream(PyObject* o, int device) : outer_(c10::cuda::getCurrentCUDAStream((c10::DeviceIndex)device)) {
+        cudaStream_t named = outer_.stream();
+        if (o != Py_None) named = reinterpret_cast<cudaStream_t>(static_cast<uintptr_t>(integer(o)));
+        if (named == cudaStreamLegacy) named = nullptr;  // two names of the default stream
+        stream_ = named;
+        other_ = named != outer_.stream();
+        if (other_)
+            c10::cuda::setCurrentCUDAStream(c10::cuda::getStreamFromExternal(named, (c10::DeviceIndex)device));
+    }
+    ~CallStream() {
+        if (other_) c10::cuda::setCurrentCUDAStream(outer_);
+    }
+    CallStream(const CallStream&) = delete;
+    CallStream& operator=(const CallStream&) = delete;
+    CUstream_st* get() const { return stream_; }
+    const at::Tensor& given(const at::Tensor& t) const {
+        if (other_) t.record_stream(outer_);
+        return t;
+    }
+
+private:
+    c10::cuda::CUDAStream outer_;
+    cudaStream_t stream_ = nullptr;
+    bool other_ = false;
+};
 
 void done(int status, const char* what) {
     if (status != FMHA_OK) throw Bad{status, what};
@@ -210,15 +239,16 @@ PyObject* rope(PyObject* const* a) {
     const Heads x = heads(q, "q", ax, dev);
     const c10::cuda::CUDAGuard guard((c10::DeviceIndex)dev);
     const at::AutoDispatchBelowADInplaceOrView below;
+    const CallStream stream(a[11], dev);
     FmhaRopeParams p{};
-    at::Tensor qo = a[9] == Py_None ? at::empty_like(q) : tensor(a[9], "out");
+    at::Tensor qo = a[9] == Py_None ? stream.given(at::empty_like(q)) : tensor(a[9], "out");
     const Heads xo = heads(qo, "out", ax, dev);
     if (!same_shape(x, xo)) bad("out must have q's and k's shapes");
     at::Tensor ko;
     if (k) {
         const Heads y = heads(*k, "k", ax, dev);
         if (!same_tokens(x, y)) bad("k must have q's tokens");
-        ko = a[10] == Py_None ? at::empty_like(*k) : tensor(a[10], "out");
+        ko = a[10] == Py_None ? stream.given(at::empty_like(*k)) : tensor(a[10], "out");
         const Heads yo = heads(ko, "out", ax, dev);
         if (!same_shape(y, yo)) bad("out must have q's and k's shapes");
         p.k = y.p, p.k_out = yo.p;
@@ -236,7 +266,7 @@ PyObject* rope(PyObject* const* a) {
     p.interleaved = truth(a[6]), p.inverse = truth(a[7]);
     if (q.numel() == 0) p.q = p.q_out = nullptr;
     if (k && k->numel() == 0) p.k = p.k_out = nullptr;
-    if (p.q || p.k) done(g_rope(&p, stream_of(a[11], dev)), "rope");
+    if (p.q || p.k) done(g_rope(&p, stream.get()), "rope");
     PyObject* first = wrapped(a[9], qo);
     PyObject* second = k ? wrapped(a[10], ko) : none();
     PyObject* both = first && second ? PyTuple_Pack(2, first, second) : nullptr;
@@ -255,6 +285,7 @@ PyObject* append(PyObject* const* a) {
     if (!same_shape(x, y)) bad("v must have k's shape");
     const c10::cuda::CUDAGuard guard((c10::DeviceIndex)dev);
     const at::AutoDispatchBelowADInplaceOrView below;
+    const CallStream stream(a[15], dev);
     const Cache c = cache(tensor(a[2], "k_cache"), tensor(a[3], "v_cache"), dev);
     if (x.heads != c.heads) bad("k must have the cache's heads");
     const Batch b = batch_of(tensor(a[4], "page_table"), tensor(a[5], "seqlens_k"), optional(a[12], "cu_seqlens_q"), x,
@@ -265,7 +296,7 @@ PyObject* append(PyObject* const* a) {
     if (q) {
         const Heads z = heads(*q, "q", ax, dev);
         if (!same_tokens(x, z)) bad("q must have k's tokens");
-        qo = a[14] == Py_None ? at::empty_like(*q) : tensor(a[14], "q_out");
+        qo = a[14] == Py_None ? stream.given(at::empty_like(*q)) : tensor(a[14], "q_out");
         const Heads zo = heads(qo, "q_out", ax, dev);
         if (!same_shape(z, zo)) bad("q_out must have q's shape");
         p.q = z.p, p.q_out = zo.p;
@@ -293,7 +324,7 @@ PyObject* append(PyObject* const* a) {
     p.total_q = ax.dense ? 0 : p.seqlen_q;
     p.nhead_k = c.heads, p.page_size = c.page, p.num_pages = c.pages, p.max_pages = b.max_pages;
     p.interleaved = truth(a[11]);
-    if (k.numel() > 0) done(g_append(&p, stream_of(a[15], dev)), "paged_append");
+    if (k.numel() > 0) done(g_append(&p, stream.get()), "paged_append");
     return q ? wrapped(a[14], qo) : none();
 }
 
@@ -306,6 +337,7 @@ PyObject* attend(PyObject* const* a) {
     const Heads x = heads(q, "q", ax, dev);
     const c10::cuda::CUDAGuard guard((c10::DeviceIndex)dev);
     const at::AutoDispatchBelowADInplaceOrView below;
+    const CallStream stream(a[16], dev);
     const Cache c = cache(tensor(a[1], "k_cache"), tensor(a[2], "v_cache"), dev);
     const Batch b = batch_of(tensor(a[3], "page_table"), tensor(a[4], "seqlens_k"), optional(a[8], "cu_seqlens_q"), x,
                              ax, dev);
@@ -319,7 +351,7 @@ PyObject* attend(PyObject* const* a) {
             bad("prefix_pages must be [pages] with room for prefix_len >= 1 keys");
         p.prefix_len = (int)len;
     }
-    at::Tensor out = a[13] == Py_None ? at::empty_like(q) : tensor(a[13], "out");
+    at::Tensor out = a[13] == Py_None ? stream.given(at::empty_like(q)) : tensor(a[13], "out");
     const Heads xo = heads(out, "out", ax, dev);
     if (!same_shape(x, xo)) bad("out must have q's shape");
     at::Tensor lse;
@@ -328,7 +360,7 @@ PyObject* attend(PyObject* const* a) {
         const std::array<int64_t, 3> want{b.batch, x.heads, x.tokens};
         const at::IntArrayRef shape(want.data() + (ax.dense ? 0 : 1), ax.dense ? 3 : 2);
         if (a[14] == Py_None) {
-            lse = at::empty(shape, q.options().dtype(at::kFloat));
+            lse = stream.given(at::empty(shape, q.options().dtype(at::kFloat)));
         } else {
             lse = tensor(a[14], "lse_out");
             if (lse.sizes() != shape || lse.scalar_type() != at::kFloat || !lse.is_contiguous() || !lse.is_cuda() ||
@@ -368,7 +400,7 @@ PyObject* attend(PyObject* const* a) {
             if (scale == -1.0 && PyErr_Occurred()) throw PythonError{};
         }
         p.scale = (float)(scale * 1.4426950408889634);
-        done((prefix ? g_prefix : g_paged)(&p, stream_of(a[16], dev)), prefix ? "prefix_fwd" : "paged_fwd");
+        done((prefix ? g_prefix : g_paged)(&p, stream.get()), prefix ? "prefix_fwd" : "paged_fwd");
     }
     PyObject* first = wrapped(a[13], out);
     if (!with_lse) return first;

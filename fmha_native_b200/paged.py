@@ -16,9 +16,10 @@ strides that are multiples of 8; a heads-before-tokens cache is passed as
 ``seqlens_k [batch]``: the sequences' lengths WITH the new tokens, so new token
 i of n has place ``seqlens_k[b] - n + i``.  Tokens are dense (``[batch,
 seqlen_q, heads, 64]``) or packed (``[total, heads, 64]`` with int32
-``cu_seqlens_q``).  Calls run on the current stream, allocate only through
-torch, read nothing back, and may be captured in CUDA graphs after a first
-call on the device.  Index data that only the device can check is reported by
+``cu_seqlens_q``).  Calls run on the current stream or on the one that ``stream``
+names (its handle, an integer), allocate only through torch and on that stream,
+read nothing back, and may be captured in CUDA graphs after a first call on the
+device.  Index data that only the device can check is reported by
 ``fmha_native_b200.status()`` as ``FMHA_ERR_INDEX``.
 """
 from __future__ import annotations

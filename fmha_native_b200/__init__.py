@@ -337,12 +337,28 @@ def fmha_fwd(q, k, v, causal: bool = False, return_lse: bool = False, layout: st
     items_workspace_bytes(n) bytes (allocated here when omitted).
     `max_seqlen_q/k` (varlen): the longest sequence lengths, if known; else
     they are read from cu_seqlens (a stream synchronisation).
+    `stream`: the handle of a stream other than the current one; results and
+    scratch that are allocated here are then that stream's memory.
     """
     import torch
 
     for t in (q, k, v):
         if not (t.is_cuda and t.dtype == torch.bfloat16 and t.shape[-1] == HEAD_DIM):
             raise FmhaError(FMHA_ERR_ARG, "q/k/v must be CUDA bf16 tensors with head_dim 64")
+    if stream is not None and (
+            out is None or (return_lse and lse_out is None)
+            or (workspace is None and (items is not None or (tiles is not None and num_splits > 1)))):
+        here = torch.cuda.current_stream(q.device)
+        if stream != here.cuda_stream:
+            # The allocator may hand out what a stream has freed to the same
+            # stream's next request while other streams still use it.
+            with torch.cuda.stream(torch.cuda.ExternalStream(stream, device=q.device)):
+                got = fmha_fwd(q, k, v, causal, return_lse, layout, cu_seqlens_q, cu_seqlens_k, out, lse_out,
+                               None, tiles, num_splits, workspace, items, max_seqlen_q, max_seqlen_k)
+            for t, given in zip(got if return_lse else (got,), (out, lse_out)):
+                if given is None:
+                    t.record_stream(here)
+            return got
     o = out if out is not None else torch.empty_like(q)
     varlen = layout in ("thd", "htd")
     lse = None

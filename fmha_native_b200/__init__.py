@@ -349,10 +349,13 @@ def fmha_fwd(q, k, v, causal: bool = False, return_lse: bool = False, layout: st
             out is None or (return_lse and lse_out is None)
             or (workspace is None and (items is not None or (tiles is not None and num_splits > 1)))):
         here = torch.cuda.current_stream(q.device)
-        if stream != here.cuda_stream:
+        # (The default stream's handles are 0 and 1.)
+        named = (torch.cuda.default_stream(q.device) if stream in (0, 1)
+                 else torch.cuda.ExternalStream(stream, device=q.device))
+        if named.cuda_stream != here.cuda_stream:
             # The allocator may hand out what a stream has freed to the same
             # stream's next request while other streams still use it.
-            with torch.cuda.stream(torch.cuda.ExternalStream(stream, device=q.device)):
+            with torch.cuda.stream(named):
                 got = fmha_fwd(q, k, v, causal, return_lse, layout, cu_seqlens_q, cu_seqlens_k, out, lse_out,
                                None, tiles, num_splits, workspace, items, max_seqlen_q, max_seqlen_k)
             for t, given in zip(got if return_lse else (got,), (out, lse_out)):

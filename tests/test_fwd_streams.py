@@ -33,6 +33,7 @@ def forms(q, k, v):
 @pytest.mark.parametrize("form", ["whole", "splits", "items", "varlen"])
 def test_memory_is_the_named_streams(cuda_device, form):
     q, k, v = (normal((1, 1100, 3, 64), i) for i in range(3))
+    assert torch.cuda.current_stream() == torch.cuda.default_stream()
     f = forms(q, k, v)[form]
     want = f()
     side, here = torch.cuda.Stream(), torch.cuda.current_stream()
@@ -52,4 +53,14 @@ def test_memory_is_the_named_streams(cuda_device, form):
     got = f(stream=side.cuda_stream, out=o, lse_out=lse)
     side.synchronize()
     assert got[0] is o and got[1] is lse and torch.equal(o, want[0]) and torch.equal(lse, want[1])
+    # the default stream by its handles: after what it was given to do first
+    new = normal(q.shape, 9)
+    torch.cuda.synchronize()
+    torch.cuda._sleep(40_000_000)
+    q.copy_(new)
+    with torch.cuda.stream(side):
+        got = [f(stream=handle) for handle in (0, 1)]
+    torch.cuda.synchronize()
+    want = f()
+    assert all(torch.equal(a[0], want[0]) and torch.equal(a[1], want[1]) for a in got)
     assert fm.status() == fm.FMHA_OK

@@ -295,10 +295,9 @@ int run(const FmhaPagedParams* p, bool prefix, cudaStream_t stream) {
         if ((st = cache_maps(ctx, t, p, kTileN)) != FMHA_OK) return st;
         t.min_rows = kMostRows + 1;
         t.max_slots = kMaxTileSlots;
+        t.max_tiles = (int)z.tiles;
         if (z.tile && z.plan == kPlanList) {
             t.items = reinterpret_cast<TileItem*>(list);
-            t.max_items = (int)z.ranges;
-            t.max_tiles = (int)z.tiles;
             t.item_count = reinterpret_cast<int*>(t.items + z.ranges);
             t.tile_first = t.item_count + 1;
             fmha_paged_plan<<<1, kPlanThreads, 0, stream>>>(t);

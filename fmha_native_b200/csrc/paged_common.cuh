@@ -64,7 +64,7 @@ struct Args {
     TileItem* items;            // kPlanList: the list, its length, and scratch to make it
     int* item_count;
     int* tile_first;
-    int max_tiles, max_items;
+    int max_tiles;              // row tiles that the host made room for
     float* slots;               // scratch of the jobs that blocks share
     int max_slots;
     float* pieces;              // rows kernel: scratch between its blocks

@@ -192,23 +192,37 @@ __device__ __forceinline__ int parts_of(int n, long long len) {
     return n <= len ? 1 : min((n + (int)len - 1) / (int)len, kMostParts);
 }
 
+// No job begins in the slots from `i` on (to be called by `n` threads).
+__device__ __forceinline__ void clear_headers(const Args& a, int i, int n) {
+    for (; i < a.max_slots; i += n) tile_headers(a)[i].parts = 0;
+}
+
 // The plan for fewer jobs (row tile, head) than resident blocks, by every block
 // for itself: the shortest range length whose ranges all fit the device at
-// once.  All threads; false: no item for this block.
+// once.  All threads; false: no item for this block.  Prefix sums that decrease
+// let sequences overlap, and so have more row tiles than the host made room for
+// (max_tiles, below kTileBlocks): they are reported, and none is worked on.
+static_assert(kTileBlocks <= kTileThreads, "a row tile per thread");
 __device__ __forceinline__ bool plan_here(const Args& a, TileShared& sm, int y, TileItem& it) {
     const int tid = threadIdx.x;
+    const int me = (int)blockIdx.x * kTileThreads + tid, everyone = (int)gridDim.x * kTileThreads;
     // Row tiles in order, one per thread.
     int tiles, b = 0, m = 0;
     if (a.seqstart_q != nullptr) {
         const int per = (a.batch + kTileThreads - 1) / kTileThreads;
         const int b0 = min(a.batch, tid * per), b1 = min(a.batch, b0 + per);
-        int mine = 0;
+        long long mine = 0, sum;
         for (int i = b0; i < b1; ++i) mine += tile_count(a, load_sequence(a, i));
-        int at = block_scan(mine, sm.scan, tiles);
-        tiles = min(tiles, kTileThreads);  // more only if the prefix sums overlap
+        long long at = block_scan(mine, sm.scan64, sum);
+        if (sum > a.max_tiles) {
+            flag_index_error(a.err_word);
+            clear_headers(a, me, everyone);
+            return false;
+        }
+        tiles = (int)sum;
         for (int i = b0; i < b1 && mine > 0; ++i) {
             const int c = tile_count(a, load_sequence(a, i));
-            for (int k = 0; k < c && at < tiles; ++k, ++at) sm.tile_of[at] = make_int2(i, k);
+            for (int k = 0; k < c; ++k, ++at) sm.tile_of[at] = make_int2(i, k);
         }
         __syncthreads();
         if (tid < tiles) b = sm.tile_of[tid].x, m = sm.tile_of[tid].y;
@@ -226,7 +240,8 @@ __device__ __forceinline__ bool plan_here(const Args& a, TileShared& sm, int y, 
     }
     long long total;
     block_scan((long long)n, sm.scan64, total);
-    // The shortest length that may do, or else (jobs round up) one that surely does.
+    // The shortest length that may do, or else (jobs round up) one that surely does:
+    // all / len + jobs <= kTileBlocks ranges.
     const long long all = total * a.nhead_k;
     const int jobs = tiles * a.nhead_k;
     long long len = (all + kTileBlocks - 1) / kTileBlocks;
@@ -235,14 +250,11 @@ __device__ __forceinline__ bool plan_here(const Args& a, TileShared& sm, int y, 
         parts = tid < tiles ? parts_of(n, len) : 0;
         // Items in the upper half, those of split jobs in the lower.
         before = block_scan(parts << 16 | (parts > 1 ? parts : 0), sm.scan, sum);
-        if (again || jobs >= kTileBlocks || (sum >> 16) * a.nhead_k <= kTileBlocks) break;
+        if (again || (sum >> 16) * a.nhead_k <= kTileBlocks) break;
         len = (all + kTileBlocks - jobs - 1) / (kTileBlocks - jobs);
     }
-    if ((sum & 0xffff) * a.nhead_k > a.max_slots) return false;  // (overlapping prefix sums)
-    // No job begins in the slots that stay unused.
-    for (int i = (sum & 0xffff) * a.nhead_k + (int)blockIdx.x * kTileThreads + tid; i < a.max_slots;
-         i += (int)gridDim.x * kTileThreads)
-        tile_headers(a)[i].parts = 0;
+    // The slots that stay unused (a range has one at most, and kTileBlocks < max_slots).
+    clear_headers(a, (sum & 0xffff) * a.nhead_k + me, everyone);
     const int x = (sum >> 16) - 1 - y;  // tiles of later tokens (the ones with more keys) first
     if (x < 0) return false;
     const int k = x - (before >> 16);
@@ -259,7 +271,6 @@ __device__ __forceinline__ bool plan_here(const Args& a, TileShared& sm, int y, 
 constexpr int kPlanThreads = 256;
 __global__ void __launch_bounds__(kPlanThreads, 1)
 fmha_paged_plan(const __grid_constant__ Args a) {
-    __shared__ int scan[kPlanThreads / 32];
     __shared__ long long scan64[kPlanThreads / 32];
     griddep_launch_dependents();
     const int tid = threadIdx.x;
@@ -270,17 +281,19 @@ fmha_paged_plan(const __grid_constant__ Args a) {
     if (packed) {
         const int per = (a.batch + kPlanThreads - 1) / kPlanThreads;
         const int b0 = min(a.batch, tid * per), b1 = min(a.batch, b0 + per);
-        int mine = 0;
+        long long mine = 0, sum;
         for (int b = b0; b < b1; ++b) mine += tile_count(a, load_sequence(a, b));
-        int at = block_scan(mine, scan, tiles);
+        long long at = block_scan(mine, scan64, sum);
+        const bool fits = sum <= a.max_tiles;  // else sequences overlap, see plan_here
+        if (!fits) flag_index_error(a.err_word);
+        tiles = fits ? (int)sum : 0;
         for (int b = b0; b < b1; ++b) {
-            first[b] = at;
+            first[b] = fits ? (int)at : 0;
             at += tile_count(a, load_sequence(a, b));
         }
         if (tid == 0) first[a.batch] = tiles;
         __syncthreads();
     }
-    tiles = min(tiles, a.max_tiles);  // more only if the prefix sums overlap
     const int per = (tiles + kPlanThreads - 1) / kPlanThreads;
     const int t0 = min(tiles, tid * per), t1 = min(tiles, t0 + per);
     int b_first = 0, m_first = 0;
@@ -326,13 +339,15 @@ fmha_paged_plan(const __grid_constant__ Args a) {
     each_tile([&](int b, const Sequence& s, int m) {
         const int p = parts_of(key_tiles(a, s, m), len);
         for (int k = 0; k < p; ++k, ++at) {
-            const int x = items - 1 - at;
-            if (x >= 0 && x < a.max_items) a.items[x] = make_item(a, b, s, m, k, p, p > 1 ? slot * a.nhead_k : -1);
+            a.items[items - 1 - at] = make_item(a, b, s, m, k, p, p > 1 ? slot * a.nhead_k : -1);
         }
         if (p > 1) slot += p;
     });
-    if (tid == 0) *a.item_count = split * a.nhead_k <= a.max_slots ? min(items, a.max_items) : 0;
-    for (int i = split * a.nhead_k + tid; i < a.max_slots; i += kPlanThreads) tile_headers(a)[i].parts = 0;
+    // A job longer than len has less than 2 n / len ranges, all of them less than
+    // 4 * kTileBlocks = max_slots over the heads; and the items are the tiles and
+    // less than total / len <= 2 * kTileBlocks / heads more, as the list has room for.
+    if (tid == 0) *a.item_count = items;
+    clear_headers(a, split * a.nhead_k + tid, kPlanThreads);
 }
 
 __global__ void __launch_bounds__(kTileThreads, 2)

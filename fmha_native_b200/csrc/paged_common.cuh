@@ -229,8 +229,16 @@ __device__ __forceinline__ void drain_phase(uint32_t bar, uint32_t parity, const
         if (globaltimer_ns() - t0 > a.wait_limit_ns) return;
 }
 
+// A page id outside the cache is flagged and becomes -1, which the tensor maps
+// read as zeros (a map has one page at least, also where the cache has none).
+__device__ __forceinline__ int checked_page(const Args& a, int id) {
+    if ((unsigned)id < (unsigned)a.num_pages) return id;
+    flag_index_error(a.err_word);
+    return -1;
+}
+
 // One box of a page: 64 values x box rows, tensor coordinates (0, token in
-// page, head, page).  A page id outside the cache reads zeros.
+// page, head, page).
 __device__ __forceinline__ void load_page_box(uint32_t dst, const CUtensorMap* tm, uint32_t bar,
                                               int token, int head, int page, uint64_t policy) {
     tma_load_4d(dst, tm, bar, 0, token, head, page, policy);

@@ -413,9 +413,9 @@ fmha_paged_rows_kernel(const __grid_constant__ Args a) {
                     __syncwarp();
                     if (lane < nbox) {
                         const uint32_t dst = ring0 + fill * (2 * kUnitBytes) + (lane << (box_shift + 7));
-                        if ((unsigned)id >= (unsigned)a.num_pages) flag_index_error(a.err_word);
-                        load_page_box(dst, &a.tm_k, bar, key0 & page_mask, head0 + p.h, id, policy);
-                        load_page_box(dst + kUnitBytes, &a.tm_v, bar, key0 & page_mask, head0 + p.h, id, policy);
+                        const int page = checked_page(a, id);
+                        load_page_box(dst, &a.tm_k, bar, key0 & page_mask, head0 + p.h, page, policy);
+                        load_page_box(dst + kUnitBytes, &a.tm_v, bar, key0 & page_mask, head0 + p.h, page, policy);
                     }
                     ++issued;
                     fill = fill == kRowStages - 1 ? 0 : fill + 1;

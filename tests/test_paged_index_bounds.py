@@ -85,3 +85,39 @@ def test_overlapping_tiles_are_left_alone(name):
 def test_prefix_sums_that_leave_the_tokens(cu, hq):
     g = Guarded(cu, 40, 40, hq, 1, [500, 700])
     assert g.run() == fm.FMHA_ERR_INDEX
+
+
+@pytest.mark.parametrize("new, prefix", [(1, 0), (40, 0), (1, 100), (40, 100)])
+def test_a_cache_of_no_pages_is_not_read(new, prefix):
+    """Page id 0 of a cache that has no pages: reported, zeros instead of what lies there."""
+    import ctypes
+
+    batch, hq, hk, page = 2, 4, 2, 16
+    k, v = normal((16, page, hk, 64), 1), normal((16, page, hk, 64), 2)
+    table = torch.zeros(batch, 16, dtype=torch.int32, device="cuda")
+    lengths = torch.tensor([90, 200], dtype=torch.int32, device="cuda")
+    q = normal((batch, new, hq, 64), 3)
+    o = torch.full_like(q, 3.0)
+    n = fm.paged_workspace_bytes(batch, new, hq, hk, 0, prefix)
+    work = torch.empty(n, dtype=torch.uint8, device="cuda")
+    p = fm.FmhaPagedParams()
+    for name, t in (("q", q), ("k_cache", k), ("v_cache", v), ("o", o), ("page_table", table), ("seqlens_k", lengths),
+                    ("prefix_pages", table), ("workspace", work)):
+        setattr(p, name, t.data_ptr())
+    p.workspace_bytes = n
+    for t in ("q", "o"):
+        for name, s in (("stride", hq * 64), ("nhead_stride", 64), ("batch_stride", new * hq * 64)):
+            setattr(p, f"{name}_{t}", s)
+    for t in ("k", "v"):
+        for name, s in (("stride", hk * 64), ("nhead_stride", 64), ("page_stride", page * hk * 64)):
+            setattr(p, f"{name}_{t}", s)
+    p.batch, p.seqlen_q, p.nhead_q, p.nhead_k = batch, new, hq, hk
+    p.page_size, p.num_pages, p.max_pages, p.table_stride, p.prefix_len, p.causal, p.scale = page, 0, 16, 16, prefix, 1, 0.18
+    lib = fm.load_library()
+    call = lib.fmha_prefix_fwd_d64_bf16 if prefix else lib.fmha_paged_fwd_d64_bf16
+    assert call(ctypes.byref(p), torch.cuda.current_stream().cuda_stream) == fm.FMHA_OK
+    assert fm.status() == fm.FMHA_ERR_INDEX
+    assert not o.any()
+    p.num_pages = 16
+    assert call(ctypes.byref(p), torch.cuda.current_stream().cuda_stream) == fm.FMHA_OK
+    assert fm.status() == fm.FMHA_OK and o.any()

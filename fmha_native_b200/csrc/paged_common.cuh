@@ -146,7 +146,9 @@ __device__ __forceinline__ long long flat_row(const Args& a, int token, int head
 }
 
 // Running state of a softmax over disjoint sets of keys: reference maximum m
-// (log2 units), weight sum l, and O un-normalised, all fp32.
+// (log2 units), weight sum l, and O un-normalised, all fp32.  No key seen: m is
+// -inf and l is 0.  A NaN among the scores (or +inf, whose softmax has none but
+// inf - inf) makes l NaN, and so whatever it is folded into.
 // fold_scales: factors for the state (m, l) and for a newcomer (m2, l2).
 struct Fold {
     float keep, take;
@@ -173,10 +175,10 @@ __device__ __forceinline__ void fold4(float& m, float& l, float4& o, float m2, f
 // LSE.  O is rounded once, to nearest even.
 __device__ __forceinline__ void write_row4(const Args& a, int token, int head, int c, float m, float l, float4 o,
                                            bool first) {
-    const float inv = l > 0.0f ? 1.0f / l : 0.0f;
-    *reinterpret_cast<uint2*>(o_row(a, token, head) + c) =
-        make_uint2(pack_bf16_rne(o.x * inv, o.y * inv), pack_bf16_rne(o.z * inv, o.w * inv));
-    if (first && a.lse != nullptr) *lse_at(a, token, head) = l > 0.0f ? (m + __log2f(l)) * kLn2 : -INFINITY;
+    const float inv = 1.0f / l;
+    const uint2 y = make_uint2(pack_bf16_rne(o.x * inv, o.y * inv), pack_bf16_rne(o.z * inv, o.w * inv));
+    *reinterpret_cast<uint2*>(o_row(a, token, head) + c) = l == 0.0f ? make_uint2(0, 0) : y;
+    if (first && a.lse != nullptr) *lse_at(a, token, head) = l == 0.0f ? -INFINITY : (m + __log2f(l)) * kLn2;
 }
 
 // The same after folding in the part_n partial results of other launches.

@@ -175,11 +175,11 @@ __device__ __forceinline__ void emit_row4(const Args& a, const Target& to, int r
         write_row4(a, token, head, c4 * 4, m, l, o, c4 == 0);
     } else if (to.slot < 0) {
         // Under a prefix: one more partial result of the row.
-        const float inv = l > 0.0f ? 1.0f / l : 0.0f;
+        const float inv = l == 0.0f ? 0.0f : 1.0f / l;
         const long long row = flat_row(a, token, head);
         *reinterpret_cast<float4*>(a.out_o + row * kHeadDim + c4 * 4) =
             make_float4(o.x * inv, o.y * inv, o.z * inv, o.w * inv);
-        if (c4 == 0) a.out_lse[row] = l > 0.0f ? m + __log2f(l) : -INFINITY;
+        if (c4 == 0) a.out_lse[row] = l == 0.0f ? -INFINITY : m + __log2f(l);
     } else {
         const long long row = piece_row(a, to.slot, to.h, rt);
         *reinterpret_cast<float4*>(piece_o(a, row) + c4 * 4) = o;

@@ -582,6 +582,7 @@ fmha_paged_tile_kernel(const __grid_constant__ Args a) {
             const int lim = (has_row ? key_limit(a, seq, tok) : kv_end) - half * 64;
             const int lim_min = key_limit(a, seq, row0 / a.group);  // of the tile's first token
             float m_run = -INFINITY, l_run = 0.0f;
+            bool finite = false;  // every m_run of the warp is
             bool ok = true;
             for (int j = 0; j < n; ++j) {
                 bool got = wait_phase(smem_u32(&sm.bar_s), j & 1, abort_flag, a);
@@ -613,13 +614,14 @@ fmha_paged_tile_kernel(const __grid_constant__ Args a) {
                     mx[q] = __uint_as_float(rr[0]);
 #pragma unroll
                     for (int e = 1; e < 15; e += 2)
-                        mx[q] = fmax3(mx[q], __uint_as_float(rr[e]), __uint_as_float(rr[e + 1]));
-                    mx[q] = fmaxf(mx[q], __uint_as_float(rr[15]));
+                        mx[q] = fmax3_nan(mx[q], __uint_as_float(rr[e]), __uint_as_float(rr[e + 1]));
+                    mx[q] = fmax_nan(mx[q], __uint_as_float(rr[15]));
                 }
-                const float half_max = fmax3(mx[0], mx[1], fmaxf(mx[2], mx[3]));
+                const float half_max = fmax3_nan(mx[0], mx[1], fmax_nan(mx[2], mx[3]));
                 // Does either half of any of the 32 rows outgrow the reference (or
-                // did either warp give up)?  Seldom after the first tile.
-                const bool grew = (half_max - m_run) * scale > kLazyLog2;
+                // did either warp give up)?  Seldom after the first tile.  NaN does
+                // (and, to no effect, a row that has seen no key yet).
+                const bool grew = !((half_max - m_run) * scale <= kLazyLog2);
                 float alpha = 1.0f;
                 bool any = bar_or(pair_bar, 64, grew || !ok);
                 if (any) {
@@ -629,11 +631,12 @@ fmha_paged_tile_kernel(const __grid_constant__ Args a) {
                     const float other = sm.half_max[half ^ 1][t];
                     ok = sm.half_ok[warp] && sm.half_ok[warp ^ 4];  // the same for both warps
                     if (!ok) break;
-                    const float m_new = fmaxf(half_max, other);
-                    if ((m_new - m_run) * scale > kLazyLog2) {
+                    const float m_new = fmax_nan(half_max, other);
+                    if (m_new != -INFINITY && !((m_new - m_run) * scale <= kLazyLog2)) {
                         alpha = ex2_approx((m_run - m_new) * scale);
                         m_run = m_new;
                     }
+                    finite = __all_sync(0xffffffffu, fabsf(m_run) < INFINITY);
                 }
                 const float neg = m_run == -INFINITY ? 0.0f : -m_run * scale;
                 const float2 scale2 = make_float2(scale, scale), neg2 = make_float2(neg, neg);
@@ -658,7 +661,9 @@ fmha_paged_tile_kernel(const __grid_constant__ Args a) {
                             p[c * 16 + pr] = pack_bf16_rne(pp.x, pp.y);
                         }
                 };
-                if (masked) exp_tile(std::false_type{});  // may hold -inf
+                // The polynomial takes no NaN, and -inf as 2^-120: not under a mask, and
+                // not where a row's maximum is NaN or infinite.
+                if (masked || !finite) exp_tile(std::false_type{});
                 else exp_tile(std::true_type{});
                 const float2 s01 = fadd2(sum[0], sum[1]);
                 l_run = fmaf(l_run, alpha, s01.x + s01.y);
@@ -706,10 +711,11 @@ fmha_paged_tile_kernel(const __grid_constant__ Args a) {
                     tmem_wait_ld();
                     reg_fence(o);
                 }
-                float inv = l_run > 0.0f ? 1.0f / l_run : 0.0f;
-                float lse2 = l_run > 0.0f ? fmaf(m_run, scale, __log2f(l_run)) : -INFINITY;
+                const bool none = l_run == 0.0f;  // the row sees no key of the range
+                const float inv = 1.0f / l_run;
+                const float lse2 = none ? -INFINITY : fmaf(m_run, scale, __log2f(l_run));
                 auto val = [&](int col) {
-                    return n > 0 ? __uint_as_float(o[col]) * inv : 0.0f;
+                    return none ? 0.0f : __uint_as_float(o[col]) * inv;
                 };
                 float* part_o = nullptr;
                 float* part_lse = nullptr;
@@ -723,7 +729,7 @@ fmha_paged_tile_kernel(const __grid_constant__ Args a) {
                 }
                 if (has_row && part_o != nullptr) {
                     if (half == 0) *part_lse = lse2;
-                    if (l_run > 0.0f) {
+                    if (!none) {
                         float4* dst = reinterpret_cast<float4*>(part_o) + half * 8;
 #pragma unroll
                         for (int c = 0; c < 8; ++c)
@@ -733,7 +739,7 @@ fmha_paged_tile_kernel(const __grid_constant__ Args a) {
                     // Under a prefix: its results belong to the row, too.
 #pragma unroll
                     for (int c = 0; c < 8; ++c)
-                        finish_row4(a, token, head, half * 32 + c * 4, lse2, l_run > 0.0f ? 1.0f : 0.0f,
+                        finish_row4(a, token, head, half * 32 + c * 4, lse2, none ? 0.0f : 1.0f,
                                     make_float4(val(4 * c), val(4 * c + 1), val(4 * c + 2), val(4 * c + 3)),
                                     half == 0 && c == 0);
                 } else if (has_row) {

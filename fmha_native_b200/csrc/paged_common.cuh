@@ -239,6 +239,27 @@ __device__ __forceinline__ int checked_page(const Args& a, int id) {
     return -1;
 }
 
+// Values that are not finite.  A matrix product hands 0 * inf = NaN to rows that
+// give a key no weight because they do not see it, so where rows differ in what
+// they see, such values are taken out of shared memory and added by themselves,
+// a weight above 0 times an infinity being the infinity.
+// probe: stays 0 while the bf16 pairs are finite (x * 0 + 0), NaN from then on.
+__device__ __forceinline__ uint32_t probe_bf16(uint32_t pair, uint32_t probe) {
+    asm("fma.rn.bf16x2 %0, %1, %2, %0;" : "+r"(probe) : "r"(pair), "r"(0u));
+    return probe;
+}
+__device__ __forceinline__ uint32_t probe_bf16(uint4 x, uint32_t probe) {
+    return probe_bf16(x.w, probe_bf16(x.z, probe_bf16(x.y, probe_bf16(x.x, probe))));
+}
+__device__ __forceinline__ bool is_finite_bf16(uint32_t bits) { return (bits & 0x7f80u) != 0x7f80u; }
+// The pair with 0 for what is not finite.
+__device__ __forceinline__ uint32_t finite_bf16(uint32_t pair) {
+    return (is_finite_bf16(pair) ? pair & 0xffffu : 0u) | (is_finite_bf16(pair >> 16) ? pair & 0xffff0000u : 0u);
+}
+__device__ __forceinline__ uint4 finite_bf16(uint4 x) {
+    return make_uint4(finite_bf16(x.x), finite_bf16(x.y), finite_bf16(x.z), finite_bf16(x.w));
+}
+
 // One box of a page: 64 values x box rows, tensor coordinates (0, token in
 // page, head, page).
 __device__ __forceinline__ void load_page_box(uint32_t dst, const CUtensorMap* tm, uint32_t bar,

@@ -38,7 +38,8 @@
 //
 // Keys past a row's limit get weight 0 by selection, and value rows past the
 // tile's last visible key are zeroed in shared memory before use, so whatever
-// the page holds there (NaN included) stays out of O.
+// the page holds there (NaN included) stays out of O.  Visible values that are
+// not finite are added to the rows that see them without a product.
 #pragma once
 #include <algorithm>
 
@@ -488,6 +489,10 @@ fmha_paged_rows_kernel(const __grid_constant__ Args a) {
                     fence_async_smem();  // ordered before the slot's next TMA write
                     __syncwarp();
                 }
+                uint32_t probe = 0;
+#pragma unroll
+                for (int i = 0; i < kUnit * 8; i += 32)
+                    probe = probe_bf16(reinterpret_cast<const uint4*>(sm.ring[warp][slot][1])[i + lane], probe);
                 // S = Q K^T
                 float s[4][4];
 #pragma unroll
@@ -551,6 +556,26 @@ fmha_paged_rows_kernel(const __grid_constant__ Args a) {
                     }
                 }
                 // O += P V
+                if (__any_sync(0xffffffffu, probe != 0)) {
+                    // (Also where all rows see them: the remainder of a weight may be 0 or negative.)
+                    for (int key = 0; key < min(valid, kUnit); ++key)
+#pragma unroll
+                        for (int n = 0; n < 8; ++n) {
+                            const uint32_t pair = *reinterpret_cast<const uint32_t*>(
+                                sm.ring[warp][slot][1] + key * 128 + ((n ^ (key & 7)) << 4) + 4 * t4);
+#pragma unroll
+                            for (int q = 0; q < 4; ++q) {
+                                const uint32_t bits = q & 1 ? pair >> 16 : pair & 0xffffu;
+                                if (!is_finite_bf16(bits) && key0 + key < lim[q >> 1])
+                                    o[n][q] += __uint_as_float(bits << 16);
+                            }
+                        }
+                    __syncwarp();
+                    uint4* v = reinterpret_cast<uint4*>(sm.ring[warp][slot][1]);
+                    for (int i = lane; i < kUnit * 8; i += 32) v[i] = finite_bf16(v[i]);
+                    fence_async_smem();  // ordered before the slot's next TMA write
+                    __syncwarp();
+                }
 #pragma unroll
                 for (int st = 0; st < 2; ++st)
 #pragma unroll

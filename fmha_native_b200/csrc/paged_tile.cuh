@@ -14,7 +14,9 @@
 //   warp  9      products  one elected lane issues every tcgen05.mma; before the
 //                          last one the warp zeroes the value rows past the last
 //                          visible key, so what a page holds there (NaN included)
-//                          stays out of O
+//                          stays out of O; in tiles that some tokens see in part
+//                          it also sets values that are not finite aside, which
+//                          the softmax threads add to the rows that see them
 //   warps 10-11  idle      complete the warpgroup for setmaxnreg
 //
 // Tensor memory of a block (256 of 512 columns): S [0,128), O [128,192), P as
@@ -52,6 +54,7 @@
 // range go to the output, the others through scratch slots that fmha_paged_end
 // folds.
 #pragma once
+#include <climits>
 #include <type_traits>
 
 #include "paged_common.cuh"
@@ -111,10 +114,16 @@ struct alignas(1024) TileShared {
     uint64_t bar_s;                   // S written (commit)
     uint64_t bar_sfree;               // S in registers (a thread's arrival per row)
     uint64_t bar_p;                   // P written, O rescaled (likewise)
-    uint64_t bar_pv;                  // O += P V done (commit)
+    uint64_t bar_pv;                  // O += P V done (commit; an arrival for what the warp wrote itself)
     uint64_t bar_drain;
     uint32_t tmem_base;
     int abort_flag;
+    // Keys of the range from all_see on are seen by some of the tile's tokens only
+    // (`partly`: there are such).  Of their values that are not finite: per column
+    // the first key with NaN, +inf and -inf (INT_MAX: none), and whether there is any.
+    int all_see;
+    bool partly, any_odd;
+    int first_odd[3][kHeadDim];
     int scan[kTileWarps];
     long long scan64[kTileWarps];
     TileItem item;
@@ -350,6 +359,45 @@ fmha_paged_plan(const __grid_constant__ Args a) {
     clear_headers(a, split * a.nhead_k + tid, kPlanThreads);
 }
 
+// Takes the values that are not finite out of rows [lo, hi) of a V tile whose
+// first key is k0, and notes the first key with each kind of them (one warp).
+// (Inline it takes registers from the softmax: 64 tokens under 8192 shared keys 34.5 us, 33.8 so.)
+__device__ __noinline__ void set_aside_odd_values(TileShared& sm, int slot, int k0, int lo, int hi) {
+    const int lane = threadIdx.x & 31;
+    uint4* v = reinterpret_cast<uint4*>(sm.kv[slot]);
+    uint32_t probe = 0;
+    for (int x = lo * 8 + lane; x < hi * 8; x += 32) probe = probe_bf16(v[x], probe);
+    if (!__any_sync(0xffffffffu, probe != 0)) return;
+    for (int x = lo * 8 + lane; x < hi * 8; x += 32) {
+        const int key = x >> 3, col0 = ((x & 7) ^ (key & 7)) * 8;
+        const uint16_t* bits = reinterpret_cast<const uint16_t*>(v + x);
+        for (int e = 0; e < 8; ++e)
+            if (!is_finite_bf16(bits[e]))
+                atomicMin(&sm.first_odd[(bits[e] & 0x7f) != 0 ? 0 : bits[e] >> 15 ? 2 : 1][col0 + e], k0 + key);
+        v[x] = finite_bf16(v[x]);
+    }
+    if (lane == 0) sm.any_odd = true;
+    asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+    __syncwarp();
+}
+
+// Adds them to the 32 columns from col0 on, at tensor memory address `at`, of the
+// threads' rows, which see the keys before `end`.
+__device__ __forceinline__ void add_odd_values(const TileShared& sm, uint32_t at, int col0, int end) {
+#pragma unroll 1
+    for (int e = 0; e < kHeadDim / 2; ++e) {
+        uint32_t r = tmem_ld1(at + e);
+        tmem_wait_ld();
+        asm volatile("" : "+r"(r));  // used after the wait
+        float o = __uint_as_float(r);
+        if (sm.first_odd[0][col0 + e] < end) o = NAN;
+        if (sm.first_odd[1][col0 + e] < end) o += INFINITY;
+        if (sm.first_odd[2][col0 + e] < end) o -= INFINITY;
+        tmem_st1(at + e, __float_as_uint(o));
+    }
+    tmem_wait_st();
+}
+
 __global__ void __launch_bounds__(kTileThreads, 2)
 fmha_paged_tile_kernel(const __grid_constant__ Args a) {
     extern __shared__ uint8_t smem_raw[];
@@ -448,7 +496,7 @@ fmha_paged_tile_kernel(const __grid_constant__ Args a) {
             mbar_init(smem_u32(&sm.bar_s), 1);
             mbar_init(smem_u32(&sm.bar_sfree), 64 * active);
             mbar_init(smem_u32(&sm.bar_p), 64 * active);
-            mbar_init(smem_u32(&sm.bar_pv), 1);
+            mbar_init(smem_u32(&sm.bar_pv), 2);
             mbar_init(smem_u32(&sm.bar_drain), 1);
             sm.abort_flag = 0;
             fence_barrier_init();
@@ -459,6 +507,13 @@ fmha_paged_tile_kernel(const __grid_constant__ Args a) {
             issue_load(2 * j, page);
             issue_load(2 * j + 1, page);
             page = next;
+        }
+    } else if (warp == kWarpMma) {
+        for (int i = lane; i < 3 * kHeadDim; i += 32) sm.first_odd[0][i] = INT_MAX;
+        if (lane == 0) {
+            sm.any_odd = false;
+            sm.all_see = max(0, key_limit(a, seq, row0 / a.group));
+            sm.partly = n > 0 && sm.all_see < min(kv_end, (j0 + n) * kTileN);
         }
     } else if (warp < kSoftmaxWarps && n > 0) {
         uint4 x[4];
@@ -558,10 +613,15 @@ fmha_paged_tile_kernel(const __grid_constant__ Args a) {
                     asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
                     __syncwarp();
                 }
+                if (ok && sm.partly) {
+                    const int k0 = (j0 + j) * kTileN;
+                    set_aside_odd_values(sm, slot_of(iv), k0, max(0, sm.all_see - k0), min(kTileN, kv_end - k0));
+                }
                 ok = ok && wait_all(&sm.bar_p, j & 1);
                 if (!ok) break;
                 tc_fence_after();
                 issue_pv(slot_of(iv), j > 0);
+                if (leader) mbar_arrive(smem_u32(&sm.bar_pv));
                 commit(&sm.bar_pv);
                 commit(&sm.bar_empty[slot_of(iv)]);
             }
@@ -707,6 +767,7 @@ fmha_paged_tile_kernel(const __grid_constant__ Args a) {
                 uint32_t o[32];
                 if (n > 0) {
                     tc_fence_after();
+                    if (sm.any_odd) add_odd_values(sm, tO, half * 32, lim + half * 64);
                     tmem_ld32(tO, o);
                     tmem_wait_ld();
                     reg_fence(o);

@@ -114,7 +114,8 @@ size_t fmha_paged_workspace_bytes(int batch, int seqlen_q, int total_q, int nhea
 
 /* O = softmax(scale * Q K^T + mask) V over each sequence's pages.  A row that
  * sees no key gets O = 0 and LSE = -inf; one with a score of NaN or +inf, which
- * has no softmax, O = LSE = NaN. */
+ * has no softmax, O = LSE = NaN.  Values of keys that a row does not see never
+ * reach it, NaN and infinities included. */
 int fmha_paged_fwd_d64_bf16(const FmhaPagedParams* params, struct CUstream_st* stream);
 
 /* The same where every sequence's keys are the prefix_len keys of

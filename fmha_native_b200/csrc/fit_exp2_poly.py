@@ -1,11 +1,12 @@
 """Fits the polynomial used by exp2_poly2() in sm100_ptx.cuh.
 
 2^x = 2^n * 2^f with n = round(x), f = x - n in [-0.5, 0.5]; 2^f is a
-degree-3 polynomial minimising the maximum RELATIVE error on that interval
-(Lawson iteratively reweighted least squares on Chebyshev points).  The
-printed float32 coefficients are the ones compiled into the kernel; the
-float32 Horner evaluation of them has max relative error ~7.5e-5, well below
-the bf16 rounding (2^-8) that P undergoes before the P.V product.
+polynomial minimising the maximum RELATIVE error on that interval (Lawson
+iteratively reweighted least squares on Chebyshev points).  The printed
+float32 coefficients are the ones compiled into the kernels.  In the float32
+Horner evaluation degree 3 (the dense kernel) has max relative error ~7.5e-5,
+well below the bf16 rounding (2^-8) that P undergoes before the P.V product;
+degree 5 (the attention over pages) ~2.3e-7, that of the hardware exponential.
 
 Run: python fmha_native_b200/csrc/fit_exp2_poly.py
 """
@@ -34,6 +35,7 @@ def fit(deg: int = 3, iters: int = 200):
 
 
 if __name__ == "__main__":
-    c, rel = fit()
-    print("coefficients c0..c3:", ", ".join(f"{x:.9e}f" for x in c))
-    print(f"max relative error (fp32 Horner): {rel:.3e}")
+    for degree in (3, 5):
+        c, rel = fit(degree)
+        print(f"coefficients c0..c{degree}:", ", ".join(f"{x:.9e}f" for x in c))
+        print(f"max relative error (fp32 Horner): {rel:.3e}")

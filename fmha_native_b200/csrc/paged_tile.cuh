@@ -30,7 +30,7 @@
 //
 // What bounds it: per key tile a block runs 16384 exponentials against 2 x
 // 128 x 128 x 64 multiply-adds, so the special-function unit (16 per clock)
-// would need twice the tensor pipe's time; a quarter of the exponentials
+// would need twice the tensor pipe's time; an eighth of the exponentials
 // therefore runs as a polynomial on the FMA pipe.  What remains is the chain
 // S -> registers -> P -> tensor memory of each tile, which the SM's other block
 // hides in part.  Measured: 4 sequences of 2048 tokens, 16 heads over 4 K/V
@@ -79,8 +79,11 @@ constexpr float kLazyLog2 = 8.0f;
 // 198 us; 220 with no job cut, however long; 198 with 8).
 constexpr int kLongRange = 16;
 constexpr int kMostParts = 64;  // ranges of a job (their fold is one block's work per 16 rows)
-// Pairs of every 16 whose exponential runs on the FMA pipe (prompt chunks: 201 us; 211 with 0, 206.5 with 6).
-constexpr int kPolyOf16 = 4;
+// Pairs of every 16 whose exponential runs on the FMA pipe, by a polynomial as
+// exact as the function unit (degree 5), since the row sums and the LSE take it
+// in fp32.  Prompt chunks: 205.6 us; 211.6 with 0, 206.0 with 3, 212.5 with 4 (a
+// polynomial of degree 3, whose 7.5e-5 show in the LSE, 204.2 with 4).
+constexpr int kPolyOf16 = 2;
 
 // A block's work (for one K/V head): range k of the keys of a row tile.
 struct alignas(16) TileItem {
@@ -714,7 +717,7 @@ fmha_paged_tile_kernel(const __grid_constant__ Args a) {
                                 make_float2(__uint_as_float(r[c][e]), __uint_as_float(r[c][e + 1])), scale2, neg2);
                             float2 pp;
                             if (kPoly && (pr + 1) * kPolyOf16 / 16 > pr * kPolyOf16 / 16)
-                                pp = exp2_poly2(x);
+                                pp = exp2_poly2<5>(x);
                             else
                                 pp = make_float2(ex2_approx(x.x), ex2_approx(x.y));
                             sum[pr & 1] = fadd2(sum[pr & 1], pp);

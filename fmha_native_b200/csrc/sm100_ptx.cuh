@@ -313,17 +313,30 @@ __device__ __forceinline__ void regs_dec() {
 // fit_exp2_poly.py, max relative error 7.5e-5) and 2^n is added to its
 // exponent field.  Inputs are clamped to >= -120 so the exponent never
 // underflows; callers use it only where every input is finite.
+// kDegree 5: max relative error 2.3e-7, as the function unit's 2^-22, for sums
+// that are kept in fp32.
+template <int kDegree = 3>
 __device__ __forceinline__ float2 exp2_poly2(float2 x) {
+    static_assert(kDegree == 3 || kDegree == 5, "fitted degrees");
     constexpr float kRound = 12582912.0f;  // 1.5 * 2^23
     x.x = fmaxf(x.x, -120.0f);
     x.y = fmaxf(x.y, -120.0f);
     const float2 t = fadd2(x, make_float2(kRound, kRound));
     const float2 n = fadd2(t, make_float2(-kRound, -kRound));
     const float2 f = ffma2(n, make_float2(-1.0f, -1.0f), x);
-    float2 p = ffma2(make_float2(5.517166853e-02f, 5.517166853e-02f), f,
-                     make_float2(2.426111400e-01f, 2.426111400e-01f));
-    p = ffma2(p, f, make_float2(6.932609677e-01f, 6.932609677e-01f));
-    p = ffma2(p, f, make_float2(9.999280572e-01f, 9.999280572e-01f));
+    auto both = [](float c) { return make_float2(c, c); };
+    float2 p;
+    if constexpr (kDegree == 3) {
+        p = ffma2(both(5.517166853e-02f), f, both(2.426111400e-01f));
+        p = ffma2(p, f, both(6.932609677e-01f));
+        p = ffma2(p, f, both(9.999280572e-01f));
+    } else {
+        p = ffma2(both(1.327647129e-03f), f, both(9.675541893e-03f));
+        p = ffma2(p, f, both(5.550713092e-02f));
+        p = ffma2(p, f, both(2.402212024e-01f));
+        p = ffma2(p, f, both(6.931469440e-01f));
+        p = ffma2(p, f, both(1.000000119e+00f));
+    }
     return make_float2(__uint_as_float(__float_as_uint(p.x) + (__float_as_uint(t.x) << 23)),
                        __uint_as_float(__float_as_uint(p.y) + (__float_as_uint(t.y) << 23)));
 }

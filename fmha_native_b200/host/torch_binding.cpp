@@ -220,6 +220,12 @@ private:
     bool other_ = false;
 };
 
+// A given tensor was written: autograd, which this module runs below, must not
+// take it for what it saved.  (Inference tensors have no version.)
+void written(const at::Tensor& t) {
+    if (!t.is_inference()) t.unsafeGetTensorImpl()->bump_version();
+}
+
 void done(int status, const char* what) {
     if (status != FMHA_OK) throw Bad{status, what};
 }
@@ -267,6 +273,8 @@ PyObject* rope(PyObject* const* a) {
     if (q.numel() == 0) p.q = p.q_out = nullptr;
     if (k && k->numel() == 0) p.k = p.k_out = nullptr;
     if (p.q || p.k) done(g_rope(&p, stream.get()), "rope");
+    if (a[9] != Py_None) written(qo);
+    if (k && a[10] != Py_None) written(ko);
     PyObject* first = wrapped(a[9], qo);
     PyObject* second = k ? wrapped(a[10], ko) : none();
     PyObject* both = first && second ? PyTuple_Pack(2, first, second) : nullptr;
@@ -324,7 +332,12 @@ PyObject* append(PyObject* const* a) {
     p.total_q = ax.dense ? 0 : p.seqlen_q;
     p.nhead_k = c.heads, p.page_size = c.page, p.num_pages = c.pages, p.max_pages = b.max_pages;
     p.interleaved = truth(a[11]);
-    if (k.numel() > 0) done(g_append(&p, stream.get()), "paged_append");
+    if (k.numel() > 0) {
+        done(g_append(&p, stream.get()), "paged_append");
+        written(tensor(a[2], "k_cache"));
+        written(tensor(a[3], "v_cache"));
+        if (q && a[14] != Py_None) written(qo);
+    }
     return q ? wrapped(a[14], qo) : none();
 }
 
@@ -401,6 +414,8 @@ PyObject* attend(PyObject* const* a) {
         }
         p.scale = (float)(scale * 1.4426950408889634);
         done((prefix ? g_prefix : g_paged)(&p, stream.get()), prefix ? "prefix_fwd" : "paged_fwd");
+        if (a[13] != Py_None) written(out);
+        if (with_lse && a[14] != Py_None) written(lse);
     }
     PyObject* first = wrapped(a[13], out);
     if (!with_lse) return first;

@@ -318,6 +318,15 @@ def params_from_tensors(q, k, v, o, lse=None, layout: str = "bshd",
     raise ValueError(f"unknown layout {layout!r}")
 
 
+def named_stream(handle: int, device):
+    """The torch stream of a handle (0 and 1 are the default stream's)."""
+    import torch
+
+    if handle in (0, 1):
+        return torch.cuda.default_stream(device)
+    return torch.cuda.ExternalStream(handle, device=device)
+
+
 def fmha_fwd(q, k, v, causal: bool = False, return_lse: bool = False, layout: str = "bshd",
              cu_seqlens_q=None, cu_seqlens_k=None, out=None, lse_out=None, stream=None,
              tiles=None, num_splits: int = 1, workspace=None, items=None,
@@ -349,9 +358,7 @@ def fmha_fwd(q, k, v, causal: bool = False, return_lse: bool = False, layout: st
             out is None or (return_lse and lse_out is None)
             or (workspace is None and (items is not None or (tiles is not None and num_splits > 1)))):
         here = torch.cuda.current_stream(q.device)
-        # (The default stream's handles are 0 and 1.)
-        named = (torch.cuda.default_stream(q.device) if stream in (0, 1)
-                 else torch.cuda.ExternalStream(stream, device=q.device))
+        named = named_stream(stream, q.device)
         if named.cuda_stream != here.cuda_stream:
             # The allocator may hand out what a stream has freed to the same
             # stream's next request while other streams still use it.

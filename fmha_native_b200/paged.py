@@ -19,7 +19,8 @@ seqlen_q, heads, 64]``) or packed (``[total, heads, 64]`` with int32
 ``cu_seqlens_q``).  Calls run on the current stream or on the one that ``stream``
 names (its handle, an integer), allocate only through torch and on that stream,
 read nothing back, and may be captured in CUDA graphs after a first call on the
-device.  Index data that only the device can check is reported by
+device.  :func:`rope` is differentiable; the cache's operators are for serving,
+and their results have no gradient.  Index data that only the device can check is reported by
 ``fmha_native_b200.status()`` as ``FMHA_ERR_INDEX``.
 """
 from __future__ import annotations
@@ -114,6 +115,34 @@ def rope_table(max_pos: int, rot_dim: int = 64, theta: float = 10000.0, inv_freq
     return torch.cat([angle.cos(), angle.sin()], 1).float().to(device if device is not None else "cuda")
 
 
+def _operand(g):
+    """A gradient as the operators take it: autograd also hands out expanded ones."""
+    ok = g.stride(-1) == 1 and all(s % 8 == 0 for s in g.stride()[:-1]) and g.data_ptr() % 16 == 0
+    return g if ok else g.contiguous()
+
+
+class _Rope(torch.autograd.Function):
+    """rope under autograd: the map is linear, and its transpose the rotation back."""
+
+    @staticmethod
+    def forward(ctx, q, k, cos_sin, positions, sections, axis_of, interleaved, inverse, layout):
+        ctx.set_materialize_grads(False)
+        ctx.save_for_backward(cos_sin, positions)
+        ctx.kw = dict(sections=sections, axis_of=axis_of, interleaved=interleaved, inverse=not inverse, layout=layout)
+        both = rope(q, k, cos_sin, positions, **dict(ctx.kw, inverse=inverse))
+        ctx.mark_non_differentiable(*(y for x, y in zip((q, k), both) if x is not None and not x.requires_grad))
+        return both
+
+    @staticmethod
+    def backward(ctx, dq, dk):
+        dq, dk = (None if g is None else _operand(g) for g in (dq, dk))
+        if dq is None:
+            dq, dk = (None, None) if dk is None else (None, rope(dk, None, *ctx.saved_tensors, **ctx.kw)[0])
+        else:
+            dq, dk = rope(dq, dk, *ctx.saved_tensors, **ctx.kw)
+        return (dq, dk) + (None,) * 7
+
+
 def rope(q, k, cos_sin, positions, *, sections=None, axis_of=None, interleaved: bool = False, inverse: bool = False,
          layout: Optional[str] = None, out=None, stream=None):
     """Q and K (or None) with their pairs rotated by the tokens' positions.
@@ -124,16 +153,30 @@ def rope(q, k, cos_sin, positions, *, sections=None, axis_of=None, interleaved: 
     turns; ``axis_of`` names the axis of every pair instead.  ``interleaved``:
     pairs (2j, 2j+1) instead of (j, j + rot_dim/2).  Dimensions from rot_dim on
     pass through.  ``out``: the tensors to write, which may be q and k
-    themselves.  Layouts: "thd", "htd", "bshd", "bhsd".
+    themselves (not while autograd records them).  Layouts: "thd", "htd", "bshd",
+    "bhsd".  Differentiable in q and k.
     """
+    if (getattr(q, "requires_grad", False) or getattr(k, "requires_grad", False)) and torch.is_grad_enabled():
+        if out is not None:
+            raise _bad("rope with out= has no gradient, and q or k requires one")
+        if stream is None:
+            return _Rope.apply(q, k, cos_sin, positions, sections, axis_of, interleaved, inverse, layout)
+        here = torch.cuda.current_stream(q.device)
+        with torch.cuda.stream(_fm.named_stream(stream, q.device)):  # the gradient runs there too
+            both = _Rope.apply(q, k, cos_sin, positions, sections, axis_of, interleaved, inverse, layout)
+        for x in both:
+            if x is not None:
+                x.record_stream(here)
+        return both
     q_out, k_out = out if out is not None else (None, None)
     return _call_rope(q, k, cos_sin, positions, sections, axis_of, interleaved, inverse, _layout(q, layout), q_out,
                       k_out, stream)
 
 
 def rope_bwd(dq, dk, cos_sin, positions, **kw):
-    """Gradients of :func:`rope`'s inputs from its outputs': the rotation back
-    (a rotation's transpose), same arguments."""
+    """Gradients of :func:`rope`'s inputs from its outputs', for callers that
+    keep no autograd graph: the rotation back (a rotation's transpose), same
+    arguments."""
     return rope(dq, dk, cos_sin, positions, inverse=True, **kw)
 
 

@@ -95,7 +95,7 @@ _LAYOUTS = {"thd": 0, "htd": 1, "bshd": 2, "bhsd": 3}
 
 def _layout(x, layout: Optional[str]) -> int:
     if layout is None:
-        return 0 if x.dim() == 3 else 2
+        return 0 if getattr(x, "ndim", 4) == 3 else 2  # (what is no tensor is refused by the call)
     try:
         return _LAYOUTS[layout]
     except KeyError:
@@ -145,7 +145,7 @@ class _Rope(torch.autograd.Function):
 
 def rope(q, k, cos_sin, positions, *, sections=None, axis_of=None, interleaved: bool = False, inverse: bool = False,
          layout: Optional[str] = None, out=None, stream=None):
-    """Q and K (or None) with their pairs rotated by the tokens' positions.
+    """Q and K (which may be None) with their pairs rotated by the tokens' positions.
 
     ``positions``: int32 over q's token dimensions (``[total]`` or ``[batch,
     seqlen]``), or ``[axes, ...]`` for positions with several axes (time,

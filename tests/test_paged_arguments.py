@@ -1,0 +1,18 @@
+"""Refusals of the serving operators that need no GPU."""
+import pytest
+import torch
+
+import fmha_native_b200 as fm
+
+
+@pytest.mark.parametrize("layout", [None, "thd", "bshd"])
+def test_operands_that_are_no_tensors(layout):
+    x = torch.zeros(2, 1, 4, 64, dtype=torch.bfloat16)
+    for call in (lambda: fm.rope(None, x, x, x, layout=layout), lambda: fm.rope(3, x, x, x, layout=layout),
+                 lambda: fm.rope_bwd(None, x, x, x, layout=layout),
+                 lambda: fm.paged_append(None, x, x, x, x, x, layout=layout),
+                 lambda: fm.paged_fwd(None, x, x, x, x, layout=layout),
+                 lambda: fm.prefix_fwd([1], x, x, x, 5, x, x, layout=layout)):
+        with pytest.raises(fm.FmhaError) as e:
+            call()
+        assert e.value.status == fm.FMHA_ERR_ARG

@@ -46,13 +46,15 @@ class PagedKV:
         return [self.free.pop() for _ in range(need)]
 
     def extend(self, new: list[int]) -> None:
-        """Makes room for new[i] tokens in slot i; lengths then include them."""
+        """Makes room for new[i] tokens in slot i; lengths then include them.  All of it or none."""
+        need = [-(-(self.host_lengths[i] + n) // self.page) for i, n in enumerate(new)]
+        if max(need) > self.host_table.shape[1]:
+            raise fm.FmhaError(fm.FMHA_ERR_ARG, f"a sequence of {max(need)} pages, {self.host_table.shape[1]} at most")
+        pages = self.pages_for(self.page * sum(max(0, n - len(own)) for n, own in zip(need, self.owned)))
         for i, n in enumerate(new):
-            want = -(-(self.host_lengths[i] + n) // self.page) - len(self.owned[i])
-            if want > 0:
-                for p in self.pages_for(want * self.page):
-                    self.host_table[i, len(self.owned[i])] = p
-                    self.owned[i].append(p)
+            while len(self.owned[i]) < need[i]:
+                self.owned[i].append(pages.pop(0))
+                self.host_table[i, len(self.owned[i]) - 1] = self.owned[i][-1]
             self.host_lengths[i] += n
         self.table.copy_(self.host_table, non_blocking=True)
         self.lengths.copy_(torch.tensor(self.host_lengths, dtype=torch.int32), non_blocking=True)

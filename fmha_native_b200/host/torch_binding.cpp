@@ -332,7 +332,7 @@ PyObject* append(PyObject* const* a) {
     p.total_q = ax.dense ? 0 : p.seqlen_q;
     p.nhead_k = c.heads, p.page_size = c.page, p.num_pages = c.pages, p.max_pages = b.max_pages;
     p.interleaved = truth(a[11]);
-    if (k.numel() > 0) {
+    if (x.tokens > 0 && x.batches > 0) {
         done(g_append(&p, stream.get()), "paged_append");
         written(tensor(a[2], "k_cache"));
         written(tensor(a[3], "v_cache"));

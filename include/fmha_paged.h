@@ -77,7 +77,7 @@ int fmha_rope_d64_bf16(const FmhaRopeParams* params, struct CUstream_st* stream)
 /* New K and V, K rotated, into the pages of the cache; q, if given, rotated
  * into q_out.  A token whose place is negative (a batch slot with fewer keys
  * than new tokens, such as an empty slot) is not stored, and its q_out row is
- * zero.  No two tokens of a call may name the same place. */
+ * zero; so it is with one whose position is outside the angle table.  No two tokens of a call may name the same place. */
 int fmha_paged_append_d64_bf16(const FmhaRopeParams* params, struct CUstream_st* stream);
 
 typedef struct FmhaPagedParams {

@@ -16,3 +16,13 @@ def test_operands_that_are_no_tensors(layout):
         with pytest.raises(fm.FmhaError) as e:
             call()
         assert e.value.status == fm.FMHA_ERR_ARG
+
+
+@pytest.mark.gpu
+def test_a_cache_without_heads_is_refused(cuda_device):
+    """Not answered with a q that nothing wrote."""
+    q = torch.zeros(2, 1, 4, 64, dtype=torch.bfloat16, device="cuda")
+    k, kc = q[:, :, :0], torch.zeros(3, 16, 0, 64, dtype=torch.bfloat16, device="cuda")
+    t, n = torch.zeros(2, 1, dtype=torch.int32, device="cuda"), torch.ones(2, dtype=torch.int32, device="cuda")
+    with pytest.raises(fm.FmhaError):
+        fm.paged_append(k, k, kc, kc, t, n, q=q)

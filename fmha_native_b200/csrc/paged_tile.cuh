@@ -364,16 +364,20 @@ fmha_paged_plan(const __grid_constant__ Args a) {
 
 // Takes the values that are not finite out of rows [lo, hi) of a V tile whose
 // first key is k0, and notes the first key with each kind of them (one warp).
-// (Inline it takes registers from the softmax: 64 tokens under 8192 shared keys 34.5 us, 33.8 so.)
-__device__ __noinline__ void set_aside_odd_values(TileShared& sm, int slot, int k0, int lo, int hi) {
+// (Loops kept small: unrolled they took registers from the softmax, 3 % of the
+// prompt chunks' time.)
+__device__ __forceinline__ void set_aside_odd_values(TileShared& sm, int slot, int k0, int lo, int hi) {
     const int lane = threadIdx.x & 31;
     uint4* v = reinterpret_cast<uint4*>(sm.kv[slot]);
     uint32_t probe = 0;
+#pragma unroll 1
     for (int x = lo * 8 + lane; x < hi * 8; x += 32) probe = probe_bf16(v[x], probe);
     if (!__any_sync(0xffffffffu, probe != 0)) return;
+#pragma unroll 1
     for (int x = lo * 8 + lane; x < hi * 8; x += 32) {
         const int key = x >> 3, col0 = ((x & 7) ^ (key & 7)) * 8;
         const uint16_t* bits = reinterpret_cast<const uint16_t*>(v + x);
+#pragma unroll 1
         for (int e = 0; e < 8; ++e)
             if (!is_finite_bf16(bits[e]))
                 atomicMin(&sm.first_odd[(bits[e] & 0x7f) != 0 ? 0 : bits[e] >> 15 ? 2 : 1][col0 + e], k0 + key);

@@ -30,8 +30,8 @@
 //
 // What bounds it: per key tile a block runs 16384 exponentials against 2 x
 // 128 x 128 x 64 multiply-adds, so the special-function unit (16 per clock)
-// would need twice the tensor pipe's time; an eighth of the exponentials
-// therefore runs as a polynomial on the FMA pipe.  What remains is the chain
+// would need twice the tensor pipe's time; three of sixteen exponentials
+// therefore run as a polynomial on the FMA pipe.  What remains is the chain
 // S -> registers -> P -> tensor memory of each tile, which the SM's other block
 // hides in part.  Measured: 4 sequences of 2048 tokens, 16 heads over 4 K/V
 // heads, no mask, 557 TF/s from pages of 64 keys, 508 of 16 and 421 of 8 (the
@@ -81,9 +81,9 @@ constexpr int kLongRange = 16;
 constexpr int kMostParts = 64;  // ranges of a job (their fold is one block's work per 16 rows)
 // Pairs of every 16 whose exponential runs on the FMA pipe, by a polynomial as
 // exact as the function unit (degree 5), since the row sums and the LSE take it
-// in fp32.  Prompt chunks: 205.6 us; 211.6 with 0, 206.0 with 3, 212.5 with 4 (a
-// polynomial of degree 3, whose 7.5e-5 show in the LSE, 204.2 with 4).
-constexpr int kPolyOf16 = 2;
+// in fp32.  Prompt chunks: 199.6 us; 208.7 with 0, 201.3 with 2, 206.9 with 4 (a
+// polynomial of degree 3, whose 7.5e-5 show in the LSE, 198.2 with 4).
+constexpr int kPolyOf16 = 3;
 
 // A block's work (for one K/V head): range k of the keys of a row tile.
 struct alignas(16) TileItem {

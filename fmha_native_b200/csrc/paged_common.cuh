@@ -231,13 +231,9 @@ __device__ __forceinline__ void drain_phase(uint32_t bar, uint32_t parity, const
         if (globaltimer_ns() - t0 > a.wait_limit_ns) return;
 }
 
-// A page id outside the cache is flagged and becomes -1, which the tensor maps
-// read as zeros (a map has one page at least, also where the cache has none).
-__device__ __forceinline__ int checked_page(const Args& a, int id) {
-    if ((unsigned)id < (unsigned)a.num_pages) return id;
-    flag_index_error(a.err_word);
-    return -1;
-}
+// The tensor maps read zeros for a page id outside the cache.  But they have one
+// page at least, also where the cache has none: then every head is outside.
+__device__ __forceinline__ int no_page_head(const Args& a) { return a.num_pages == 0 ? a.nhead_k : 0; }
 
 // Values that are not finite.  A matrix product hands 0 * inf = NaN to rows that
 // give a key no weight because they do not see it, so where rows differ in what

@@ -26,8 +26,9 @@
 //   arithmetic   mma.sync m16n8k16 with the rows as M: the tile of a decode
 //                step is far too thin for a 128-row tensor-memory tile, and
 //                the reads leave the tensor pipe idle anyway.  P enters the
-//                second product as a sum of two bf16 (value and remainder), so
-//                O keeps fp32 accuracy until its one rounding at the end.
+//                second product as a sum of two bf16 (value and remainder, to
+//                2^-16 of it), so O is rounded once, at its end.  Both are above
+//                0 where P is, so that an infinite V gives an infinite O.
 //
 // Measured (in a graph): 4 sequences of 60 000 to 130 000 keys, 16 K/V heads,
 // 251 us for 1.62 GB (6.4 TB/s, a copy's rate); 64 sequences of 100 to 4095 keys,
@@ -38,8 +39,9 @@
 //
 // Keys past a row's limit get weight 0 by selection, and value rows past the
 // tile's last visible key are zeroed in shared memory before use, so whatever
-// the page holds there (NaN included) stays out of O.  Visible values that are
-// not finite are added to the rows that see them without a product.
+// the page holds there (NaN included) stays out of O.  In units that some rows
+// see in part, values that are not finite are taken out of the product and added
+// to the rows that see them.
 #pragma once
 #include <algorithm>
 
@@ -163,8 +165,40 @@ __device__ __forceinline__ void mma_16816(float (&d)[4], const uint32_t (&a)[4],
         : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
         : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
+// The largest bf16 below x, for x > 0; 0 for 0 (and NaN for NaN).
+__device__ __forceinline__ float below_bf16(float x) {
+    return __uint_as_float((uint32_t)max((int)__float_as_uint(x) - 1, 0) & 0xffff0000u);
+}
 __device__ __forceinline__ void fence_async_smem() {
     asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+}
+
+// Takes the values that are not finite out of the V of a unit of `keys` keys, and
+// notes them in the bits of the o[n][q] (m16n8 fragments of the lane's rows, which
+// see seen0 and seen1 of the keys) that they belong to.  One warp, which fences.
+__device__ __forceinline__ void note_odd_values(uint4* v, int keys, int seen0, int seen1, uint32_t (&odd)[3]) {
+    const int lane = threadIdx.x & 31;
+    uint32_t probe = 0;
+#pragma unroll 1
+    for (int i = lane; i < keys * 8; i += 32) probe = probe_bf16(v[i], probe);
+    if (!__any_sync(0xffffffffu, probe != 0)) return;
+#pragma unroll 1
+    for (int x = 0; x < keys * 8; ++x) {
+        const int key = x >> 3, n = x & 7;
+        const uint32_t pair = reinterpret_cast<const uint32_t*>(v + key * 8 + (n ^ (key & 7)))[lane & 3];
+#pragma unroll 1
+        for (int q = 0; q < 4; ++q) {
+            const uint32_t bits = q & 1 ? pair >> 16 : pair & 0xffffu;
+            if (is_finite_bf16(bits) || key >= (q < 2 ? seen0 : seen1)) continue;
+            const uint32_t bit = 1u << (4 * n + q);
+            if ((bits & 0x7fu) != 0) odd[0] |= bit;
+            else if ((bits & 0x8000u) == 0) odd[1] |= bit;
+            else odd[2] |= bit;
+        }
+    }
+    __syncwarp();
+#pragma unroll 1
+    for (int i = lane; i < keys * 8; i += 32) v[i] = finite_bf16(v[i]);
 }
 
 // Row rt of a result, columns [4 c4, 4 c4 + 4): into the final rows or the
@@ -262,6 +296,7 @@ fmha_paged_rows_kernel(const __grid_constant__ Args a) {
     const int group_blocks = a.group_blocks, heads = a.group_heads;
     const int group = (int)blockIdx.x / group_blocks, index = (int)blockIdx.x - group * group_blocks;
     const int head0 = group * heads;
+    const int map_head0 = head0 + no_page_head(a);
     const unsigned cost_mine = mine + mine_n * kSeqCost;
     before += before_n * kSeqCost;
     total += total_n * kSeqCost;
@@ -414,9 +449,9 @@ fmha_paged_rows_kernel(const __grid_constant__ Args a) {
                     __syncwarp();
                     if (lane < nbox) {
                         const uint32_t dst = ring0 + fill * (2 * kUnitBytes) + (lane << (box_shift + 7));
-                        const int page = checked_page(a, id);
-                        load_page_box(dst, &a.tm_k, bar, key0 & page_mask, head0 + p.h, page, policy);
-                        load_page_box(dst + kUnitBytes, &a.tm_v, bar, key0 & page_mask, head0 + p.h, page, policy);
+                        if ((unsigned)id >= (unsigned)a.num_pages) flag_index_error(a.err_word);
+                        load_page_box(dst, &a.tm_k, bar, key0 & page_mask, map_head0 + p.h, id, policy);
+                        load_page_box(dst + kUnitBytes, &a.tm_v, bar, key0 & page_mask, map_head0 + p.h, id, policy);
                     }
                     ++issued;
                     fill = fill == kRowStages - 1 ? 0 : fill + 1;
@@ -442,11 +477,13 @@ fmha_paged_rows_kernel(const __grid_constant__ Args a) {
         float o[8][4], m[2], l[2];
         int lim[2];
         int u0 = 0;
+        uint32_t odd[3];  // bit 4 n + q: NaN, +inf or -inf among the values that belong to o[n][q]
         bool ok = true;
         for (long long it = 0; it < count; ++it) {
             const int rows = c.x.count * a.group;
             if (it == 0 || c.u == 0) {
                 u0 = c.u;
+                odd[0] = odd[1] = odd[2] = 0;
 #pragma unroll
                 for (int hr = 0; hr < 2; ++hr) {
                     const int r = hr * 8 + g;
@@ -483,16 +520,15 @@ fmha_paged_rows_kernel(const __grid_constant__ Args a) {
                 const uint32_t vs = smem_u32(sm.ring[warp][slot][1]);
                 const int key0 = (c.unit0 + c.u) * kUnit;
                 const int valid = c.x.kv_end - key0;
-                if (valid < kUnit) {
+                // (The first token sees the fewest keys.)
+                const int all_see = key_limit(a, Sequence{c.x.first, c.x.count, c.x.keys}, 0) - key0;
+                if (all_see < kUnit) {  // some rows see only a part of the unit
                     uint4* v = reinterpret_cast<uint4*>(sm.ring[warp][slot][1]);
                     for (int i = valid * 8 + lane; i < kUnit * 8; i += 32) v[i] = make_uint4(0, 0, 0, 0);
+                    if (all_see < min(valid, kUnit)) note_odd_values(v, min(valid, kUnit), lim[0] - key0, lim[1] - key0, odd);
                     fence_async_smem();  // ordered before the slot's next TMA write
                     __syncwarp();
                 }
-                uint32_t probe = 0;
-#pragma unroll
-                for (int i = 0; i < kUnit * 8; i += 32)
-                    probe = probe_bf16(reinterpret_cast<const uint4*>(sm.ring[warp][slot][1])[i + lane], probe);
                 // S = Q K^T
                 float s[4][4];
 #pragma unroll
@@ -542,11 +578,9 @@ fmha_paged_rows_kernel(const __grid_constant__ Args a) {
                         const float p0 = ex2_approx(fmaf(s[n][2 * hr], a.scale, -mu));
                         const float p1 = ex2_approx(fmaf(s[n][2 * hr + 1], a.scale, -mu));
                         sum += p0 + p1;
-                        const uint32_t hi = pack_bf16_rne(p0, p1);
-                        ph[n >> 1][hr + 2 * (n & 1)] = hi;
-                        pl[n >> 1][hr + 2 * (n & 1)] =
-                            pack_bf16_rne(p0 - __uint_as_float(hi << 16),
-                                          p1 - __uint_as_float(hi & 0xffff0000u));
+                        const float h0 = below_bf16(p0), h1 = below_bf16(p1);
+                        ph[n >> 1][hr + 2 * (n & 1)] = pack_bf16_trunc(h0, h1);
+                        pl[n >> 1][hr + 2 * (n & 1)] = pack_bf16_rne(p0 - h0, p1 - h1);
                     }
                     l[hr] = l[hr] * keep + sum;
 #pragma unroll
@@ -556,26 +590,6 @@ fmha_paged_rows_kernel(const __grid_constant__ Args a) {
                     }
                 }
                 // O += P V
-                if (__any_sync(0xffffffffu, probe != 0)) {
-                    // (Also where all rows see them: the remainder of a weight may be 0 or negative.)
-                    for (int key = 0; key < min(valid, kUnit); ++key)
-#pragma unroll
-                        for (int n = 0; n < 8; ++n) {
-                            const uint32_t pair = *reinterpret_cast<const uint32_t*>(
-                                sm.ring[warp][slot][1] + key * 128 + ((n ^ (key & 7)) << 4) + 4 * t4);
-#pragma unroll
-                            for (int q = 0; q < 4; ++q) {
-                                const uint32_t bits = q & 1 ? pair >> 16 : pair & 0xffffu;
-                                if (!is_finite_bf16(bits) && key0 + key < lim[q >> 1])
-                                    o[n][q] += __uint_as_float(bits << 16);
-                            }
-                        }
-                    __syncwarp();
-                    uint4* v = reinterpret_cast<uint4*>(sm.ring[warp][slot][1]);
-                    for (int i = lane; i < kUnit * 8; i += 32) v[i] = finite_bf16(v[i]);
-                    fence_async_smem();  // ordered before the slot's next TMA write
-                    __syncwarp();
-                }
 #pragma unroll
                 for (int st = 0; st < 2; ++st)
 #pragma unroll
@@ -616,6 +630,13 @@ fmha_paged_rows_kernel(const __grid_constant__ Args a) {
                             *reinterpret_cast<float2*>(po + rt * kHeadDim + n * 8 + 2 * t4) =
                                 make_float2(o[n][2 * hr], o[n][2 * hr + 1]);
                         if (t4 == 0) *reinterpret_cast<float2*>(pml + rt * 2) = make_float2(m[hr], lt);
+                    }
+                    for (uint32_t left = odd[0] | odd[1] | odd[2]; left != 0; left &= left - 1) {
+                        const int i = __ffs(left) - 1;
+                        float* x = po + ((i >> 1 & 1) * 8 + g) * kHeadDim + (i >> 2) * 8 + 2 * t4 + (i & 1);
+                        if (odd[0] >> i & 1) *x = NAN;
+                        if (odd[1] >> i & 1) *x += INFINITY;
+                        if (odd[2] >> i & 1) *x -= INFINITY;
                     }
                     __syncwarp();
                 }

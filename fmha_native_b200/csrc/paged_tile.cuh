@@ -484,8 +484,9 @@ fmha_paged_tile_kernel(const __grid_constant__ Args a) {
         if (lane == 0) mbar_arrive_expect_tx(bar, boxes * box_rows * kHeadDim * 2);
         __syncwarp();
         if (lane < boxes) {
+            if (page < 0 || page >= a.num_pages) flag_index_error(a.err_word);
             load_page_box(smem_u32(sm.kv[slot]) + lane * box_rows * kHeadDim * 2, (i & 1) ? &a.tm_v : &a.tm_k, bar,
-                          (key0 + lane * box_rows) & ((1 << a.page_shift) - 1), kvh, checked_page(a, page), policy);
+                          (key0 + lane * box_rows) & ((1 << a.page_shift) - 1), kvh + no_page_head(a), page, policy);
         }
     };
     constexpr int kAhead = kTileStages / 2;  // tiles loaded before the block starts

@@ -22,7 +22,7 @@ using namespace fmha_paged;
 // the tile kernel's blocks shared, by the others.  One kernel for both saves a
 // launch (50 sequences of 3 to 12 tokens: 20.2 -> 19.5 us); where there is only
 // the merge, the fold's registers would cost more (64 sequences of 100 to 4095
-// keys: 43.8 us with it, 42.4 without).
+// keys: 3 % longer with it).
 constexpr int kEndThreads = 256;
 template <bool kMerge, bool kCombine>
 __global__ void __launch_bounds__(kEndThreads)

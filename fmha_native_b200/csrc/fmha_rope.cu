@@ -16,8 +16,8 @@
 //
 // What bounds them is memory; the step to a copy's rate is the angles, gathered
 // per token, and for the append the scattered pages.  Measured (in a graph):
-// 30011 tokens of 16 + 16 heads with three axes, there and back, 96 us for 497 MB
-// (5.2 TB/s, 80 % of a copy's rate); 32k prompt tokens of 16 + 4 + 4 heads into
+// 30011 tokens of 16 + 16 heads with three axes, there and back, 95 us for 497 MB
+// (5.2 TB/s, 81 % of a copy's rate); 32k prompt tokens of 16 + 4 + 4 heads into
 // pages of 64, 45 us for 199 MB (4.4 TB/s); 16 tokens of 8 + 2 heads 2.5 us,
 // which is a launch.
 #include <cuda_runtime.h>

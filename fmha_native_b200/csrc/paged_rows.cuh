@@ -31,11 +31,15 @@
 //                0 where P is, so that an infinite V gives an infinite O.
 //
 // Measured (in a graph): 4 sequences of 60 000 to 130 000 keys, 16 K/V heads,
-// 251 us for 1.62 GB (6.4 TB/s, a copy's rate); 64 sequences of 100 to 4095 keys,
-// 32 heads over 8, 41 us for 172 MB (4.2 TB/s: start, first loads and fold are
-// about 12 us of it); one sequence of 776 keys 9.1 us, which is two launches in
-// line.  The tile kernel, which could take these rows too: 282, 59 and 11.3 us.  (A tensor map that promotes its reads to 256 bytes in L2 made it
-// fetch twice what it used.)
+// 250 us for 1.62 GB (6.5 TB/s, a copy's rate; 254 in a long loop, under the power
+// limit); 64 sequences of 100 to 4095 keys, 32 heads over 8, 41 us for 172 MB (4.2
+// TB/s: start, first loads and fold are about 12 us of it); one sequence of 776
+// keys 9.1 us, which is two launches in line.  The tile kernel, which could take
+// these rows too, took 12, 44 and 24 % longer.  (A tensor map that promotes its
+// reads to 256 bytes in L2 made it fetch twice what it used.)
+//
+// Below, where a choice was measured, each pair of figures is of one state of the
+// code: what counts is their ratio.
 //
 // Keys past a row's limit get weight 0 by selection, and value rows past the
 // tile's last visible key are zeroed in shared memory before use, so whatever
@@ -64,18 +68,18 @@ constexpr int kMostRows = 16;
 constexpr int kRowStages = 3;
 // A sequence's start and end in a block cost about as much time as this many
 // units (its first loads, Q, the results), and the shares count them: 64 sequences
-// of 100 to 4095 keys 41 us, 43 without; 111 of none or one under a prefix of 335
-// 13 us, 17 without.
+// of 100 to 4095 keys take 5 % longer without, 111 of none or one under a prefix of
+// 335 a third longer.
 constexpr int kSeqCost = 5;
 
 // Groups of blocks that share out the K/V heads: each group works on all keys.
 // More heads a block keep more neighbouring memory together, more groups make
 // longer ranges, and so fewer pieces to fold; what the pieces weigh depends on
 // the rows.  Per group about 8 heads for 1 or 2 rows (4 sequences of 60 000 to
-// 130 000 keys, 16 heads: 248 us, 265 with one group, 260 with 4 heads), 4 for up
-// to 8 (64 sequences of 100 to 4095 keys, 8 heads of 4 rows: 41.0 us, 42.3 with
-// one group), 2 beyond (one sequence of 16384 keys, 32 heads of 16 rows: 32 us, 87
-// with one group, 36 with 8 heads).
+// 130 000 keys, 16 heads: 7 % longer with one group, 5 % with 4 heads), 4 for up
+// to 8 (64 sequences of 100 to 4095 keys, 8 heads of 4 rows: 3 % longer with one
+// group), 2 beyond (one sequence of 16384 keys, 32 heads of 16 rows: 32 us, 87 with
+// one group, 36 with 8 heads).
 constexpr int kMostGroups = 16;
 inline int head_groups(int nhead_k, int rows) {
     const int least = rows <= 2 ? 8 : rows <= 8 ? 4 : 2;

@@ -34,13 +34,12 @@
 // therefore run as a polynomial on the FMA pipe.  What remains is the chain
 // S -> registers -> P -> tensor memory of each tile, which the SM's other block
 // hides in part.  Measured: 4 sequences of 2048 tokens, 16 heads over 4 K/V
-// heads, no mask, 557 TF/s from pages of 64 keys, 508 of 16 and 421 of 8 (the
-// dense kernel: 650); 6 prompt chunks of 513 to 2048 tokens over up to 8191
-// keys, 198 us; the kernel alone, with cold caches, 204: tensor pipe
-// 30 % busy, special functions 49 %, issue slots 54 %.  One thread per row took
-// 216 us there instead of 209 with two, blocks of 64 keys a tile (three to an
-// SM) 280 to 315, an arrival per warp instead of per thread at the barriers of
-// S and P 4 to 6 % more.
+// heads, no mask, 579 TF/s from pages of 64 keys, 522 of 16 and 434 of 8 (the
+// dense kernel: 702); 6 prompt chunks of 513 to 2048 tokens over up to 8191
+// keys, 200 us (118 GFLOP); the kernel alone, with cold caches, 205: tensor pipe
+// 30 % busy, special functions 52 %, issue slots 52 %.  There one thread per row
+// took 3 % longer than two, blocks of 64 keys a tile (three to an SM) 30 to 47 %,
+// an arrival per warp instead of per thread at the barriers of S and P 4 to 6 %.
 //
 // Work split.  A shared prefix has one length, so the host cuts every row
 // tile's keys into `splits` equal ranges, a block each, and whatever ends the
@@ -50,7 +49,7 @@
 // all of them busy (kPlanHere: 24 sequences of 5 tokens, 24 heads over 4, 200 to
 // 3001 keys 17 us, with a list 26); with more, a first kernel writes the list of
 // whole tiles, cutting only what is far longer than the rest (kPlanList: the
-// prompt chunks 205 us, 213 with every block planning for itself).  Jobs of one
+// prompt chunks take 4 % longer with every block planning for itself).  Jobs of one
 // range go to the output, the others through scratch slots that fmha_paged_end
 // folds.
 #pragma once
@@ -75,14 +74,14 @@ constexpr uint32_t kColS = 0, kColO = 128, kColP = 192;
 constexpr int kTileRegsSoftmax = 96, kTileRegsControl = 48;
 static_assert(256 * kTileRegsSoftmax + 128 * kTileRegsControl <= kTileThreads * 80, "register split");
 constexpr float kLazyLog2 = 8.0f;
-// Key tiles up to which a job is not worth cutting where jobs abound (prompt chunks:
-// 198 us; 220 with no job cut, however long; 198 with 8).
+// Key tiles up to which a job is not worth cutting where jobs abound (prompt chunks
+// take 11 % longer with no job cut, however long; as long with 8).
 constexpr int kLongRange = 16;
 constexpr int kMostParts = 64;  // ranges of a job (their fold is one block's work per 16 rows)
 // Pairs of every 16 whose exponential runs on the FMA pipe, by a polynomial as
 // exact as the function unit (degree 5), since the row sums and the LSE take it
-// in fp32.  Prompt chunks: 199.6 us; 208.7 with 0, 201.3 with 2, 206.9 with 4 (a
-// polynomial of degree 3, whose 7.5e-5 show in the LSE, 198.2 with 4).
+// in fp32.  Prompt chunks: 200 us; 5 % longer with 0, 1 % with 2, 4 % with 4 (a
+// polynomial of degree 3, whose 7.5e-5 show in the LSE: 1 % shorter with 4).
 constexpr int kPolyOf16 = 3;
 
 // A block's work (for one K/V head): range k of the keys of a row tile.

@@ -21,14 +21,19 @@
  *     (after the first on a device), so calls may be captured in CUDA graphs.
  *   - Limits: tokens * nhead_q and the 32-key units of batch * max_pages pages
  *     below 2^31; nhead_q at most 8192; strides below 2^39.
+ *   - O is rounded to bf16 once.  Sequences of up to 16 rows (new tokens x query
+ *     heads of a K/V head's group) carry the softmax weights to 2^-16 of
+ *     themselves before that; for more rows, and for all keys of a shared
+ *     prefix, they are rounded to bf16 as well.  The LSE is fp32 throughout.
  *   - seqstart_q should cover tokens 0 .. total_q - 1; a token outside every
  *     sequence is not worked on: append reports it and zeroes its row of q_out,
  *     the attention leaves its row of o unwritten.
  *   - Returns an FMHA_* status.  Bad values that only the device can see (a
  *     page id outside the cache, a length past the page table, a position
  *     outside the angle table, prefix sums that decrease or leave the tokens, more
- *     new tokens in a sequence than seqlen_q) access no memory out of range
- *     and are reported once by fmha_fwd_d64_status as FMHA_ERR_INDEX.
+ *     new tokens in a sequence than seqlen_q) access no memory out of range (rows
+ *     of overlapping sequences may be left unwritten) and are reported once by
+ *     fmha_fwd_d64_status as FMHA_ERR_INDEX.
  */
 #ifndef FMHA_PAGED_H
 #define FMHA_PAGED_H

@@ -20,8 +20,8 @@ seqlen_q, heads, 64]``) or packed (``[total, heads, 64]`` with int32
 names (its handle, an integer), allocate only through torch and on that stream,
 read nothing back, and may be captured in CUDA graphs after a first call on the
 device.  :func:`rope` is differentiable; the cache's operators are for serving,
-and their results have no gradient.  Index data that only the device can check is reported by
-``fmha_native_b200.status()`` as ``FMHA_ERR_INDEX``.
+and their results have no gradient.  Index data that only the device can check
+is reported by ``fmha_native_b200.status()`` as ``FMHA_ERR_INDEX``.
 """
 from __future__ import annotations
 
@@ -159,7 +159,7 @@ def rope(q, k, cos_sin, positions, *, sections=None, axis_of=None, interleaved: 
     if (getattr(q, "requires_grad", False) or getattr(k, "requires_grad", False)) and torch.is_grad_enabled():
         if out is not None:
             raise _bad("rope with out= has no gradient, and q or k requires one")
-        if stream is None:
+        if stream is None or not isinstance(q, torch.Tensor):
             return _Rope.apply(q, k, cos_sin, positions, sections, axis_of, interleaved, inverse, layout)
         here = torch.cuda.current_stream(q.device)
         with torch.cuda.stream(_fm.named_stream(stream, q.device)):  # the gradient runs there too

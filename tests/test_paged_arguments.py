@@ -26,3 +26,10 @@ def test_a_cache_without_heads_is_refused(cuda_device):
     t, n = torch.zeros(2, 1, dtype=torch.int32, device="cuda"), torch.ones(2, dtype=torch.int32, device="cuda")
     with pytest.raises(fm.FmhaError):
         fm.paged_append(k, k, kc, kc, t, n, q=q)
+
+
+def test_no_q_beside_a_k_that_requires_a_gradient():
+    x = torch.zeros(2, 1, 4, 64, dtype=torch.bfloat16)
+    for stream in (None, 12345):
+        with pytest.raises(fm.FmhaError):
+            fm.rope(None, x.clone().requires_grad_(), x, x, stream=stream)
